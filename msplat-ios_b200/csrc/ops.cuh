@@ -1,0 +1,173 @@
+// ops.cuh — what the kernels behind include/msplat_ops.h share: element types,
+// the description of one matrix product with its epilogue, and the launchers.
+#pragma once
+#include <cstdint>
+#include <stdexcept>
+#include <string>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include "msplat_backend.h"
+#include "msplat_ops.h"
+#include "kernels.cuh"
+
+namespace msplat {
+namespace ops {
+
+struct Error : std::runtime_error {
+    int code;
+    Error(int c, const std::string& m) : std::runtime_error(m), code(c) {}
+};
+
+#define OPS_CK(call)                                                                                \
+    do {                                                                                            \
+        cudaError_t e_ = (call);                                                                    \
+        if (e_ != cudaSuccess)                                                                      \
+            throw ::msplat::ops::Error(MSPLAT_ERR_CUDA, std::string(#call) + ": " + cudaGetErrorString(e_)); \
+    } while (0)
+
+inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+inline int64_t round_up(int64_t a, int64_t b) { return ceil_div(a, b) * b; }
+inline int dtype_size(int dtype) { return dtype == MSPLAT_DTYPE_F32 ? 4 : 2; }
+constexpr int kSMs = 148;
+
+template <typename T>
+__device__ __forceinline__ float to_f32(T v);
+template <>
+__device__ __forceinline__ float to_f32<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ float to_f32<__half>(__half v) { return __half2float(v); }
+template <>
+__device__ __forceinline__ float to_f32<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T>
+__device__ __forceinline__ T from_f32(float v);
+template <>
+__device__ __forceinline__ float from_f32<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+
+__device__ __forceinline__ float activate(float z, int act) {
+    switch (act) {
+        case MSPLAT_ACT_RELU: return z > 0.f ? z : (z != z ? z : 0.f);
+        case MSPLAT_ACT_GELU: return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
+        case MSPLAT_ACT_SILU: return z / (1.f + __expf(-z));
+        case MSPLAT_ACT_SIGMOID: return 1.f / (1.f + __expf(-z));
+        default: return z;
+    }
+}
+// act'(z)
+__device__ __forceinline__ float act_slope(float z, int act) {
+    switch (act) {
+        case MSPLAT_ACT_RELU: return z > 0.f ? 1.f : 0.f;
+        case MSPLAT_ACT_GELU:
+            return fmaf(z * 0.3989422804014327f, __expf(-0.5f * z * z),
+                        0.5f * (1.f + erff(z * 0.70710678118654752f)));
+        case MSPLAT_ACT_SILU: {
+            const float q = 1.f / (1.f + __expf(-z));
+            return q * fmaf(z, 1.f - q, 1.f);
+        }
+        case MSPLAT_ACT_SIGMOID: {
+            const float q = 1.f / (1.f + __expf(-z));
+            return q * (1.f - q);
+        }
+        default: return 1.f;
+    }
+}
+
+// What a matrix product does with its result.
+enum EpiKind {
+    kEpiLinear = 0,  // bias, activation, residual; element type T or float
+    kEpiSlab = 1,    // float partial sums: slab[split][row][col] = or += result
+    kEpiStats = 2,   // per row and column block: max and sum of exp of the logits; the label's logit
+    kEpiGrad = 3,    // (softmax - one-hot), times g_scale, in T
+};
+
+// C[i, j] = sum_r A(i, r) B(j, r), i < M, j < N, r < R.
+// A(i, r) = a_mn ? A[r * lda + i] : A[i * lda + r], B(j, r) likewise.
+struct Product {
+    int64_t M, N, R;
+    const void* A;
+    const void* B;
+    int64_t lda, ldb;
+    bool a_mn, b_mn;
+    int dtype;
+    int epi;
+    // kEpiLinear
+    const void* bias;
+    int act;
+    const void* residual;
+    int64_t ldr;
+    void* preact;
+    int64_t ldz;
+    void* out;          // kEpiLinear, kEpiGrad
+    int64_t ldo;
+    int out_dtype;
+    float alpha;              // times the product (kEpiLinear)
+    const float* alpha_dev;   // times this, when not null
+    // kEpiSlab: R is cut into `splits` pieces of `split_len`
+    float* slab;
+    int splits;
+    int64_t split_len;
+    int accumulate;
+    // labels: rows (kEpiStats, kEpiGrad, kEpiLinear for dx) without one count
+    // for nothing; with label_reduces the labels belong to r and unlabelled r
+    // are read as zeros of B
+    const int32_t* targets;
+    int64_t labels;     // number of labels
+    int label_reduces;
+    int64_t col0;       // label of column 0 of this piece
+    float logit_scale;
+    float g_scale;
+    float2* stats;            // [column blocks of the whole table][stats_ld]
+    int64_t stats_ld;
+    int64_t stats_block0;     // first column block of this piece
+    float* label_logit;       // [M]
+    const float* lse;         // [M], in units of log2
+};
+
+// Width of the column blocks that kEpiStats reduces over.
+int stats_block(const Product& p);
+
+void launch_product(const Product& p, cudaStream_t s);
+void launch_product_simt(const Product& p, cudaStream_t s);
+
+// dz = dy act'(z) (dz may be null) and the column sums of dz in pieces of
+// rows: partial[piece][n]. Returns the number of pieces.
+int dz_pieces(int64_t m, int64_t n);
+void launch_dz(int64_t m, int64_t n, const void* z, int64_t ldz, int act, const void* dy, int64_t lddy, void* dz,
+               int64_t lddz, float* partial, int dtype, cudaStream_t s);
+// out[i, j] = alpha * sum_p slab[p][i][j]
+void launch_slab_sum(int64_t rows, int64_t cols, const float* slab, int pieces, void* out, int64_t ldo, float alpha,
+                     const float* alpha_dev, const int32_t* targets, int64_t labels, int dtype, cudaStream_t s);
+// Joins the column blocks' statistics of m rows into lse (log2 units) and
+// row_loss; partial[block] = (sum of the labelled rows' losses, their number).
+struct JoinArgs {
+    int64_t m, blocks;
+    const float2* stats;
+    int64_t stats_ld;
+    const float* label_logit;
+    const int32_t* targets;
+    int64_t labels;
+    float* lse;
+    float* row_loss;
+    double* partial;      // [join_blocks(m)][2]
+};
+int join_blocks(int64_t m);
+void launch_join(const JoinArgs& a, cudaStream_t s);
+// loss = weight * mean, *alpha = factor / number of labelled rows (both 0
+// without any), from all the partial sums.
+void launch_loss_total(const double* partial, int blocks, float weight, float factor, float* loss, float* alpha,
+                       cudaStream_t s);
+
+void launch_dropout(int64_t rows, int64_t cols, const void* x, int64_t ldx, const void* residual, int64_t ldr, void* y,
+                    int64_t ldy, uint32_t below, float scale, uint64_t seed, uint64_t offset,
+                    const uint64_t* offset_dev, int dtype, cudaStream_t s);
+
+}  // namespace ops
+}  // namespace msplat
