@@ -114,6 +114,12 @@ int msplat_loss_cross_entropy(int64_t m, int64_t v, int64_t d, const void* x, in
                               float* row_loss, void* dx, int64_t lddx, void* dw, int64_t lddw, int32_t dtype,
                               void* workspace, uint64_t workspace_bytes, void* stream);
 
+/* Waits for `stream`, then MSPLAT_OK, or MSPLAT_ERR_CUDA when a kernel of this
+ * file gave up waiting for its own copies or products since the last call (its
+ * waits are bounded; its results are then not valid). Not for use while a
+ * stream is being captured. */
+int msplat_ops_status(void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,6 +1,7 @@
 // ops.cuh — what the kernels behind include/msplat_ops.h share: element types,
 // the description of one matrix product with its epilogue, and the launchers.
 #pragma once
+#include <algorithm>
 #include <cstdint>
 #include <stdexcept>
 #include <string>
@@ -131,11 +132,16 @@ struct Product {
     const float* lse;         // [M], in units of log2
 };
 
-// Width of the column blocks that kEpiStats reduces over.
-int stats_block(const Product& p);
+// Column blocks that a kEpiStats product leaves statistics of; at most
+// stats_blocks_most(N) for any type and alignment.
+int64_t stats_blocks(const Product& p);
+inline int64_t stats_blocks_most(int64_t n) { return 2 * ceil_div(n, 128); }
 
 void launch_product(const Product& p, cudaStream_t s);
 void launch_product_simt(const Product& p, cudaStream_t s);
+bool can_product_tc16(const Product& p);
+void launch_product_tc16(const Product& p, cudaStream_t s);
+bool gave_up_tc16(cudaStream_t s);
 
 // dz = dy act'(z) (dz may be null) and the column sums of dz in pieces of
 // rows: partial[piece][n]. Returns the number of pieces.

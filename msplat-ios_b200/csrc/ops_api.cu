@@ -129,9 +129,7 @@ struct LossPlan {
     char* g = nullptr;
     float *slab_x = nullptr, *slab_w = nullptr;
     LossPlan(Arena& a, int64_t m, int64_t v, int64_t d, bool grad, int dtype) {
-        Product p{};
-        p.M = m; p.N = v; p.R = d; p.dtype = dtype; p.epi = kEpiStats;
-        blocks = ceil_div(v, stats_block(p));
+        blocks = stats_blocks_most(v);
         stats_rows = round_up(std::max<int64_t>(kStatsBytes / (8 * blocks), 1), 256);
         if (stats_rows > m) stats_rows = m;
         alpha = a.take<float>(1);
@@ -198,6 +196,13 @@ using namespace msplat;
 using namespace msplat::ops;
 
 extern "C" {
+
+int msplat_ops_status(void* stream) {
+    return guarded([&] {
+        if (gave_up_tc16(static_cast<cudaStream_t>(stream)))
+            throw Error(MSPLAT_ERR_CUDA, "a kernel gave up waiting: the results since the last call are not valid");
+    });
+}
 
 int msplat_linear_forward(int64_t m, int64_t n, int64_t k, const void* x, int64_t ldx, const void* w, int64_t ldw,
                           const void* bias, int32_t activation, const void* residual, int64_t ldr, void* preact,
@@ -389,7 +394,7 @@ int msplat_loss_cross_entropy(int64_t m, int64_t v, int64_t d, const void* x, in
             p.label_logit = plan.label_logit + r0;
             launch_product(p, s);
             JoinArgs j{};
-            j.m = rows; j.blocks = plan.blocks;
+            j.m = rows; j.blocks = stats_blocks(p);
             j.stats = plan.stats; j.stats_ld = plan.stats_rows;
             j.label_logit = plan.label_logit + r0;
             j.targets = targets + r0; j.labels = v;

@@ -52,12 +52,17 @@ __global__ void __launch_bounds__(256) k_join(JoinArgs a) {
     __shared__ double ssum[256], scount[256];
     double sum = 0, count = 0;
     for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < a.m; i += gridDim.x * 256ll) {
+        // a block whose sum is 0 (columns beyond the last, or logits of -inf
+        // only) has no reference; a sum of NaN counts
         float top = -INFINITY;
-        for (int64_t b = 0; b < a.blocks; ++b) top = fmaxf(top, a.stats[b * a.stats_ld + i].x);
+        for (int64_t b = 0; b < a.blocks; ++b) {
+            const float2 v = a.stats[b * a.stats_ld + i];
+            if (v.y != 0.f) top = fmaxf(top, v.x);
+        }
         float total = 0.f;
         for (int64_t b = 0; b < a.blocks; ++b) {
             const float2 v = a.stats[b * a.stats_ld + i];
-            total += v.y * exp2f(v.x - top);
+            if (v.y != 0.f) total += v.y * exp2f(v.x - top);
         }
         const float lse = top + log2f(total);
         const int32_t t = a.targets[i];

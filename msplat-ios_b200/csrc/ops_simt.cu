@@ -104,7 +104,7 @@ __global__ void __launch_bounds__(256) k_product_simt(const __grid_constant__ Pr
                     if (j0 + tx * 4 + x < p.N) sum += exp2f(acc[y][x] - ref);
                 for (int o = 8; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
                 if (in && tx == 0)
-                    p.stats[(p.stats_block0 + blockIdx.x % tiles_n) * p.stats_ld + i] = make_float2(ref, sum);
+                    p.stats[(p.stats_block0 + blockIdx.x % tiles_n) * p.stats_ld + i] = make_float2(top, sum);
             } else if (in) {
                 const bool zero = !labelled(p, i);
                 const float lse = p.lse[i];
@@ -146,8 +146,14 @@ void launch_product_simt(const Product& p, cudaStream_t s) {
         typed<__nv_bfloat16>(p, s);
 }
 
-int stats_block(const Product&) { return kTileN; }
-void launch_product(const Product& p, cudaStream_t s) { launch_product_simt(p, s); }
+int64_t stats_blocks(const Product& p) {
+    if (!can_product_tc16(p)) return ceil_div(p.N, kTileN);
+    return 2 * ceil_div(p.N, p.N > 128 ? 256 : p.N > 64 ? 128 : 64);  // halves of a tile
+}
+void launch_product(const Product& p, cudaStream_t s) {
+    if (can_product_tc16(p)) return launch_product_tc16(p, s);
+    launch_product_simt(p, s);
+}
 
 }  // namespace ops
 }  // namespace msplat

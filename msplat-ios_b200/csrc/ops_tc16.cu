@@ -1,0 +1,308 @@
+// ops_tc16.cu — products of 16-bit matrices on the 5th-generation tensor cores.
+//
+// A block owns a 128 x bn tile of the result at a time (bn 64, 128 or 256) and
+// walks the tiles of its SM. Warp 0 brings 64 columns of the reduction per stage
+// with TMA (128-byte swizzle, out-of-range elements read as zeros, so no size is
+// special); warp 1 issues tcgen05.mma from shared memory into one of two
+// accumulators in TMEM; warps 4-11 read the other accumulator, 32 lanes x 32
+// columns at a time, and do the end of the product while the next tile runs.
+// Either operand may have the reduction across its rows (dx, dw): TMA then
+// brings boxes of 64 x 64 and the instruction reads them transposed, so no
+// operand is ever copied into another layout.
+#include "ops_tc.cuh"
+
+namespace msplat {
+namespace ops {
+
+namespace {
+
+constexpr int kThreads = 384;
+constexpr int kMaxStages = 8;
+
+struct Smem {
+    uint64_t full[kMaxStages], empty[kMaxStages];
+    uint64_t acc_full[2], acc_empty[2], drain;
+    uint32_t tmem;
+    int gave_up;
+};
+
+__device__ __forceinline__ void tile_of(const Product& p, const Tiles& tl, int w, int& tm, int& tn, int& split,
+                                        int64_t& r0, int64_t& r1) {
+    const int per = tl.tiles_m * tl.tiles_n;
+    split = w / per;
+    w -= split * per;
+    tm = w / tl.tiles_n;
+    tn = w - tm * tl.tiles_n;
+    r0 = 0;
+    r1 = p.R;
+    if (p.epi == kEpiSlab) {
+        r0 = split * p.split_len;
+        r1 = min(p.R, r0 + p.split_len);
+    }
+}
+
+template <typename T, int EPI>
+__global__ void __launch_bounds__(kThreads, 1)
+    k_product_tc16(const __grid_constant__ Product p, const __grid_constant__ Tiles tl,
+                   const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b) {
+    extern __shared__ __align__(1024) uint8_t dyn[];
+    __shared__ Smem sm;
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    uint8_t* tiles = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(dyn) + 1023) & ~(uintptr_t)1023);
+    float* staging = reinterpret_cast<float*>(tiles + (size_t)tl.stages * tl.stage_bytes);
+    const uint32_t tmem_cols = 2 * tl.bn;
+
+    if (threadIdx.x == 0) {
+        for (int q = 0; q < tl.stages; ++q) {
+            mbar_init(smem_u32(&sm.full[q]), 1);
+            mbar_init(smem_u32(&sm.empty[q]), 1);
+        }
+        for (int q = 0; q < 2; ++q) {
+            mbar_init(smem_u32(&sm.acc_full[q]), 1);
+            mbar_init(smem_u32(&sm.acc_empty[q]), kEpiWarps);
+        }
+        mbar_init(smem_u32(&sm.drain), 1);
+        sm.gave_up = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    if (warp == 2) tmem_alloc(smem_u32(&sm.tmem), tmem_cols);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = sm.tmem;
+    volatile int* gave_up = &sm.gave_up;
+
+    if (warp == 0) {
+        if (elect_one()) {
+            int stage = 0;
+            uint32_t phase = 0;
+            int64_t fills = 0;
+            bool ok = true;
+            for (int w = blockIdx.x; w < tl.total && ok; w += gridDim.x) {
+                int tm, tn, split;
+                int64_t r0, r1;
+                tile_of(p, tl, w, tm, tn, split, r0, r1);
+                for (int64_t r = r0; r < r1; r += kBR) {
+                    if (!(ok = mbar_wait(smem_u32(&sm.empty[stage]), phase ^ 1, gave_up))) break;
+                    const uint32_t bar = smem_u32(&sm.full[stage]);
+                    const uint32_t a = smem_u32(tiles + (size_t)stage * tl.stage_bytes), b = a + kBM * 128;
+                    mbar_expect(bar, tl.stage_bytes);
+                    if (p.a_mn) {
+                        for (int q = 0; q < kBM / 64; ++q)
+                            tma_load(a + q * 8192, &map_a, tm * kBM + q * 64, (int)r, bar);
+                    } else {
+                        tma_load(a, &map_a, (int)r, tm * kBM, bar);
+                    }
+                    if (p.b_mn) {
+                        for (int q = 0; q < tl.bn / 64; ++q)
+                            tma_load(b + q * 8192, &map_b, tn * tl.bn + q * 64, (int)r, bar);
+                    } else {
+                        tma_load(b, &map_b, (int)r, tn * tl.bn, bar);
+                    }
+                    ++fills;
+                    if (++stage == tl.stages) {
+                        stage = 0;
+                        phase ^= 1;
+                    }
+                }
+            }
+            if (!ok) {
+                // the copies in flight must land before the block may end
+                const int out = (int)min(fills, (int64_t)tl.stages);
+                for (int q = 0; q < out; ++q) {
+                    if (--stage < 0) {
+                        stage = tl.stages - 1;
+                        phase ^= 1;
+                    }
+                    mbar_wait_bounded(smem_u32(&sm.full[stage]), phase, nullptr);
+                }
+            }
+        }
+    } else if (warp == 1) {
+        int stage = 0, acc = 0;
+        uint32_t phase = 0, acc_phase = 0;
+        bool ok = true;
+        for (int w = blockIdx.x; w < tl.total && ok; w += gridDim.x) {
+            int tm, tn, split;
+            int64_t r0, r1;
+            tile_of(p, tl, w, tm, tn, split, r0, r1);
+            if (!(ok = mbar_wait(smem_u32(&sm.acc_empty[acc]), acc_phase ^ 1, gave_up))) break;
+            tc_fence_after();
+            const uint32_t d = tmem + acc * tl.bn;
+            for (int64_t r = r0; r < r1; r += kBR) {
+                // unlabelled rows of x must not reach dw: bit q stands for row r + q
+                uint32_t off0 = 0, off1 = 0;
+                if (p.label_reduces) {
+                    const int64_t a = r + lane, b = a + 32;
+                    off0 = __ballot_sync(~0u, a < p.R && !labelled(p, a));
+                    off1 = __ballot_sync(~0u, b < p.R && !labelled(p, b));
+                }
+                if (!(ok = mbar_wait(smem_u32(&sm.full[stage]), phase, gave_up))) break;
+                uint8_t* sa = tiles + (size_t)stage * tl.stage_bytes;
+                if (off0 | off1) {
+                    uint8_t* sb = sa + kBM * 128;
+                    for (int q = 0; q < kBR; ++q) {
+                        if (!((q < 32 ? off0 >> q : off1 >> (q - 32)) & 1)) continue;
+                        for (int c = lane; c < tl.bn / 8; c += 32)
+                            *reinterpret_cast<uint4*>(sb + (c / 8) * 8192 + q * 128 + (c % 8) * 16) = make_uint4(0, 0, 0, 0);
+                    }
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
+                }
+                tc_fence_after();
+                if (elect_one()) {
+                    const uint32_t a = smem_u32(sa), b = a + kBM * 128;
+                    const uint64_t da = smem_desc(a, p.a_mn ? 8192 : 16), db = smem_desc(b, p.b_mn ? 8192 : 16);
+                    const uint32_t step_a = p.a_mn ? 2048 >> 4 : 32 >> 4, step_b = p.b_mn ? 2048 >> 4 : 32 >> 4;
+#pragma unroll
+                    for (int k = 0; k < kBR / 16; ++k)
+                        tc_mma(d, da + k * step_a, db + k * step_b, tl.idesc, r > r0 || k > 0);
+                    tc_commit(smem_u32(&sm.empty[stage]));
+                }
+                __syncwarp();
+                if (++stage == tl.stages) {
+                    stage = 0;
+                    phase ^= 1;
+                }
+            }
+            if (!ok) break;
+            if (elect_one()) tc_commit(smem_u32(&sm.acc_full[acc]));
+            __syncwarp();
+            acc ^= 1;
+            if (acc == 0) acc_phase ^= 1;
+        }
+        if (!ok) {
+            // products in flight must end before the block frees TMEM
+            if (elect_one()) {
+                tc_commit(smem_u32(&sm.drain));
+                mbar_wait_bounded(smem_u32(&sm.drain), 0, nullptr);
+            }
+            __syncwarp();
+        }
+    } else if (warp >= 4) {
+        const int quarter = warp % 4, half = (warp - 4) / 4;
+        float* st = staging + (warp - 4) * 32 * kStagePitch;
+        int acc = 0;
+        uint32_t acc_phase = 0;
+        for (int w = blockIdx.x; w < tl.total; w += gridDim.x) {
+            int tm, tn, split;
+            int64_t r0, r1;
+            tile_of(p, tl, w, tm, tn, split, r0, r1);
+            const int64_t i0 = (int64_t)tm * kBM + quarter * 32;
+            RowState row = row_begin<EPI>(p, i0, lane);
+            if (!mbar_wait(smem_u32(&sm.acc_full[acc]), acc_phase, gave_up)) break;
+            tc_fence_after();
+            if (i0 < p.M) {
+                for (int c = half * (tl.bn / 2); c < (half + 1) * (tl.bn / 2); c += 32) {
+                    if ((int64_t)tn * tl.bn + c >= p.N) break;
+                    uint32_t raw[32];
+                    tmem_load32(tmem + ((uint32_t)quarter << 21) + acc * tl.bn + c, raw);
+                    tmem_wait();
+                    float v[32];
+#pragma unroll
+                    for (int q = 0; q < 32; ++q) v[q] = __uint_as_float(raw[q]);
+                    columns32<T, EPI>(p, tl, row, v, i0, (int64_t)tn * tl.bn + c, split, st, lane);
+                }
+                row_end<EPI>(p, row, 2 * tn + half);
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&sm.acc_empty[acc]));
+            acc ^= 1;
+            if (acc == 0) acc_phase ^= 1;
+        }
+    }
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 2) tmem_free(tmem, tmem_cols);
+}
+
+using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                              const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeFn encoder() {
+    static EncodeFn fn = [] {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult found;
+        OPS_CK(cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &found));
+        if (found != cudaDriverEntryPointSuccess || !p) throw Error(MSPLAT_ERR_CUDA, "no cuTensorMapEncodeTiled");
+        return reinterpret_cast<EncodeFn>(p);
+    }();
+    return fn;
+}
+
+// The map of a [rows, cols] matrix read in boxes of 64 columns (128 bytes) x
+// box_rows rows.
+CUtensorMap make_map(const void* base, int64_t rows, int64_t cols, int64_t ld, int box_rows, int dtype) {
+    CUtensorMap m;
+    const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+    const cuuint64_t strides[1] = {(cuuint64_t)(rows > 1 ? ld * 2 : round_up(cols * 2, 16))};
+    const cuuint32_t box[2] = {64, (cuuint32_t)box_rows}, step[2] = {1, 1};
+    const CUresult r = encoder()(
+        &m, dtype == MSPLAT_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2,
+        const_cast<void*>(base), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) throw Error(MSPLAT_ERR_CUDA, "cuTensorMapEncodeTiled failed");
+    return m;
+}
+
+bool tma_ready(const void* p, int64_t ld, int64_t rows) {
+    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && (rows <= 1 || (ld % 8 == 0 && ld * 2 < (1ll << 40)));
+}
+
+template <typename T, int EPI>
+void run(const Product& p, const Tiles& tl, const CUtensorMap& a, const CUtensorMap& b, cudaStream_t s) {
+    const int bytes = tl.stages * tl.stage_bytes + kStagingBytes + 1024;
+    OPS_CK(cudaFuncSetAttribute(k_product_tc16<T, EPI>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    note_launches(1);
+    k_product_tc16<T, EPI><<<std::min(tl.total, kSMs), kThreads, bytes, s>>>(p, tl, a, b);
+    OPS_CK(cudaGetLastError());
+}
+
+template <typename T>
+void typed(const Product& p, const Tiles& tl, const CUtensorMap& a, const CUtensorMap& b, cudaStream_t s) {
+    switch (p.epi) {
+        case kEpiLinear: return run<T, kEpiLinear>(p, tl, a, b, s);
+        case kEpiSlab: return run<T, kEpiSlab>(p, tl, a, b, s);
+        case kEpiStats: return run<T, kEpiStats>(p, tl, a, b, s);
+        default: return run<T, kEpiGrad>(p, tl, a, b, s);
+    }
+}
+
+}  // namespace
+
+bool gave_up_tc16(cudaStream_t s) { return take_gave_up(s); }
+
+bool can_product_tc16(const Product& p) {
+    return p.dtype != MSPLAT_DTYPE_F32 && tma_ready(p.A, p.lda, p.a_mn ? p.R : p.M) &&
+           tma_ready(p.B, p.ldb, p.b_mn ? p.R : p.N);
+}
+
+void launch_product_tc16(const Product& p, cudaStream_t s) {
+    Tiles tl{};
+    tl.bn = tile_columns(p, 256);
+    const int64_t tm = ceil_div(p.M, kBM), tn = ceil_div(p.N, tl.bn);
+    const int64_t total = tm * tn * (p.epi == kEpiSlab ? p.splits : 1);
+    if (total > 0x3fffffff) throw Error(MSPLAT_ERR_CAPACITY, "too many tiles");
+    tl.tiles_m = (int)tm;
+    tl.tiles_n = (int)tn;
+    tl.total = (int)total;
+    tl.stage_bytes = (kBM + tl.bn) * 128;
+    tl.stages = std::min(kMaxStages, (int)((227 * 1024 - 1024 - 512 - kStagingBytes) / tl.stage_bytes));
+    tl.idesc = instr_desc(p.dtype == MSPLAT_DTYPE_BF16, p.a_mn, p.b_mn, tl.bn);
+    tl.vec = pick_vec(p);
+    const CUtensorMap a = p.a_mn ? make_map(p.A, p.R, p.M, p.lda, kBR, p.dtype)
+                                 : make_map(p.A, p.M, p.R, p.lda, kBM, p.dtype);
+    const CUtensorMap b = p.b_mn ? make_map(p.B, p.R, p.N, p.ldb, kBR, p.dtype)
+                                 : make_map(p.B, p.N, p.R, p.ldb, tl.bn, p.dtype);
+    if (p.dtype == MSPLAT_DTYPE_F16)
+        typed<__half>(p, tl, a, b, s);
+    else
+        typed<__nv_bfloat16>(p, tl, a, b, s);
+}
+
+}  // namespace ops
+}  // namespace msplat

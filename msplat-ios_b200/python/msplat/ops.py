@@ -17,7 +17,7 @@ import torch
 
 from ._backend import MsplatError, load
 
-__all__ = ["linear_forward", "linear_backward", "dropout", "loss_cross_entropy", "ACTIVATIONS", "MsplatError"]
+__all__ = ["linear_forward", "linear_backward", "dropout", "loss_cross_entropy", "ACTIVATIONS", "status", "MsplatError"]
 
 ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "silu": 3, "sigmoid": 4}
 _DTYPES = {torch.float32: 0, torch.float16: 4, torch.bfloat16: 5}
@@ -41,8 +41,10 @@ def _lib():
     L.msplat_loss_cross_entropy_workspace.argtypes = [i64, i64, i64, i32, i32, pu64]
     L.msplat_loss_cross_entropy.argtypes = [i64, i64, i64, vp, i64, vp, i64, vp, f, f, vp, vp, vp, i64, vp, i64, i32,
                                             vp, u64, vp]
+    L.msplat_ops_status.argtypes = [vp]
     for name in ("msplat_linear_forward", "msplat_linear_backward_workspace", "msplat_linear_backward",
-                 "msplat_dropout", "msplat_loss_cross_entropy_workspace", "msplat_loss_cross_entropy"):
+                 "msplat_dropout", "msplat_loss_cross_entropy_workspace", "msplat_loss_cross_entropy",
+                 "msplat_ops_status"):
         getattr(L, name).restype = C.c_int
     _L = L
     return L
@@ -241,3 +243,10 @@ def loss_cross_entropy(x, w, targets, logit_scale=1.0, weight=1.0, grad=True, st
                                            dw.data_ptr() if grad else None, d, dt, ws.data_ptr() if size else None,
                                            size, on.handle))
     return loss, row_loss, dx, dw
+
+
+def status(stream=None):
+    """Waits for the stream and raises MsplatError when a kernel gave up
+    waiting since the last call (its waits are bounded)."""
+    s = stream if stream is not None else torch.cuda.current_stream()
+    _check(_lib().msplat_ops_status(s.cuda_stream))
