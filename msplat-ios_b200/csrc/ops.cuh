@@ -138,10 +138,14 @@ int64_t stats_blocks(const Product& p);
 inline int64_t stats_blocks_most(int64_t n) { return 2 * ceil_div(n, 128); }
 
 void launch_product(const Product& p, cudaStream_t s);
-void launch_product_simt(const Product& p, cudaStream_t s);
+// 16-bit matrices that TMA can address (ops_tc16.cu); everything else (ops_tcv.cu).
 bool can_product_tc16(const Product& p);
+int64_t stats_blocks_tc16(const Product& p);
 void launch_product_tc16(const Product& p, cudaStream_t s);
 bool gave_up_tc16(cudaStream_t s);
+void launch_product_tcv(const Product& p, cudaStream_t s);
+int64_t stats_blocks_tcv(const Product& p);
+bool gave_up_tcv(cudaStream_t s);
 
 // dz = dy act'(z) (dz may be null) and the column sums of dz in pieces of
 // rows: partial[piece][n]. Returns the number of pieces.

@@ -67,17 +67,20 @@ void check_workspace(const Arena& a, void* workspace, uint64_t bytes) {
     require(bytes >= a.used, "workspace is too small");
 }
 
-// Pieces of a long reduction: enough tiles for every SM, and pieces of at
-// least 512.
+// Pieces of a long reduction of an M x N result: enough tiles for every SM, in
+// pieces of at least 512. The tensor cores truncate when they add, so 32-bit
+// results take pieces of at most 1024 (whose sums are added with rounding) as
+// long as the pieces take no more than kSlabBytes.
+constexpr int64_t kSlabBytes = 256ll << 20;
 struct Split {
     int splits;
     int64_t len;
 };
-Split plan_split(int64_t M, int64_t N, int64_t R) {
+Split plan_split(int64_t M, int64_t N, int64_t R, int dtype) {
     const int64_t tiles = ceil_div(M, 128) * ceil_div(N, 128);
-    int64_t s = tiles >= kSMs ? 1 : kSMs / tiles;
-    const int64_t most = ceil_div(R, 512);
-    if (s > most) s = most;
+    int64_t s = std::min(ceil_div(R, 512), tiles >= kSMs ? 1 : kSMs / tiles);
+    if (dtype == MSPLAT_DTYPE_F32)
+        s = std::max(s, std::min(ceil_div(R, 1024), std::max<int64_t>(1, kSlabBytes / (M * N * 4))));
     const int64_t len = round_up(ceil_div(R, s), 64);
     return {(int)ceil_div(R, len), len};
 }
@@ -96,7 +99,7 @@ struct BackwardPlan {
     float* sums = nullptr;
     int pieces = 0;
     BackwardPlan(Arena& a, int64_t m, int64_t n, int64_t k, int act, int dtype) {
-        split = plan_split(n, k, m);
+        split = plan_split(n, k, m, dtype);
         pieces = dz_pieces(m, n);
         lddz = round_up(n, 16 / dtype_size(dtype));
         if (act != MSPLAT_ACT_NONE) dz = a.take<char>(m * lddz * dtype_size(dtype));
@@ -145,8 +148,8 @@ struct LossPlan {
         ldg = by_rows ? other : round_up(chunk, 16 / es);
         g = a.take<char>((by_rows ? chunk : m) * ldg * es);
         const int64_t rows = by_rows ? chunk : m, cols = by_rows ? v : chunk;
-        sx = plan_split(rows, d, cols);
-        sw = plan_split(cols, d, rows);
+        sx = plan_split(rows, d, cols, dtype);
+        sw = plan_split(cols, d, rows, dtype);
         const bool pieces = chunk < all;
         if ((!by_rows && pieces) || sx.splits > 1) slab_x = a.take<float>((int64_t)sx.splits * rows * d);
         if ((by_rows && pieces) || sw.splits > 1) slab_w = a.take<float>((int64_t)sw.splits * cols * d);
@@ -199,7 +202,8 @@ extern "C" {
 
 int msplat_ops_status(void* stream) {
     return guarded([&] {
-        if (gave_up_tc16(static_cast<cudaStream_t>(stream)))
+        const bool tc16 = gave_up_tc16(static_cast<cudaStream_t>(stream));
+        if (gave_up_tcv(static_cast<cudaStream_t>(stream)) || tc16)
             throw Error(MSPLAT_ERR_CUDA, "a kernel gave up waiting: the results since the last call are not valid");
     });
 }

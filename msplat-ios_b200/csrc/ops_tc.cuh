@@ -151,6 +151,22 @@ struct Tiles {
     int vec;             // outputs, residual and bias can be accessed four elements at a time
 };
 
+// Tile w of a product: its place, its piece of the reduction.
+__device__ __forceinline__ void tile_of(const Product& p, const Tiles& tl, int w, int& tm, int& tn, int& split,
+                                        int64_t& r0, int64_t& r1) {
+    const int per = tl.tiles_m * tl.tiles_n;
+    split = w / per;
+    w -= split * per;
+    tm = w / tl.tiles_n;
+    tn = w - tm * tl.tiles_n;
+    r0 = 0;
+    r1 = p.R;
+    if (p.epi == kEpiSlab) {
+        r0 = split * p.split_len;
+        r1 = min(p.R, r0 + p.split_len);
+    }
+}
+
 // The end of a product for the 16 columns from j0 of the warp's 32 rows from
 // i0, out of the staging buffer: VEC = 4 gives a lane four columns of a row
 // (full sectors, one 8 or 16 byte access), VEC = 1 a single one.
@@ -347,6 +363,16 @@ inline int pick_vec(const Product& p) {
                    aligned4(p.preact, p.ldz, p.M, eo)
                ? 4
                : 1;
+}
+
+inline void set_tiles(const Product& p, Tiles& tl) {
+    const int64_t tm = ceil_div(p.M, kBM), tn = ceil_div(p.N, tl.bn);
+    const int64_t total = tm * tn * (p.epi == kEpiSlab ? p.splits : 1);
+    if (total > 0x3fffffff) throw Error(MSPLAT_ERR_CAPACITY, "too many tiles");
+    tl.tiles_m = (int)tm;
+    tl.tiles_n = (int)tn;
+    tl.total = (int)total;
+    tl.vec = pick_vec(p);
 }
 
 }  // namespace ops

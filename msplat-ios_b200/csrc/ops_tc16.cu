@@ -26,21 +26,6 @@ struct Smem {
     int gave_up;
 };
 
-__device__ __forceinline__ void tile_of(const Product& p, const Tiles& tl, int w, int& tm, int& tn, int& split,
-                                        int64_t& r0, int64_t& r1) {
-    const int per = tl.tiles_m * tl.tiles_n;
-    split = w / per;
-    w -= split * per;
-    tm = w / tl.tiles_n;
-    tn = w - tm * tl.tiles_n;
-    r0 = 0;
-    r1 = p.R;
-    if (p.epi == kEpiSlab) {
-        r0 = split * p.split_len;
-        r1 = min(p.R, r0 + p.split_len);
-    }
-}
-
 template <typename T, int EPI>
 __global__ void __launch_bounds__(kThreads, 1)
     k_product_tc16(const __grid_constant__ Product p, const __grid_constant__ Tiles tl,
@@ -281,19 +266,16 @@ bool can_product_tc16(const Product& p) {
            tma_ready(p.B, p.ldb, p.b_mn ? p.R : p.N);
 }
 
+// the halves of the tiles
+int64_t stats_blocks_tc16(const Product& p) { return 2 * ceil_div(p.N, tile_columns(p, 256)); }
+
 void launch_product_tc16(const Product& p, cudaStream_t s) {
     Tiles tl{};
     tl.bn = tile_columns(p, 256);
-    const int64_t tm = ceil_div(p.M, kBM), tn = ceil_div(p.N, tl.bn);
-    const int64_t total = tm * tn * (p.epi == kEpiSlab ? p.splits : 1);
-    if (total > 0x3fffffff) throw Error(MSPLAT_ERR_CAPACITY, "too many tiles");
-    tl.tiles_m = (int)tm;
-    tl.tiles_n = (int)tn;
-    tl.total = (int)total;
+    set_tiles(p, tl);
     tl.stage_bytes = (kBM + tl.bn) * 128;
     tl.stages = std::min(kMaxStages, (int)((227 * 1024 - 1024 - 512 - kStagingBytes) / tl.stage_bytes));
     tl.idesc = instr_desc(p.dtype == MSPLAT_DTYPE_BF16, p.a_mn, p.b_mn, tl.bn);
-    tl.vec = pick_vec(p);
     const CUtensorMap a = p.a_mn ? make_map(p.A, p.R, p.M, p.lda, kBR, p.dtype)
                                  : make_map(p.A, p.M, p.R, p.lda, kBM, p.dtype);
     const CUtensorMap b = p.b_mn ? make_map(p.B, p.R, p.N, p.ldb, kBR, p.dtype)

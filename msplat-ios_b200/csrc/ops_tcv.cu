@@ -1,0 +1,369 @@
+// ops_tcv.cu — products on the tensor cores whose operands pass through
+// registers on their way to shared memory: 32-bit matrices, and 16-bit ones
+// that TMA cannot address (odd row strides or starting columns).
+//
+// A 32-bit factor is the sum of three bf16 numbers, x = h + m + l, each the
+// rounded rest of the one before: together they keep its 24 bits. The product
+// of two factors is then h h' (accumulated on its own) and h m' + m h' + m m' +
+// h l' + l h' (accumulated together, 2^-8 smaller), six tcgen05.mma in place of
+// one; what is left out is below 2^-24 of the product. The tensor cores
+// truncate when they add (measured: 1e-9 of the sum per element of the
+// reduction), so a long reduction changes to a fresh accumulator after every
+// 512 elements while there are some, and the accumulators are added with
+// rounding at the end.
+//
+// A block owns 128 x bn tiles (bn 64 or 128) and walks its share of them. Warps
+// 8-15 load, split and store the stages (the layout is TMA's 128-byte swizzle,
+// 64 elements of the reduction per stage), warp 0 issues the products, warps 4-7
+// do the ends of the finished tile from TMEM meanwhile.
+#include "ops_tc.cuh"
+
+namespace msplat {
+namespace ops {
+namespace {
+
+constexpr int kThreads = 512;
+constexpr int kLoaders = 256;
+constexpr int kMaxStages = 8;
+constexpr int kGroup = 8;  // stages (of 64) that one accumulator takes
+
+struct Smem {
+    uint64_t full[kMaxStages], empty[kMaxStages];
+    uint64_t acc_full[2], acc_empty[2], drain;
+    uint32_t tmem;
+    int gave_up;
+};
+
+template <typename T>
+constexpr int planes() { return sizeof(T) == 4 ? 3 : 1; }
+
+// Eight consecutive elements on their way to shared memory.
+template <typename T>
+struct Chunk;
+template <>
+struct Chunk<float> {
+    float v[8];
+    __device__ __forceinline__ void zero() {
+#pragma unroll
+        for (int q = 0; q < 8; ++q) v[q] = 0.f;
+    }
+    __device__ __forceinline__ void load(const float* g) {
+        const float4 a = __ldg(reinterpret_cast<const float4*>(g)), b = __ldg(reinterpret_cast<const float4*>(g) + 1);
+        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    }
+    __device__ __forceinline__ void set(int q, float x) { v[q] = x; }
+    // the three parts, `plane` bytes apart
+    __device__ __forceinline__ void store(uint8_t* s, uint32_t plane) const {
+        uint32_t w[3][4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            float a = v[2 * q], b = v[2 * q + 1];
+#pragma unroll
+            for (int k = 0; k < 3; ++k) {
+                const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+                w[k][q] = *reinterpret_cast<const uint32_t*>(&h);
+                if (k < 2) {
+                    a -= __uint_as_float(w[k][q] << 16);
+                    b -= __uint_as_float(w[k][q] & 0xFFFF0000u);
+                }
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < 3; ++k)
+            *reinterpret_cast<uint4*>(s + k * plane) = make_uint4(w[k][0], w[k][1], w[k][2], w[k][3]);
+    }
+};
+template <typename T>
+struct Chunk {
+    uint4 w;
+    __device__ __forceinline__ void zero() { w = make_uint4(0, 0, 0, 0); }
+    __device__ __forceinline__ void load(const T* g) { w = __ldg(reinterpret_cast<const uint4*>(g)); }
+    __device__ __forceinline__ void set(int q, T x) {
+        const uint32_t bits = (uint32_t)*reinterpret_cast<const uint16_t*>(&x) << 16 * (q & 1);
+        (q < 2 ? w.x : q < 4 ? w.y : q < 6 ? w.z : w.w) |= bits;
+    }
+    __device__ __forceinline__ void store(uint8_t* s, uint32_t) const { *reinterpret_cast<uint4*>(s) = w; }
+};
+
+// One operand as rows of consecutive elements: [i][r], or [r][i] when mn.
+template <typename T>
+struct Operand {
+    const T* p;
+    int64_t ld, rows, cols;
+    bool mn, vec;
+    const Product* masked;  // rows without a label read as zeros
+};
+
+// The stage's tile of an operand: WIDE / 32 chunks of eight per thread, thread
+// t taking chunk t % 8 of row t / 8 + 32 q (eight lanes read one row's 64
+// elements and fill one 128-byte row of shared memory).
+template <typename T, int WIDE>
+__device__ __forceinline__ void load_tile(const Operand<T>& o, int64_t i0, int64_t r0, int t, Chunk<T> (&c)[WIDE / 32]) {
+#pragma unroll
+    for (int q = 0; q < WIDE / 32; ++q) {
+        const int line = t / 8 + 32 * q;
+        // mn: 64 rows of r per group of 64 i
+        const int64_t row = o.mn ? r0 + line % 64 : i0 + line;
+        const int64_t col = (o.mn ? i0 + line / 64 * 64 : r0) + t % 8 * 8;
+        c[q].zero();
+        if (row >= o.rows || col >= o.cols || (o.masked && !labelled(*o.masked, row))) continue;
+        const T* g = o.p + row * o.ld + col;
+        if (o.vec && col + 8 <= o.cols) {
+            c[q].load(g);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (col + e < o.cols) c[q].set(e, __ldg(g + e));
+        }
+    }
+}
+template <typename T, int WIDE>
+__device__ __forceinline__ void store_tile(uint8_t* s, int t, const Chunk<T> (&c)[WIDE / 32]) {
+#pragma unroll
+    for (int q = 0; q < WIDE / 32; ++q) {
+        const int line = t / 8 + 32 * q;
+        c[q].store(s + line * 128 + ((t % 8) ^ (line & 7)) * 16, WIDE * 128);
+    }
+}
+
+template <typename T, int EPI, int BN>
+__global__ void __launch_bounds__(kThreads, 1)
+    k_product_tcv(const __grid_constant__ Product p, const __grid_constant__ Tiles tl, const bool vec_a,
+                  const bool vec_b) {
+    constexpr int P = planes<T>();
+    constexpr int kA = P * kBM * 128, kB = P * BN * 128;
+    // accumulators of one tile: the groups' and, for split factors, the corrections'
+    constexpr int kGroups = 512 / 2 / BN - (P > 1 ? 1 : 0);
+    constexpr int kTileCols = 256;
+    extern __shared__ __align__(1024) uint8_t dyn[];
+    __shared__ Smem sm;
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    uint8_t* tiles = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(dyn) + 1023) & ~(uintptr_t)1023);
+    float* staging = reinterpret_cast<float*>(tiles + (size_t)tl.stages * (kA + kB));
+
+    if (threadIdx.x == 0) {
+        for (int q = 0; q < tl.stages; ++q) {
+            mbar_init(smem_u32(&sm.full[q]), kLoaders / 32);
+            mbar_init(smem_u32(&sm.empty[q]), 1);
+        }
+        for (int q = 0; q < 2; ++q) {
+            mbar_init(smem_u32(&sm.acc_full[q]), 1);
+            mbar_init(smem_u32(&sm.acc_empty[q]), 4);
+        }
+        mbar_init(smem_u32(&sm.drain), 1);
+        sm.gave_up = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) tmem_alloc(smem_u32(&sm.tmem), 2 * kTileCols);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = sm.tmem;
+    volatile int* gave_up = &sm.gave_up;
+
+    if (warp >= 8) {
+        const int t = threadIdx.x - 256;
+        const Operand<T> oa{static_cast<const T*>(p.A), p.lda, p.a_mn ? p.R : p.M, p.a_mn ? p.M : p.R, p.a_mn, vec_a,
+                            nullptr};
+        const Operand<T> ob{static_cast<const T*>(p.B), p.ldb, p.b_mn ? p.R : p.N, p.b_mn ? p.N : p.R, p.b_mn, vec_b,
+                            p.label_reduces ? &p : nullptr};
+        int stage = 0;
+        uint32_t phase = 0;
+        bool ok = true;
+        for (int w = blockIdx.x; w < tl.total && ok; w += gridDim.x) {
+            int tm, tn, split;
+            int64_t r0, r1;
+            tile_of(p, tl, w, tm, tn, split, r0, r1);
+            for (int64_t r = r0; r < r1; r += kBR) {
+                Chunk<T> a[kBM / 32], b[BN / 32];
+                load_tile<T, kBM>(oa, (int64_t)tm * kBM, r, t, a);
+                load_tile<T, BN>(ob, (int64_t)tn * BN, r, t, b);
+                if (!(ok = mbar_wait(smem_u32(&sm.empty[stage]), phase ^ 1, gave_up))) break;
+                uint8_t* s = tiles + (size_t)stage * (kA + kB);
+                store_tile<T, kBM>(s, t, a);
+                store_tile<T, BN>(s + kA, t, b);
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&sm.full[stage]));
+                if (++stage == tl.stages) {
+                    stage = 0;
+                    phase ^= 1;
+                }
+            }
+        }
+    } else if (warp == 0) {
+        int stage = 0, acc = 0;
+        uint32_t phase = 0, acc_phase = 0;
+        bool ok = true;
+        for (int w = blockIdx.x; w < tl.total && ok; w += gridDim.x) {
+            int tm, tn, split;
+            int64_t r0, r1;
+            tile_of(p, tl, w, tm, tn, split, r0, r1);
+            if (!(ok = mbar_wait(smem_u32(&sm.acc_empty[acc]), acc_phase ^ 1, gave_up))) break;
+            tc_fence_after();
+            const uint32_t d = tmem + acc * kTileCols, dc = d + kGroups * BN;
+            int block = 0;
+            for (int64_t r = r0; r < r1; r += kBR, ++block) {
+                if (!(ok = mbar_wait(smem_u32(&sm.full[stage]), phase, gave_up))) break;
+                tc_fence_after();
+                if (elect_one()) {
+                    const uint32_t a = smem_u32(tiles + (size_t)stage * (kA + kB)), b = a + kA;
+                    const uint32_t step_a = p.a_mn ? 2048 >> 4 : 32 >> 4, step_b = p.b_mn ? 2048 >> 4 : 32 >> 4;
+                    uint64_t da[P], db[P];
+#pragma unroll
+                    for (int q = 0; q < P; ++q) {
+                        da[q] = smem_desc(a + q * kBM * 128, p.a_mn ? 8192 : 16);
+                        db[q] = smem_desc(b + q * BN * 128, p.b_mn ? 8192 : 16);
+                    }
+                    const int group = min(block / kGroup, kGroups - 1);
+                    const bool fresh = block % kGroup == 0 && block / kGroup < kGroups;
+#pragma unroll
+                    for (int k = 0; k < kBR / 16; ++k) {
+                        if (P > 1) {
+                            const int pa[5] = {0, 2, 1, 0, 1}, pb[5] = {2, 0, 1, 1, 0};
+#pragma unroll
+                            for (int q = 0; q < 5; ++q)
+                                tc_mma(dc, da[pa[q]] + k * step_a, db[pb[q]] + k * step_b, tl.idesc,
+                                       block > 0 || k > 0 || q > 0);
+                        }
+                        tc_mma(d + group * BN, da[0] + k * step_a, db[0] + k * step_b, tl.idesc, !fresh || k > 0);
+                    }
+                    tc_commit(smem_u32(&sm.empty[stage]));
+                }
+                __syncwarp();
+                if (++stage == tl.stages) {
+                    stage = 0;
+                    phase ^= 1;
+                }
+            }
+            if (!ok) break;
+            if (elect_one()) tc_commit(smem_u32(&sm.acc_full[acc]));
+            __syncwarp();
+            acc ^= 1;
+            if (acc == 0) acc_phase ^= 1;
+        }
+        if (!ok) {
+            // products in flight must end before the block frees TMEM
+            if (elect_one()) {
+                tc_commit(smem_u32(&sm.drain));
+                mbar_wait_bounded(smem_u32(&sm.drain), 0, nullptr);
+            }
+            __syncwarp();
+        }
+    } else if (warp >= 4) {
+        float* st = staging + (warp - 4) * 32 * kStagePitch;
+        int acc = 0;
+        uint32_t acc_phase = 0;
+        for (int w = blockIdx.x; w < tl.total; w += gridDim.x) {
+            int tm, tn, split;
+            int64_t r0, r1;
+            tile_of(p, tl, w, tm, tn, split, r0, r1);
+            const int64_t i0 = (int64_t)tm * kBM + (warp - 4) * 32;
+            const int groups = (int)min((int64_t)kGroups, (r1 - r0 + kGroup * kBR - 1) / (kGroup * kBR));
+            RowState row = row_begin<EPI>(p, i0, lane);
+            if (!mbar_wait(smem_u32(&sm.acc_full[acc]), acc_phase, gave_up)) break;
+            tc_fence_after();
+            if (i0 < p.M) {
+                const uint32_t d = tmem + ((uint32_t)(warp - 4) << 21) + acc * kTileCols;
+                for (int c = 0; c < BN; c += 32) {
+                    if ((int64_t)tn * BN + c >= p.N) break;
+                    uint32_t raw[32];
+                    float v[32];
+                    if (P > 1) {
+                        tmem_load32(d + kGroups * BN + c, raw);
+                        tmem_wait();
+#pragma unroll
+                        for (int q = 0; q < 32; ++q) v[q] = __uint_as_float(raw[q]);
+                    } else {
+#pragma unroll
+                        for (int q = 0; q < 32; ++q) v[q] = 0.f;
+                    }
+                    for (int g = 0; g < groups; ++g) {
+                        tmem_load32(d + g * BN + c, raw);
+                        tmem_wait();
+#pragma unroll
+                        for (int q = 0; q < 32; ++q) v[q] += __uint_as_float(raw[q]);
+                    }
+                    columns32<T, EPI>(p, tl, row, v, i0, (int64_t)tn * BN + c, split, st, lane);
+                }
+                row_end<EPI>(p, row, tn);
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&sm.acc_empty[acc]));
+            acc ^= 1;
+            if (acc == 0) acc_phase ^= 1;
+        }
+    }
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 1) tmem_free(tmem, 2 * kTileCols);
+}
+
+template <typename T>
+bool vectors(const void* q, int64_t ld, int64_t rows) {
+    return reinterpret_cast<uintptr_t>(q) % 16 == 0 && (rows <= 1 || ld % (16 / (int64_t)sizeof(T)) == 0);
+}
+
+template <typename T, int EPI, int BN>
+void run(const Product& p, Tiles tl, cudaStream_t s) {
+    constexpr int stage = planes<T>() * (kBM + BN) * 128, staging = 4 * 32 * kStagePitch * 4;
+    tl.stages = std::min(kMaxStages, (227 * 1024 - 2048 - staging) / stage);
+    const int bytes = tl.stages * stage + staging + 1024;
+    OPS_CK(cudaFuncSetAttribute(k_product_tcv<T, EPI, BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    note_launches(1);
+    k_product_tcv<T, EPI, BN><<<std::min(tl.total, kSMs), kThreads, bytes, s>>>(
+        p, tl, vectors<T>(p.A, p.lda, p.a_mn ? p.R : p.M), vectors<T>(p.B, p.ldb, p.b_mn ? p.R : p.N));
+    OPS_CK(cudaGetLastError());
+}
+
+template <typename T, int EPI>
+void sized(const Product& p, const Tiles& tl, cudaStream_t s) {
+    if (tl.bn == 64)
+        run<T, EPI, 64>(p, tl, s);
+    else
+        run<T, EPI, 128>(p, tl, s);
+}
+
+template <typename T>
+void typed(const Product& p, const Tiles& tl, cudaStream_t s) {
+    switch (p.epi) {
+        case kEpiLinear: return sized<T, kEpiLinear>(p, tl, s);
+        case kEpiSlab: return sized<T, kEpiSlab>(p, tl, s);
+        case kEpiStats: return sized<T, kEpiStats>(p, tl, s);
+        default: return sized<T, kEpiGrad>(p, tl, s);
+    }
+}
+
+// 64 columns leave room for more accumulators, which a reduction longer than
+// one accumulator's share needs (for 32-bit results).
+int columns_tcv(const Product& p) {
+    const bool exact = p.dtype == MSPLAT_DTYPE_F32;
+    const int64_t len = p.epi == kEpiSlab ? std::min(p.R, p.split_len) : p.R;
+    return tile_columns(p, exact && len > kGroup * kBR ? 64 : 128);
+}
+
+}  // namespace
+
+bool gave_up_tcv(cudaStream_t s) { return take_gave_up(s); }
+
+int64_t stats_blocks_tcv(const Product& p) { return ceil_div(p.N, columns_tcv(p)); }
+
+void launch_product_tcv(const Product& p, cudaStream_t s) {
+    Tiles tl{};
+    tl.bn = columns_tcv(p);
+    set_tiles(p, tl);
+    // the parts of 32-bit factors are bf16
+    tl.idesc = instr_desc(p.dtype != MSPLAT_DTYPE_F16, p.a_mn, p.b_mn, tl.bn);
+    if (p.dtype == MSPLAT_DTYPE_F32)
+        typed<float>(p, tl, s);
+    else if (p.dtype == MSPLAT_DTYPE_F16)
+        typed<__half>(p, tl, s);
+    else
+        typed<__nv_bfloat16>(p, tl, s);
+}
+
+}  // namespace ops
+}  // namespace msplat
