@@ -53,41 +53,61 @@ __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { retu
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
-__device__ __forceinline__ float activate(float z, int act) {
-    switch (act) {
-        case MSPLAT_ACT_RELU: return z > 0.f ? z : (z != z ? z : 0.f);
-        case MSPLAT_ACT_GELU: return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
-        case MSPLAT_ACT_SILU: return z / (1.f + __expf(-z));
-        case MSPLAT_ACT_SIGMOID: return 1.f / (1.f + __expf(-z));
-        default: return z;
-    }
+// The Gaussian distribution function through the error function's
+// approximation 7.1.26 of Abramowitz and Stegun, Handbook of Mathematical
+// Functions: erfc(x) = t (a1 + t (a2 + ...)) exp(-x^2), t = 1 / (1 + p x), off by
+// at most 1.5e-7; a reciprocal and an exponential in place of erff's longer
+// polynomials. *density: exp(-z^2 / 2).
+__device__ __forceinline__ float normal_cdf(float z, float* density) {
+    const float x = fabsf(z) * 0.70710678118654752f;
+    const float t = __fdividef(1.f, fmaf(0.3275911f, x, 1.f));
+    const float e = exp2f(-kLog2e * x * x);
+    float q = fmaf(1.061405429f, t, -1.453152027f);
+    q = fmaf(q, t, 1.421413741f);
+    q = fmaf(q, t, -0.284496736f);
+    q = fmaf(q, t, 0.254829592f);
+    q = 0.5f * q * t * e;  // half of erfc(x)
+    *density = e;
+    return z < 0.f ? q : 1.f - q;
 }
+__device__ __forceinline__ float logistic(float z) { return __fdividef(1.f, 1.f + exp2f(-kLog2e * z)); }
+
+__device__ __forceinline__ float act_relu(float z) { return z < 0.f ? 0.f : z; }
+__device__ __forceinline__ float act_gelu(float z) {
+    float e;
+    return z * normal_cdf(z, &e);
+}
+__device__ __forceinline__ float act_silu(float z) { return z * logistic(z); }
+__device__ __forceinline__ float act_sigmoid(float z) { return logistic(z); }
 // act'(z)
-__device__ __forceinline__ float act_slope(float z, int act) {
-    switch (act) {
-        case MSPLAT_ACT_RELU: return z > 0.f ? 1.f : 0.f;
-        case MSPLAT_ACT_GELU:
-            return fmaf(z * 0.3989422804014327f, __expf(-0.5f * z * z),
-                        0.5f * (1.f + erff(z * 0.70710678118654752f)));
-        case MSPLAT_ACT_SILU: {
-            const float q = 1.f / (1.f + __expf(-z));
-            return q * fmaf(z, 1.f - q, 1.f);
-        }
-        case MSPLAT_ACT_SIGMOID: {
-            const float q = 1.f / (1.f + __expf(-z));
-            return q * (1.f - q);
-        }
-        default: return 1.f;
+template <int ACT>
+__device__ __forceinline__ float act_slope(float z) {
+    if (ACT == MSPLAT_ACT_RELU) return z > 0.f ? 1.f : 0.f;
+    if (ACT == MSPLAT_ACT_GELU) {
+        float e;
+        const float c = normal_cdf(z, &e);
+        return fmaf(z * 0.3989422804014327f, e, c);
     }
+    if (ACT == MSPLAT_ACT_SILU) {
+        const float q = logistic(z);
+        return q * fmaf(z, 1.f - q, 1.f);
+    }
+    if (ACT == MSPLAT_ACT_SIGMOID) {
+        const float q = logistic(z);
+        return q * (1.f - q);
+    }
+    return 1.f;
 }
 
 // What a matrix product does with its result.
 enum EpiKind {
     kEpiLinear = 0,  // bias, activation, residual; element type T or float
-    kEpiSlab = 1,    // float partial sums: slab[split][row][col] = or += result
+    kEpiSlab = 1,    // float partial sums: slab[split][row][col] = or += result, slab_ld(N) floats per row
     kEpiStats = 2,   // per row and column block: max and sum of exp of the logits; the label's logit
     kEpiGrad = 3,    // (softmax - one-hot), times g_scale, in T
 };
+
+inline int64_t slab_ld(int64_t n) { return round_up(n, 4); }
 
 // C[i, j] = sum_r A(i, r) B(j, r), i < M, j < N, r < R.
 // A(i, r) = a_mn ? A[r * lda + i] : A[i * lda + r], B(j, r) likewise.
@@ -152,8 +172,8 @@ bool gave_up_tcv(cudaStream_t s);
 int dz_pieces(int64_t m, int64_t n);
 void launch_dz(int64_t m, int64_t n, const void* z, int64_t ldz, int act, const void* dy, int64_t lddy, void* dz,
                int64_t lddz, float* partial, int dtype, cudaStream_t s);
-// out[i, j] = alpha * sum_p slab[p][i][j]
-void launch_slab_sum(int64_t rows, int64_t cols, const float* slab, int pieces, void* out, int64_t ldo, float alpha,
+// out[i, j] = alpha * sum_p slab[p][i][j]; slab rows of ld floats
+void launch_slab_sum(int64_t rows, int64_t cols, const float* slab, int64_t ld, int pieces, void* out, int64_t ldo, float alpha,
                      const float* alpha_dev, const int32_t* targets, int64_t labels, int dtype, cudaStream_t s);
 // Joins the column blocks' statistics of m rows into lse (log2 units) and
 // row_loss; partial[block] = (sum of the labelled rows' losses, their number).

@@ -103,7 +103,7 @@ struct BackwardPlan {
         pieces = dz_pieces(m, n);
         lddz = round_up(n, 16 / dtype_size(dtype));
         if (act != MSPLAT_ACT_NONE) dz = a.take<char>(m * lddz * dtype_size(dtype));
-        slab = a.take<float>((int64_t)split.splits * n * k);
+        slab = a.take<float>((int64_t)split.splits * n * slab_ld(k));
         sums = a.take<float>((int64_t)pieces * n);
     }
 };
@@ -151,8 +151,8 @@ struct LossPlan {
         sx = plan_split(rows, d, cols, dtype);
         sw = plan_split(cols, d, rows, dtype);
         const bool pieces = chunk < all;
-        if ((!by_rows && pieces) || sx.splits > 1) slab_x = a.take<float>((int64_t)sx.splits * rows * d);
-        if ((by_rows && pieces) || sw.splits > 1) slab_w = a.take<float>((int64_t)sw.splits * cols * d);
+        if ((!by_rows && pieces) || sx.splits > 1) slab_x = a.take<float>((int64_t)sx.splits * rows * slab_ld(d));
+        if ((by_rows && pieces) || sw.splits > 1) slab_w = a.take<float>((int64_t)sw.splits * cols * slab_ld(d));
     }
 };
 
@@ -184,7 +184,7 @@ void launch_gradient(Product q, const LossPlan& plan, float* slab, Split split, 
     q.accumulate = sums && !first;
     launch_product(q, s);
     if (!sums || last)
-        launch_slab_sum(q.M, q.N, slab, sums ? split.splits : q.splits, out, ldo, 1.f, plan.alpha,
+        launch_slab_sum(q.M, q.N, slab, slab_ld(q.N), sums ? split.splits : q.splits, out, ldo, 1.f, plan.alpha,
                         q.label_reduces ? nullptr : q.targets, labels, dtype, s);
 }
 
@@ -285,7 +285,7 @@ int msplat_linear_backward(int64_t m, int64_t n, int64_t k, const void* x, int64
         if (activation != MSPLAT_ACT_NONE || dbias) {
             launch_dz(m, n, preact, ldz, activation, dy, lddy, plan.dz, plan.lddz, dbias ? plan.sums : nullptr, dtype,
                       s);
-            if (dbias) launch_slab_sum(1, n, plan.sums, plan.pieces, dbias, n, 1.f, nullptr, nullptr, 0, dtype, s);
+            if (dbias) launch_slab_sum(1, n, plan.sums, n, plan.pieces, dbias, n, 1.f, nullptr, nullptr, 0, dtype, s);
             if (plan.dz) {
                 dz = plan.dz;
                 lddz = plan.lddz;
@@ -313,7 +313,7 @@ int msplat_linear_backward(int64_t m, int64_t n, int64_t k, const void* x, int64
             p.splits = plan.split.splits;
             p.split_len = plan.split.len;
             launch_product(p, s);
-            launch_slab_sum(n, k, plan.slab, plan.split.splits, dw, lddw, 1.f, nullptr, nullptr, 0, dtype, s);
+            launch_slab_sum(n, k, plan.slab, slab_ld(k), plan.split.splits, dw, lddw, 1.f, nullptr, nullptr, 0, dtype, s);
         }
     });
 }

@@ -9,8 +9,8 @@ namespace ops {
 namespace {
 
 // A block takes a piece of the rows and 32 columns; eight warps walk the rows.
-template <typename T>
-__global__ void __launch_bounds__(256) k_dz(int64_t m, int64_t n, const T* z, int64_t ldz, int act, const T* dy,
+template <typename T, int ACT>
+__global__ void __launch_bounds__(256) k_dz(int64_t m, int64_t n, const T* z, int64_t ldz, const T* dy,
                                             int64_t lddy, T* dz, int64_t lddz, float* partial, int64_t piece_rows) {
     __shared__ float sums[8][33];
     const int64_t j = blockIdx.x * 32 + threadIdx.x;
@@ -19,7 +19,7 @@ __global__ void __launch_bounds__(256) k_dz(int64_t m, int64_t n, const T* z, in
     if (j < n)
         for (int64_t i = i0 + threadIdx.y; i < i1; i += 8) {
             float v = to_f32(dy[i * lddy + j]);
-            if (act != MSPLAT_ACT_NONE) v *= act_slope(to_f32(z[i * ldz + j]), act);
+            if (ACT != MSPLAT_ACT_NONE) v *= act_slope<ACT>(to_f32(z[i * ldz + j]));
             if (dz) dz[i * lddz + j] = from_f32<T>(v);
             sum += v;
         }
@@ -33,15 +33,16 @@ __global__ void __launch_bounds__(256) k_dz(int64_t m, int64_t n, const T* z, in
 }
 
 template <typename T>
-__global__ void __launch_bounds__(256) k_slab_sum(int64_t rows, int64_t cols, const float* slab, int pieces, T* out,
+__global__ void __launch_bounds__(256) k_slab_sum(int64_t rows, int64_t cols, const float* slab, int64_t ld, int pieces, T* out,
                                                   int64_t ldo, float alpha, const float* alpha_dev,
                                                   const int32_t* targets, int64_t labels) {
     const int64_t n = rows * cols;
     const float a = alpha * (alpha_dev ? *alpha_dev : 1.f);
     for (int64_t e = blockIdx.x * 256ll + threadIdx.x; e < n; e += gridDim.x * 256ll) {
         float t = 0.f;
-        for (int q = 0; q < pieces; ++q) t += slab[q * n + e];
         const int64_t i = e / cols;
+        const float* at = slab + i * ld + (e - i * cols);
+        for (int q = 0; q < pieces; ++q) t += at[q * rows * ld];
         t *= a;
         if (targets && !(targets[i] >= 0 && targets[i] < labels)) t = 0.f;
         out[i * ldo + (e - i * cols)] = from_f32<T>(t);
@@ -120,8 +121,17 @@ void dz_typed(int64_t m, int64_t n, const void* z, int64_t ldz, int act, const v
     const int pieces = dz_pieces(m, n);
     const dim3 grid((unsigned)ceil_div(n, 32), pieces);
     note_launches(1);
-    k_dz<T><<<grid, dim3(32, 8), 0, s>>>(m, n, static_cast<const T*>(z), ldz, act, static_cast<const T*>(dy), lddy,
-                                         static_cast<T*>(dz), lddz, partial, ceil_div(m, pieces));
+    auto go = [&](auto kernel) {
+        kernel<<<grid, dim3(32, 8), 0, s>>>(m, n, static_cast<const T*>(z), ldz, static_cast<const T*>(dy), lddy,
+                                            static_cast<T*>(dz), lddz, partial, ceil_div(m, pieces));
+    };
+    switch (act) {
+        case MSPLAT_ACT_RELU: go(k_dz<T, MSPLAT_ACT_RELU>); break;
+        case MSPLAT_ACT_GELU: go(k_dz<T, MSPLAT_ACT_GELU>); break;
+        case MSPLAT_ACT_SILU: go(k_dz<T, MSPLAT_ACT_SILU>); break;
+        case MSPLAT_ACT_SIGMOID: go(k_dz<T, MSPLAT_ACT_SIGMOID>); break;
+        default: go(k_dz<T, MSPLAT_ACT_NONE>); break;
+    }
     OPS_CK(cudaGetLastError());
 }
 
@@ -144,19 +154,19 @@ void launch_dz(int64_t m, int64_t n, const void* z, int64_t ldz, int act, const 
         dz_typed<__nv_bfloat16>(m, n, z, ldz, act, dy, lddy, dz, lddz, partial, s);
 }
 
-void launch_slab_sum(int64_t rows, int64_t cols, const float* slab, int pieces, void* out, int64_t ldo, float alpha,
+void launch_slab_sum(int64_t rows, int64_t cols, const float* slab, int64_t ld, int pieces, void* out, int64_t ldo, float alpha,
                      const float* alpha_dev, const int32_t* targets, int64_t labels, int dtype, cudaStream_t s) {
     const int64_t ctas = ceil_div(rows * cols, 256);
     const unsigned grid = (unsigned)(ctas < kSMs * 8 ? ctas : kSMs * 8);
     note_launches(1);
     if (dtype == MSPLAT_DTYPE_F32)
-        k_slab_sum<float><<<grid, 256, 0, s>>>(rows, cols, slab, pieces, static_cast<float*>(out), ldo, alpha,
+        k_slab_sum<float><<<grid, 256, 0, s>>>(rows, cols, slab, ld, pieces, static_cast<float*>(out), ldo, alpha,
                                                alpha_dev, targets, labels);
     else if (dtype == MSPLAT_DTYPE_F16)
-        k_slab_sum<__half><<<grid, 256, 0, s>>>(rows, cols, slab, pieces, static_cast<__half*>(out), ldo, alpha,
+        k_slab_sum<__half><<<grid, 256, 0, s>>>(rows, cols, slab, ld, pieces, static_cast<__half*>(out), ldo, alpha,
                                                 alpha_dev, targets, labels);
     else
-        k_slab_sum<__nv_bfloat16><<<grid, 256, 0, s>>>(rows, cols, slab, pieces, static_cast<__nv_bfloat16*>(out),
+        k_slab_sum<__nv_bfloat16><<<grid, 256, 0, s>>>(rows, cols, slab, ld, pieces, static_cast<__nv_bfloat16*>(out),
                                                        ldo, alpha, alpha_dev, targets, labels);
     OPS_CK(cudaGetLastError());
 }

@@ -10,9 +10,6 @@ namespace ops {
 
 constexpr int kBM = 128;       // rows of a tile: the lanes of TMEM
 constexpr int kBR = 64;        // reduction length of one stage: 128 bytes of a 16-bit type, one swizzle span
-constexpr int kEpiWarps = 8;
-constexpr int kStagePitch = 20;  // floats per row of the staging buffers (16 columns + 4: conflict-free)
-constexpr int kStagingBytes = kEpiWarps * 32 * kStagePitch * 4;
 
 // Set when a wait in a kernel ran out (read and cleared by take_gave_up).
 static __device__ unsigned g_ops_gave_up;
@@ -73,6 +70,34 @@ __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, i
         ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(bar)
         : "memory");
 }
+
+__device__ __forceinline__ void tma_store(const CUtensorMap* map, uint32_t src, int x, int y, int z, bool add) {
+    if (add)
+        asm volatile("cp.reduce.async.bulk.tensor.3d.global.shared::cta.add.tile.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(
+                         map),
+                     "r"(src), "r"(x), "r"(y), "r"(z)
+                     : "memory");
+    else
+        asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(map),
+                     "r"(src), "r"(x), "r"(y), "r"(z)
+                     : "memory");
+}
+__device__ __forceinline__ void tma_load3(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+        ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(0), "r"(bar)
+        : "memory");
+}
+__device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+// all but the last `pending` (0 or 1) groups of stores have read their buffers
+__device__ __forceinline__ void bulk_wait_read(int pending) {
+    if (pending)
+        asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+    else
+        asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+}
+__device__ __forceinline__ void bulk_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+__device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
 __device__ __forceinline__ bool elect_one() {
     uint32_t p;
@@ -148,7 +173,16 @@ struct Tiles {
     int total;           // with the splits of the reduction
     int stages, stage_bytes;
     uint32_t idesc;
-    int vec;             // outputs, residual and bias can be accessed four elements at a time
+    int resident;        // the block's columns stay the same (ops_tcv.cu)
+    // the outputs' boxes of 32 x 32 in shared memory
+    int tma_out;         // they move by TMA (16-byte aligned outputs), else element by element
+    int ring;            // boxes per output and warp, 1 or 2
+    int box_bytes;       // 2048 or 4096
+    int warp_bytes;      // what a warp needs: boxes of y and preact
+};
+
+struct OutMaps {
+    CUtensorMap y, z, r;
 };
 
 // Tile w of a product: its place, its piece of the reduction.
@@ -167,89 +201,103 @@ __device__ __forceinline__ void tile_of(const Product& p, const Tiles& tl, int w
     }
 }
 
-// The end of a product for the 16 columns from j0 of the warp's 32 rows from
-// i0, out of the staging buffer: VEC = 4 gives a lane four columns of a row
-// (full sectors, one 8 or 16 byte access), VEC = 1 a single one.
-template <typename T, typename TO, int EPI, int VEC>
-__device__ __forceinline__ void flush16(const Product& p, const float* st, int64_t i0, int64_t j0, int split,
-                                        float alpha, uint32_t zero_rows, int lane) {
-    constexpr int kLanes = 16 / VEC, kRows = 32 / kLanes;
-    const int c = (lane % kLanes) * VEC;
-    const int64_t j = j0 + c;
-    if (j >= p.N) return;
-    float bias[VEC];
+// A warp's boxes. A box holds 32 rows of 32 columns, 128 or 64 bytes per row, in
+// TMA's 128- or 64-byte swizzle: a thread writes its row's 16-byte pieces
+// without bank conflicts and one instruction stores the box, clipped at the
+// matrix' edges.
+struct WarpOut {
+    uint8_t* y;       // ring boxes
+    uint8_t* z;       // ring boxes, with preact
+    float* bias;      // 32 floats
+    uint32_t bar;     // 2 barriers for the residual's boxes
+    uint32_t phase;   // their phases
+    int k;            // boxes done
+};
+
+template <typename TO>
+__device__ __forceinline__ uint32_t box_piece(int row, int piece) {
+    return sizeof(TO) == 4 ? row * 128 + ((piece ^ (row & 7)) << 4) : row * 64 + ((piece ^ (row >> 1 & 3)) << 4);
+}
+template <typename TO>
+__device__ __forceinline__ TO* box_at(uint8_t* box, int row, int col) {
+    constexpr int n = 16 / sizeof(TO);
+    return reinterpret_cast<TO*>(box + box_piece<TO>(row, col / n)) + col % n;
+}
+template <typename TO>
+struct Piece {
+    union {
+        uint4 w;
+        TO t[16 / sizeof(TO)];
+    };
+    __device__ __forceinline__ Piece() {}
+};
+template <typename TO>
+__device__ __forceinline__ void box_write(uint8_t* box, int row, const float (&v)[32]) {
+    constexpr int n = 16 / sizeof(TO);
 #pragma unroll
-    for (int q = 0; q < VEC; ++q)
-        bias[q] = EPI == kEpiLinear && p.bias && j + q < p.N ? to_f32(static_cast<const T*>(p.bias)[j + q]) : 0.f;
-    const bool whole = j + VEC <= p.N;
-    union Vec { TO t[VEC]; uint4 q4; uint2 q2; };
+    for (int q = 0; q < 32 / n; ++q) {
+        Piece<TO> o;
 #pragma unroll
-    for (int k = 0; k < 32 / kRows; ++k) {
-        const int row = k * kRows + lane / kLanes;
-        const int64_t i = i0 + row;
-        if (i >= p.M) continue;
-        float v[VEC];
+        for (int e = 0; e < n; ++e) o.t[e] = from_f32<TO>(v[q * n + e]);
+        *reinterpret_cast<uint4*>(box + box_piece<TO>(row, q)) = o.w;
+    }
+}
+template <typename TO>
+__device__ __forceinline__ void box_add(const uint8_t* box, int row, float (&v)[32]) {
+    constexpr int n = 16 / sizeof(TO);
 #pragma unroll
-        for (int q = 0; q < VEC; ++q) v[q] = st[row * kStagePitch + c + q];
-        auto put = [&](TO* to) {
-            if (VEC > 1 && whole) {
-                Vec o;
+    for (int q = 0; q < 32 / n; ++q) {
+        Piece<TO> o;
+        o.w = *reinterpret_cast<const uint4*>(box + box_piece<TO>(row, q));
 #pragma unroll
-                for (int q = 0; q < VEC; ++q) o.t[q] = from_f32<TO>(v[q]);
-                if (sizeof(TO) == 4)
-                    *reinterpret_cast<uint4*>(to) = o.q4;
-                else
-                    *reinterpret_cast<uint2*>(to) = o.q2;
-            } else {
+        for (int e = 0; e < n; ++e) v[q * n + e] += to_f32(o.t[e]);
+    }
+}
+// Element by element between a box and rows i0 .., columns j0 .. of a matrix:
+// consecutive lanes take consecutive elements.
+template <typename TO, bool IN>
+__device__ __forceinline__ void box_copy(uint8_t* box, TO* g, int64_t ld, int64_t i0, int64_t j0, int64_t M, int64_t N,
+                                         int lane) {
+    const int n = (int)min((int64_t)32, N - j0), rows = (int)min((int64_t)32, M - i0);
+    for (int e = lane; e < rows * n; e += 32) {
+        const int r = e / n, c = e - r * n;
+        TO* b = box_at<TO>(box, r, c);
+        TO* m = g + (i0 + r) * ld + j0 + c;
+        if (IN)
+            *b = *m;
+        else
+            *m = *b;
+    }
+}
+
+__device__ __forceinline__ void activate32(float (&v)[32], int act) {
+    switch (act) {
+        case MSPLAT_ACT_RELU:
 #pragma unroll
-                for (int q = 0; q < VEC; ++q)
-                    if (j + q < p.N) to[q] = from_f32<TO>(v[q]);
-            }
-        };
-        auto add = [&](const TO* from) {
-            if (VEC > 1 && whole) {
-                Vec o;
-                if (sizeof(TO) == 4)
-                    o.q4 = *reinterpret_cast<const uint4*>(from);
-                else
-                    o.q2 = *reinterpret_cast<const uint2*>(from);
+            for (int q = 0; q < 32; ++q) v[q] = act_relu(v[q]);
+            break;
+        case MSPLAT_ACT_GELU:
 #pragma unroll
-                for (int q = 0; q < VEC; ++q) v[q] += to_f32(o.t[q]);
-            } else {
+            for (int q = 0; q < 32; ++q) v[q] = act_gelu(v[q]);
+            break;
+        case MSPLAT_ACT_SILU:
 #pragma unroll
-                for (int q = 0; q < VEC; ++q)
-                    if (j + q < p.N) v[q] += to_f32(from[q]);
-            }
-        };
-        if (EPI == kEpiLinear) {
-            const bool zero = zero_rows >> row & 1;
+            for (int q = 0; q < 32; ++q) v[q] = act_silu(v[q]);
+            break;
+        case MSPLAT_ACT_SIGMOID:
 #pragma unroll
-            for (int q = 0; q < VEC; ++q) v[q] = zero ? 0.f : fmaf(v[q], alpha, bias[q]);
-            if (p.preact) put(static_cast<TO*>(p.preact) + i * p.ldz + j);
-            if (p.act != MSPLAT_ACT_NONE) {
-#pragma unroll
-                for (int q = 0; q < VEC; ++q) v[q] = activate(v[q], p.act);
-            }
-            if (p.residual) add(static_cast<const TO*>(p.residual) + i * p.ldr + j);
-            put(static_cast<TO*>(p.out) + i * p.ldo + j);
-        } else if (EPI == kEpiSlab) {
-            TO* to = reinterpret_cast<TO*>(p.slab) + ((int64_t)split * p.M + i) * p.N + j;
-            if (p.accumulate) add(to);
-            put(to);
-        } else {
-            put(static_cast<TO*>(p.out) + i * p.ldo + j);
-        }
+            for (int q = 0; q < 32; ++q) v[q] = act_sigmoid(v[q]);
+            break;
+        default: break;
     }
 }
 
 // What a warp needs of its rows over the columns of a tile: thread = row.
 struct RowState {
     int64_t i;
-    bool in;
+    bool in, zero;
     int32_t target;
-    float lse, top, sum;
-    uint32_t zero_rows;  // kEpiLinear: rows of the warp without a label
-    float alpha;
+    float lse, top, sum, alpha;
 };
 
 template <int EPI>
@@ -261,7 +309,7 @@ __device__ __forceinline__ RowState row_begin(const Product& p, int64_t i0, int 
     r.lse = 0.f;
     r.top = -INFINITY;
     r.sum = 0.f;
-    r.zero_rows = 0;
+    r.zero = false;
     r.alpha = p.alpha;
     if (EPI == kEpiStats || EPI == kEpiGrad) {
         if (r.in) r.target = __ldg(p.targets + r.i);
@@ -269,18 +317,92 @@ __device__ __forceinline__ RowState row_begin(const Product& p, int64_t i0, int 
     }
     if (EPI == kEpiLinear) {
         if (p.alpha_dev) r.alpha *= __ldg(p.alpha_dev);
-        if (p.targets && !p.label_reduces) r.zero_rows = __ballot_sync(~0u, r.in && !labelled(p, r.i));
+        if (p.targets && !p.label_reduces) r.zero = r.in && !labelled(p, r.i);
     }
     return r;
 }
 
-// 32 columns from j0 of the accumulators, one row per thread.
+// Starts the residual's box at (i0, j0) towards the warp's next box. Its store
+// of `ring` boxes ago has been read (bulk_wait_read).
+__device__ __forceinline__ void fetch_residual(const Product& p, const Tiles& tl, const OutMaps& maps, const WarpOut& o,
+                                               int64_t i0, int64_t j0, int lane) {
+    if (!p.residual || !tl.tma_out || j0 >= p.N || i0 >= p.M || lane != 0) return;
+    const int b = o.k % tl.ring;
+    mbar_expect(o.bar + 8 * b, tl.box_bytes);
+    tma_load3(smem_u32(o.y + b * tl.box_bytes), &maps.r, (int)j0, (int)i0, o.bar + 8 * b);
+}
+
+// The end of a product for 32 x 32 results, one row per thread, through the
+// warp's boxes. j_next: the tile's next columns (N or above: none).
+template <typename T, typename TO, int EPI>
+__device__ __forceinline__ bool write32(const Product& p, const Tiles& tl, const OutMaps& maps, WarpOut& o,
+                                        const RowState& r, float (&v)[32], int64_t i0, int64_t j0, int64_t j_next,
+                                        int split, int lane, volatile int* gave_up) {
+    const int b = o.k % tl.ring;
+    uint8_t* y = o.y + b * tl.box_bytes;
+    uint8_t* z = o.z + b * tl.box_bytes;
+    if (EPI == kEpiLinear) {
+        if (p.bias) {
+            o.bias[lane] = j0 + lane < p.N ? to_f32(static_cast<const T*>(p.bias)[j0 + lane]) : 0.f;
+            __syncwarp();
+#pragma unroll
+            for (int q = 0; q < 8; ++q) {
+                const float4 f = reinterpret_cast<const float4*>(o.bias)[q];
+                v[4 * q] = fmaf(v[4 * q], r.alpha, f.x);
+                v[4 * q + 1] = fmaf(v[4 * q + 1], r.alpha, f.y);
+                v[4 * q + 2] = fmaf(v[4 * q + 2], r.alpha, f.z);
+                v[4 * q + 3] = fmaf(v[4 * q + 3], r.alpha, f.w);
+            }
+        } else if (r.alpha != 1.f) {
+#pragma unroll
+            for (int q = 0; q < 32; ++q) v[q] *= r.alpha;
+        }
+        if (r.zero) {
+#pragma unroll
+            for (int q = 0; q < 32; ++q) v[q] = 0.f;
+        }
+        if (p.preact) box_write<TO>(z, lane, v);
+        activate32(v, p.act);
+        if (p.residual) {
+            if (tl.tma_out) {
+                if (!mbar_wait(o.bar + 8 * b, o.phase >> b & 1, gave_up)) return false;
+                o.phase ^= 1u << b;
+            } else {
+                box_copy<TO, true>(y, const_cast<TO*>(static_cast<const TO*>(p.residual)), p.ldr, i0, j0, p.M, p.N, lane);
+                __syncwarp();
+            }
+            box_add<TO>(y, lane, v);
+        }
+    }
+    box_write<TO>(y, lane, v);
+    if (tl.tma_out) {
+        fence_async();
+        __syncwarp();
+        if (lane == 0) {
+            if (EPI == kEpiLinear && p.preact) tma_store(&maps.z, smem_u32(z), (int)j0, (int)i0, 0, false);
+            tma_store(&maps.y, smem_u32(y), (int)j0, (int)i0, split, EPI == kEpiSlab && p.accumulate);
+            bulk_commit();
+            bulk_wait_read(tl.ring - 1);
+        }
+    } else {
+        __syncwarp();
+        if (p.preact) box_copy<TO, false>(z, static_cast<TO*>(p.preact), p.ldz, i0, j0, p.M, p.N, lane);
+        box_copy<TO, false>(y, static_cast<TO*>(p.out), p.ldo, i0, j0, p.M, p.N, lane);
+    }
+    ++o.k;
+    fetch_residual(p, tl, maps, o, i0, j_next, lane);
+    __syncwarp();
+    return true;
+}
+
+// 32 columns from j0 of the accumulators, one row per thread; false when a wait
+// gave up.
 template <typename T, int EPI>
-__device__ __forceinline__ void columns32(const Product& p, const Tiles& tl, RowState& r, float (&v)[32], int64_t i0,
-                                          int64_t j0, int split, float* st, int lane) {
-    if (j0 >= p.N) return;
-    const int n = (int)min((int64_t)32, p.N - j0);
+__device__ __forceinline__ bool columns32(const Product& p, const Tiles& tl, const OutMaps& maps, WarpOut& o,
+                                          RowState& r, float (&v)[32], int64_t i0, int64_t j0, int64_t j_next,
+                                          int split, int lane, volatile int* gave_up) {
     if (EPI == kEpiStats) {
+        const int n = (int)min((int64_t)32, p.N - j0);
         const float to2 = p.logit_scale * kLog2e;
         float top = r.top;
 #pragma unroll
@@ -299,7 +421,7 @@ __device__ __forceinline__ void columns32(const Product& p, const Tiles& tl, Row
         }
         r.top = top;
         r.sum = sum;
-        return;
+        return true;
     }
     if (EPI == kEpiGrad) {
         const float to2 = p.logit_scale * kLog2e;
@@ -309,32 +431,9 @@ __device__ __forceinline__ void columns32(const Product& p, const Tiles& tl, Row
         for (int q = 0; q < 32; ++q)
             v[q] = has ? epi_grad(__fmul_rn(v[q], to2), r.lse, q == at, p.g_scale) : 0.f;
     }
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        if (16 * h >= n) break;
-        float4* row = reinterpret_cast<float4*>(st + lane * kStagePitch);
-#pragma unroll
-        for (int q = 0; q < 4; ++q)
-            row[q] = make_float4(v[16 * h + 4 * q], v[16 * h + 4 * q + 1], v[16 * h + 4 * q + 2], v[16 * h + 4 * q + 3]);
-        __syncwarp();
-        if (EPI == kEpiSlab) {
-            if (tl.vec == 4)
-                flush16<T, float, EPI, 4>(p, st, i0, j0 + 16 * h, split, 0.f, 0, lane);
-            else
-                flush16<T, float, EPI, 1>(p, st, i0, j0 + 16 * h, split, 0.f, 0, lane);
-        } else if (EPI == kEpiLinear && p.out_dtype == MSPLAT_DTYPE_F32) {
-            if (tl.vec == 4)
-                flush16<T, float, EPI, 4>(p, st, i0, j0 + 16 * h, split, r.alpha, r.zero_rows, lane);
-            else
-                flush16<T, float, EPI, 1>(p, st, i0, j0 + 16 * h, split, r.alpha, r.zero_rows, lane);
-        } else {
-            if (tl.vec == 4)
-                flush16<T, T, EPI, 4>(p, st, i0, j0 + 16 * h, split, r.alpha, r.zero_rows, lane);
-            else
-                flush16<T, T, EPI, 1>(p, st, i0, j0 + 16 * h, split, r.alpha, r.zero_rows, lane);
-        }
-        __syncwarp();
-    }
+    if (EPI == kEpiSlab || (EPI == kEpiLinear && sizeof(T) == 2 && p.out_dtype == MSPLAT_DTYPE_F32))
+        return write32<T, float, EPI>(p, tl, maps, o, r, v, i0, j0, j_next, split, lane, gave_up);
+    return write32<T, T, EPI>(p, tl, maps, o, r, v, i0, j0, j_next, split, lane, gave_up);
 }
 
 template <int EPI>
@@ -353,16 +452,43 @@ inline int tile_columns(const Product& p, int widest) {
     return bn;
 }
 
-inline bool aligned4(const void* q, int64_t ld, int64_t rows, int es) {
-    return !q || (reinterpret_cast<uintptr_t>(q) % (4 * es) == 0 && (rows <= 1 || ld % 4 == 0));
+// TMA descriptors (ops_tc16.cu): a [rows, cols] matrix in boxes of 64 columns
+// of 16 bits x box_rows; an output in boxes of 32 x 32, with `layers` matrices
+// of rows * ld elements behind one another.
+CUtensorMap map_operand(const void* base, int64_t rows, int64_t cols, int64_t ld, int box_rows, int dtype);
+CUtensorMap map_output(const void* base, int64_t rows, int64_t cols, int64_t ld, int64_t layers, int dtype);
+bool tma_ready(const void* p, int64_t ld, int64_t rows, int elem);
+
+// Boxes of the outputs and, when TMA can move them, their descriptors.
+inline void set_outputs(const Product& p, Tiles& tl, OutMaps& maps) {
+    if (p.epi == kEpiStats) return;
+    const int dtype = p.epi == kEpiSlab ? MSPLAT_DTYPE_F32 : p.out_dtype, es = dtype_size(dtype);
+    tl.box_bytes = 32 * 32 * es;
+    tl.tma_out = 1;
+    if (p.epi == kEpiSlab) {
+        maps.y = map_output(p.slab, p.M, p.N, slab_ld(p.N), p.splits, dtype);
+        return;
+    }
+    tl.tma_out = tma_ready(p.out, p.ldo, p.M, es) && (!p.preact || tma_ready(p.preact, p.ldz, p.M, es)) &&
+                 (!p.residual || tma_ready(p.residual, p.ldr, p.M, es));
+    if (!tl.tma_out) return;
+    maps.y = map_output(p.out, p.M, p.N, p.ldo, 1, dtype);
+    if (p.preact) maps.z = map_output(p.preact, p.M, p.N, p.ldz, 1, dtype);
+    if (p.residual) maps.r = map_output(p.residual, p.M, p.N, p.ldr, 1, dtype);
 }
-inline int pick_vec(const Product& p) {
-    if (p.epi == kEpiSlab) return p.N % 4 == 0 ? 4 : 1;
-    const int eo = dtype_size(p.out_dtype);
-    return aligned4(p.out, p.ldo, p.M, eo) && aligned4(p.residual, p.ldr, p.M, eo) &&
-                   aligned4(p.preact, p.ldz, p.M, eo)
-               ? 4
-               : 1;
+
+// Shares the block's memory between the stages and `warps` warps' boxes: two
+// boxes per output where that leaves least_stages. Returns the dynamic bytes.
+constexpr int kBlockBytes = 227 * 1024 - 2048;  // without the static part and the alignment of the stages
+inline int share_memory(const Product& p, Tiles& tl, int warps, int fixed, int least_stages, int most_stages) {
+    const int outputs = p.epi == kEpiStats ? 0 : 1 + (p.epi == kEpiLinear && p.preact);
+    for (tl.ring = 2;; --tl.ring) {
+        tl.warp_bytes = tl.ring * outputs * tl.box_bytes;
+        const int rest = kBlockBytes - fixed - warps * tl.warp_bytes;
+        tl.stages = std::min(most_stages, rest / tl.stage_bytes);
+        if (tl.stages >= least_stages || tl.ring == 1) break;
+    }
+    return 1024 + fixed + tl.stages * tl.stage_bytes + warps * tl.warp_bytes;
 }
 
 inline void set_tiles(const Product& p, Tiles& tl) {
@@ -372,7 +498,6 @@ inline void set_tiles(const Product& p, Tiles& tl) {
     tl.tiles_m = (int)tm;
     tl.tiles_n = (int)tn;
     tl.total = (int)total;
-    tl.vec = pick_vec(p);
 }
 
 }  // namespace ops

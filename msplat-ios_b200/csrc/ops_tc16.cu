@@ -9,6 +9,8 @@
 // Either operand may have the reduction across its rows (dx, dw): TMA then
 // brings boxes of 64 x 64 and the instruction reads them transposed, so no
 // operand is ever copied into another layout.
+#include <cstddef>
+
 #include "ops_tc.cuh"
 
 namespace msplat {
@@ -17,24 +19,28 @@ namespace ops {
 namespace {
 
 constexpr int kThreads = 384;
+constexpr int kEpiWarps = 8;
 constexpr int kMaxStages = 8;
 
 struct Smem {
     uint64_t full[kMaxStages], empty[kMaxStages];
-    uint64_t acc_full[2], acc_empty[2], drain;
+    uint64_t acc_full[2], acc_empty[2], drain, residual[kEpiWarps][2];
+    alignas(16) float bias[kEpiWarps][32];
     uint32_t tmem;
     int gave_up;
 };
+static_assert(offsetof(Smem, bias) % 16 == 0 && sizeof(Smem) <= 2048, "read as float4; share_memory counts 2048");
 
 template <typename T, int EPI>
 __global__ void __launch_bounds__(kThreads, 1)
     k_product_tc16(const __grid_constant__ Product p, const __grid_constant__ Tiles tl,
-                   const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b) {
+                   const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+                   const __grid_constant__ OutMaps maps) {
     extern __shared__ __align__(1024) uint8_t dyn[];
     __shared__ Smem sm;
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     uint8_t* tiles = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(dyn) + 1023) & ~(uintptr_t)1023);
-    float* staging = reinterpret_cast<float*>(tiles + (size_t)tl.stages * tl.stage_bytes);
+    uint8_t* boxes = tiles + (size_t)tl.stages * tl.stage_bytes;
     const uint32_t tmem_cols = 2 * tl.bn;
 
     if (threadIdx.x == 0) {
@@ -47,6 +53,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             mbar_init(smem_u32(&sm.acc_empty[q]), kEpiWarps);
         }
         mbar_init(smem_u32(&sm.drain), 1);
+        for (int q = 0; q < 2 * kEpiWarps; ++q) mbar_init(smem_u32(&sm.residual[q / 2][q % 2]), 1);
         sm.gave_up = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -167,27 +174,37 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
     } else if (warp >= 4) {
         const int quarter = warp % 4, half = (warp - 4) / 4;
-        float* st = staging + (warp - 4) * 32 * kStagePitch;
+        WarpOut o;
+        o.y = boxes + (warp - 4) * tl.warp_bytes;
+        o.z = o.y + tl.ring * tl.box_bytes;
+        o.bias = sm.bias[warp - 4];
+        o.bar = smem_u32(sm.residual[warp - 4]);
+        o.phase = 0;
+        o.k = 0;
         int acc = 0;
         uint32_t acc_phase = 0;
-        for (int w = blockIdx.x; w < tl.total; w += gridDim.x) {
+        bool ok = true;
+        for (int w = blockIdx.x; w < tl.total && ok; w += gridDim.x) {
             int tm, tn, split;
             int64_t r0, r1;
             tile_of(p, tl, w, tm, tn, split, r0, r1);
-            const int64_t i0 = (int64_t)tm * kBM + quarter * 32;
+            const int64_t i0 = (int64_t)tm * kBM + quarter * 32, j0 = (int64_t)tn * tl.bn + half * (tl.bn / 2);
+            const int64_t j_end = min(p.N, j0 + tl.bn / 2);
             RowState row = row_begin<EPI>(p, i0, lane);
-            if (!mbar_wait(smem_u32(&sm.acc_full[acc]), acc_phase, gave_up)) break;
+            if (EPI == kEpiLinear && j0 < j_end) fetch_residual(p, tl, maps, o, i0, j0, lane);
+            if (!(ok = mbar_wait(smem_u32(&sm.acc_full[acc]), acc_phase, gave_up))) break;
             tc_fence_after();
             if (i0 < p.M) {
-                for (int c = half * (tl.bn / 2); c < (half + 1) * (tl.bn / 2); c += 32) {
-                    if ((int64_t)tn * tl.bn + c >= p.N) break;
+                const uint32_t d = tmem + ((uint32_t)quarter << 21) + acc * tl.bn + half * (tl.bn / 2);
+                for (int64_t j = j0; j < j_end && ok; j += 32) {
                     uint32_t raw[32];
-                    tmem_load32(tmem + ((uint32_t)quarter << 21) + acc * tl.bn + c, raw);
+                    tmem_load32(d + (uint32_t)(j - j0), raw);
                     tmem_wait();
                     float v[32];
 #pragma unroll
                     for (int q = 0; q < 32; ++q) v[q] = __uint_as_float(raw[q]);
-                    columns32<T, EPI>(p, tl, row, v, i0, (int64_t)tn * tl.bn + c, split, st, lane);
+                    ok = columns32<T, EPI>(p, tl, maps, o, row, v, i0, j, j + 32 < j_end ? j + 32 : p.N, split, lane,
+                                           gave_up);
                 }
                 row_end<EPI>(p, row, 2 * tn + half);
             }
@@ -196,6 +213,11 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (lane == 0) mbar_arrive(smem_u32(&sm.acc_empty[acc]));
             acc ^= 1;
             if (acc == 0) acc_phase ^= 1;
+        }
+        if (EPI != kEpiStats && lane == 0) {
+            bulk_wait_all();
+            if (!ok && p.residual && tl.tma_out)  // a residual's box may be on its way
+                mbar_wait_bounded(o.bar + 8 * (o.k % tl.ring), o.phase >> (o.k % tl.ring) & 1, nullptr);
         }
     }
     __syncwarp();
@@ -219,9 +241,32 @@ EncodeFn encoder() {
     return fn;
 }
 
-// The map of a [rows, cols] matrix read in boxes of 64 columns (128 bytes) x
-// box_rows rows.
-CUtensorMap make_map(const void* base, int64_t rows, int64_t cols, int64_t ld, int box_rows, int dtype) {
+struct Maps {
+    CUtensorMap a, b;
+    OutMaps out;
+};
+
+template <typename T, int EPI>
+void run(const Product& p, const Tiles& tl, const Maps& m, int bytes, cudaStream_t s) {
+    OPS_CK(cudaFuncSetAttribute(k_product_tc16<T, EPI>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    note_launches(1);
+    k_product_tc16<T, EPI><<<std::min(tl.total, kSMs), kThreads, bytes, s>>>(p, tl, m.a, m.b, m.out);
+    OPS_CK(cudaGetLastError());
+}
+
+template <typename T>
+void typed(const Product& p, const Tiles& tl, const Maps& m, int bytes, cudaStream_t s) {
+    switch (p.epi) {
+        case kEpiLinear: return run<T, kEpiLinear>(p, tl, m, bytes, s);
+        case kEpiSlab: return run<T, kEpiSlab>(p, tl, m, bytes, s);
+        case kEpiStats: return run<T, kEpiStats>(p, tl, m, bytes, s);
+        default: return run<T, kEpiGrad>(p, tl, m, bytes, s);
+    }
+}
+
+}  // namespace
+
+CUtensorMap map_operand(const void* base, int64_t rows, int64_t cols, int64_t ld, int box_rows, int dtype) {
     CUtensorMap m;
     const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
     const cuuint64_t strides[1] = {(cuuint64_t)(rows > 1 ? ld * 2 : round_up(cols * 2, 16))};
@@ -234,36 +279,35 @@ CUtensorMap make_map(const void* base, int64_t rows, int64_t cols, int64_t ld, i
     return m;
 }
 
-bool tma_ready(const void* p, int64_t ld, int64_t rows) {
-    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && (rows <= 1 || (ld % 8 == 0 && ld * 2 < (1ll << 40)));
+CUtensorMap map_output(const void* base, int64_t rows, int64_t cols, int64_t ld, int64_t layers, int dtype) {
+    CUtensorMap m;
+    const int es = dtype_size(dtype);
+    const cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)layers};
+    const cuuint64_t row = (cuuint64_t)(rows > 1 || layers > 1 ? ld * es : round_up(cols * es, 16));
+    const cuuint64_t strides[2] = {row, row * (cuuint64_t)rows};
+    const cuuint32_t box[3] = {32, 32, 1}, step[3] = {1, 1, 1};
+    const CUresult r = encoder()(
+        &m, dtype == MSPLAT_DTYPE_F32    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+            : dtype == MSPLAT_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                         : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+        3, const_cast<void*>(base), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+        es == 4 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) throw Error(MSPLAT_ERR_CUDA, "cuTensorMapEncodeTiled failed");
+    return m;
 }
 
-template <typename T, int EPI>
-void run(const Product& p, const Tiles& tl, const CUtensorMap& a, const CUtensorMap& b, cudaStream_t s) {
-    const int bytes = tl.stages * tl.stage_bytes + kStagingBytes + 1024;
-    OPS_CK(cudaFuncSetAttribute(k_product_tc16<T, EPI>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
-    note_launches(1);
-    k_product_tc16<T, EPI><<<std::min(tl.total, kSMs), kThreads, bytes, s>>>(p, tl, a, b);
-    OPS_CK(cudaGetLastError());
+// Strides of a descriptor stay below 2^40 bytes.
+bool tma_ready(const void* p, int64_t ld, int64_t rows, int elem) {
+    return reinterpret_cast<uintptr_t>(p) % 16 == 0 &&
+           (rows <= 1 || (ld * elem % 16 == 0 && ld * elem < (1ll << 40) / rows));
 }
-
-template <typename T>
-void typed(const Product& p, const Tiles& tl, const CUtensorMap& a, const CUtensorMap& b, cudaStream_t s) {
-    switch (p.epi) {
-        case kEpiLinear: return run<T, kEpiLinear>(p, tl, a, b, s);
-        case kEpiSlab: return run<T, kEpiSlab>(p, tl, a, b, s);
-        case kEpiStats: return run<T, kEpiStats>(p, tl, a, b, s);
-        default: return run<T, kEpiGrad>(p, tl, a, b, s);
-    }
-}
-
-}  // namespace
 
 bool gave_up_tc16(cudaStream_t s) { return take_gave_up(s); }
 
 bool can_product_tc16(const Product& p) {
-    return p.dtype != MSPLAT_DTYPE_F32 && tma_ready(p.A, p.lda, p.a_mn ? p.R : p.M) &&
-           tma_ready(p.B, p.ldb, p.b_mn ? p.R : p.N);
+    return p.dtype != MSPLAT_DTYPE_F32 && tma_ready(p.A, p.lda, p.a_mn ? p.R : p.M, 2) &&
+           tma_ready(p.B, p.ldb, p.b_mn ? p.R : p.N, 2);
 }
 
 // the halves of the tiles
@@ -274,16 +318,17 @@ void launch_product_tc16(const Product& p, cudaStream_t s) {
     tl.bn = tile_columns(p, 256);
     set_tiles(p, tl);
     tl.stage_bytes = (kBM + tl.bn) * 128;
-    tl.stages = std::min(kMaxStages, (int)((227 * 1024 - 1024 - 512 - kStagingBytes) / tl.stage_bytes));
     tl.idesc = instr_desc(p.dtype == MSPLAT_DTYPE_BF16, p.a_mn, p.b_mn, tl.bn);
-    const CUtensorMap a = p.a_mn ? make_map(p.A, p.R, p.M, p.lda, kBR, p.dtype)
-                                 : make_map(p.A, p.M, p.R, p.lda, kBM, p.dtype);
-    const CUtensorMap b = p.b_mn ? make_map(p.B, p.R, p.N, p.ldb, kBR, p.dtype)
-                                 : make_map(p.B, p.N, p.R, p.ldb, tl.bn, p.dtype);
+    Maps m{};
+    m.a = p.a_mn ? map_operand(p.A, p.R, p.M, p.lda, kBR, p.dtype) : map_operand(p.A, p.M, p.R, p.lda, kBM, p.dtype);
+    m.b = p.b_mn ? map_operand(p.B, p.R, p.N, p.ldb, kBR, p.dtype)
+                 : map_operand(p.B, p.N, p.R, p.ldb, tl.bn, p.dtype);
+    set_outputs(p, tl, m.out);
+    const int bytes = share_memory(p, tl, kEpiWarps, 0, tl.bn == 256 ? 4 : 5, kMaxStages);
     if (p.dtype == MSPLAT_DTYPE_F16)
-        typed<__half>(p, tl, a, b, s);
+        typed<__half>(p, tl, m, bytes, s);
     else
-        typed<__nv_bfloat16>(p, tl, a, b, s);
+        typed<__nv_bfloat16>(p, tl, m, bytes, s);
 }
 
 }  // namespace ops

@@ -16,6 +16,8 @@
 // 8-15 load, split and store the stages (the layout is TMA's 128-byte swizzle,
 // 64 elements of the reduction per stage), warp 0 issues the products, warps 4-7
 // do the ends of the finished tile from TMEM meanwhile.
+#include <cstddef>
+
 #include "ops_tc.cuh"
 
 namespace msplat {
@@ -24,15 +26,18 @@ namespace {
 
 constexpr int kThreads = 512;
 constexpr int kLoaders = 256;
+constexpr int kEpiWarps = 4;
 constexpr int kMaxStages = 8;
 constexpr int kGroup = 8;  // stages (of 64) that one accumulator takes
 
 struct Smem {
     uint64_t full[kMaxStages], empty[kMaxStages];
-    uint64_t acc_full[2], acc_empty[2], drain;
+    uint64_t acc_full[2], acc_empty[2], drain, residual[kEpiWarps][2];
+    alignas(16) float bias[kEpiWarps][32];
     uint32_t tmem;
     int gave_up;
 };
+static_assert(offsetof(Smem, bias) % 16 == 0 && sizeof(Smem) <= 2048, "read as float4; share_memory counts 2048");
 
 template <typename T>
 constexpr int planes() { return sizeof(T) == 4 ? 3 : 1; }
@@ -128,8 +133,8 @@ __device__ __forceinline__ void store_tile(uint8_t* s, int t, const Chunk<T> (&c
 
 template <typename T, int EPI, int BN>
 __global__ void __launch_bounds__(kThreads, 1)
-    k_product_tcv(const __grid_constant__ Product p, const __grid_constant__ Tiles tl, const bool vec_a,
-                  const bool vec_b) {
+    k_product_tcv(const __grid_constant__ Product p, const __grid_constant__ Tiles tl,
+                  const __grid_constant__ OutMaps maps, const bool vec_a, const bool vec_b) {
     constexpr int P = planes<T>();
     constexpr int kA = P * kBM * 128, kB = P * BN * 128;
     // accumulators of one tile: the groups' and, for split factors, the corrections'
@@ -139,7 +144,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     __shared__ Smem sm;
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     uint8_t* tiles = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(dyn) + 1023) & ~(uintptr_t)1023);
-    float* staging = reinterpret_cast<float*>(tiles + (size_t)tl.stages * (kA + kB));
+    uint8_t* boxes = tiles + (size_t)tl.stages * (kA + kB);
 
     if (threadIdx.x == 0) {
         for (int q = 0; q < tl.stages; ++q) {
@@ -151,6 +156,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             mbar_init(smem_u32(&sm.acc_empty[q]), 4);
         }
         mbar_init(smem_u32(&sm.drain), 1);
+        for (int q = 0; q < 2 * kEpiWarps; ++q) mbar_init(smem_u32(&sm.residual[q / 2][q % 2]), 1);
         sm.gave_up = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -251,22 +257,31 @@ __global__ void __launch_bounds__(kThreads, 1)
             __syncwarp();
         }
     } else if (warp >= 4) {
-        float* st = staging + (warp - 4) * 32 * kStagePitch;
+        WarpOut o;
+        o.y = boxes + (warp - 4) * tl.warp_bytes;
+        o.z = o.y + tl.ring * tl.box_bytes;
+        o.bias = sm.bias[warp - 4];
+        o.bar = smem_u32(sm.residual[warp - 4]);
+        o.phase = 0;
+        o.k = 0;
         int acc = 0;
         uint32_t acc_phase = 0;
-        for (int w = blockIdx.x; w < tl.total; w += gridDim.x) {
+        bool ok = true;
+        for (int w = blockIdx.x; w < tl.total && ok; w += gridDim.x) {
             int tm, tn, split;
             int64_t r0, r1;
             tile_of(p, tl, w, tm, tn, split, r0, r1);
-            const int64_t i0 = (int64_t)tm * kBM + (warp - 4) * 32;
+            const int64_t i0 = (int64_t)tm * kBM + (warp - 4) * 32, j0 = (int64_t)tn * BN;
+            const int64_t j_end = min(p.N, j0 + BN);
             const int groups = (int)min((int64_t)kGroups, (r1 - r0 + kGroup * kBR - 1) / (kGroup * kBR));
             RowState row = row_begin<EPI>(p, i0, lane);
-            if (!mbar_wait(smem_u32(&sm.acc_full[acc]), acc_phase, gave_up)) break;
+            if (EPI == kEpiLinear) fetch_residual(p, tl, maps, o, i0, j0, lane);
+            if (!(ok = mbar_wait(smem_u32(&sm.acc_full[acc]), acc_phase, gave_up))) break;
             tc_fence_after();
             if (i0 < p.M) {
                 const uint32_t d = tmem + ((uint32_t)(warp - 4) << 21) + acc * kTileCols;
-                for (int c = 0; c < BN; c += 32) {
-                    if ((int64_t)tn * BN + c >= p.N) break;
+                for (int64_t j = j0; j < j_end && ok; j += 32) {
+                    const uint32_t c = (uint32_t)(j - j0);
                     uint32_t raw[32];
                     float v[32];
                     if (P > 1) {
@@ -284,7 +299,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                         for (int q = 0; q < 32; ++q) v[q] += __uint_as_float(raw[q]);
                     }
-                    columns32<T, EPI>(p, tl, row, v, i0, (int64_t)tn * BN + c, split, st, lane);
+                    ok = columns32<T, EPI>(p, tl, maps, o, row, v, i0, j, j + 32 < j_end ? j + 32 : p.N, split, lane,
+                                           gave_up);
                 }
                 row_end<EPI>(p, row, tn);
             }
@@ -293,6 +309,11 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (lane == 0) mbar_arrive(smem_u32(&sm.acc_empty[acc]));
             acc ^= 1;
             if (acc == 0) acc_phase ^= 1;
+        }
+        if (EPI != kEpiStats && lane == 0) {
+            bulk_wait_all();
+            if (!ok && p.residual && tl.tma_out)  // a residual's box may be on its way
+                mbar_wait_bounded(o.bar + 8 * (o.k % tl.ring), o.phase >> (o.k % tl.ring) & 1, nullptr);
         }
     }
     __syncwarp();
@@ -309,13 +330,14 @@ bool vectors(const void* q, int64_t ld, int64_t rows) {
 
 template <typename T, int EPI, int BN>
 void run(const Product& p, Tiles tl, cudaStream_t s) {
-    constexpr int stage = planes<T>() * (kBM + BN) * 128, staging = 4 * 32 * kStagePitch * 4;
-    tl.stages = std::min(kMaxStages, (227 * 1024 - 2048 - staging) / stage);
-    const int bytes = tl.stages * stage + staging + 1024;
+    OutMaps maps{};
+    set_outputs(p, tl, maps);
+    tl.stage_bytes = planes<T>() * (kBM + BN) * 128;
+    const int bytes = share_memory(p, tl, kEpiWarps, 0, 2, kMaxStages);
     OPS_CK(cudaFuncSetAttribute(k_product_tcv<T, EPI, BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
     note_launches(1);
     k_product_tcv<T, EPI, BN><<<std::min(tl.total, kSMs), kThreads, bytes, s>>>(
-        p, tl, vectors<T>(p.A, p.lda, p.a_mn ? p.R : p.M), vectors<T>(p.B, p.ldb, p.b_mn ? p.R : p.N));
+        p, tl, maps, vectors<T>(p.A, p.lda, p.a_mn ? p.R : p.M), vectors<T>(p.B, p.ldb, p.b_mn ? p.R : p.N));
     OPS_CK(cudaGetLastError());
 }
 
