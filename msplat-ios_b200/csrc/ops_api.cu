@@ -77,10 +77,21 @@ struct Split {
     int64_t len;
 };
 Split plan_split(int64_t M, int64_t N, int64_t R, int dtype) {
-    const int64_t tiles = ceil_div(M, 128) * ceil_div(N, 128);
-    int64_t s = std::min(ceil_div(R, 512), tiles >= kSMs ? 1 : kSMs / tiles);
-    if (dtype == MSPLAT_DTYPE_F32)
-        s = std::max(s, std::min(ceil_div(R, 1024), std::max<int64_t>(1, kSlabBytes / (M * N * 4))));
+    // the share of the SMs' rounds that has work, with as few pieces as come
+    // within a twentieth of the best
+    const bool exact = dtype == MSPLAT_DTYPE_F32;
+    const int64_t tiles = ceil_div(M, 128) * ceil_div(N, exact ? 128 : N > 128 ? 256 : N > 64 ? 128 : 64);
+    const int64_t most = std::min<int64_t>(ceil_div(R, 512), std::max<int64_t>(1, 2 * kSMs / tiles));
+    int64_t s = 1;
+    double best = 0;
+    for (int64_t q = 1; q <= most; ++q) {
+        const double used = (double)(tiles * q) / (double)(ceil_div(tiles * q, kSMs) * kSMs);
+        if (used > best + 0.05) {
+            best = used;
+            s = q;
+        }
+    }
+    if (exact) s = std::max(s, std::min(ceil_div(R, 1024), std::max<int64_t>(1, kSlabBytes / (M * N * 4))));
     const int64_t len = round_up(ceil_div(R, s), 64);
     return {(int)ceil_div(R, len), len};
 }

@@ -8,44 +8,125 @@ namespace msplat {
 namespace ops {
 namespace {
 
-// A block takes a piece of the rows and 32 columns; eight warps walk the rows.
-template <typename T, int ACT>
+// A block takes a piece of the rows and up to 32 vectors of V columns (16 bytes
+// when the matrices are aligned, else one element); `lanes` threads (a power of
+// two) share a row. Bound by reading z and dy and writing dz: each thread has
+// two rows of both in flight.
+template <typename T, int ACT, int V>
 __global__ void __launch_bounds__(256) k_dz(int64_t m, int64_t n, const T* z, int64_t ldz, const T* dy,
-                                            int64_t lddy, T* dz, int64_t lddz, float* partial, int64_t piece_rows) {
-    __shared__ float sums[8][33];
-    const int64_t j = blockIdx.x * 32 + threadIdx.x;
+                                            int64_t lddy, T* dz, int64_t lddz, float* partial, int64_t piece_rows,
+                                            int lanes) {
+    __shared__ float sums[256 * V];
+    const int cx = threadIdx.x % lanes, ry = threadIdx.x / lanes, rows = 256 / lanes;
+    const int64_t j = ((int64_t)blockIdx.x * lanes + cx) * V;
     const int64_t i0 = blockIdx.y * piece_rows, i1 = min(m, i0 + piece_rows);
-    float sum = 0.f;
-    if (j < n)
-        for (int64_t i = i0 + threadIdx.y; i < i1; i += 8) {
-            float v = to_f32(dy[i * lddy + j]);
-            if (ACT != MSPLAT_ACT_NONE) v *= act_slope<ACT>(to_f32(z[i * ldz + j]));
-            if (dz) dz[i * lddz + j] = from_f32<T>(v);
-            sum += v;
+    union Vec {
+        T t[V];
+        uint4 w;
+        __device__ Vec() {}
+    };
+    float sum[V];
+#pragma unroll
+    for (int q = 0; q < V; ++q) sum[q] = 0.f;
+    // the last vector of an aligned row may end behind the row's last column
+    const int count = V == 1 ? 1 : (int)min((int64_t)V, n - j);
+    auto get = [&](Vec& v, const T* g) {
+        if (V > 1 && count == V) {
+            v.w = __ldg(reinterpret_cast<const uint4*>(g));
+        } else {
+#pragma unroll
+            for (int q = 0; q < V; ++q) v.t[q] = q < count ? g[q] : from_f32<T>(0.f);
         }
-    sums[threadIdx.y][threadIdx.x] = sum;
+    };
+    auto one = [&](const Vec& a, const Vec& b, int64_t i) {
+        Vec o;
+#pragma unroll
+        for (int q = 0; q < V; ++q) {
+            float v = to_f32(a.t[q]);
+            if (ACT != MSPLAT_ACT_NONE) v *= act_slope<ACT>(to_f32(b.t[q]));
+            o.t[q] = from_f32<T>(v);
+            sum[q] += v;
+        }
+        if (!dz) return;
+        T* g = dz + i * lddz + j;
+        if (V > 1 && count == V) {
+            *reinterpret_cast<uint4*>(g) = o.w;
+        } else {
+#pragma unroll
+            for (int q = 0; q < V; ++q)
+                if (q < count) g[q] = o.t[q];
+        }
+    };
+    if (j < n) {
+        int64_t i = i0 + ry;
+        for (; i + rows < i1; i += 2 * rows) {
+            Vec a0, a1, b0, b1;
+            get(a0, dy + i * lddy + j);
+            get(a1, dy + (i + rows) * lddy + j);
+            if (ACT != MSPLAT_ACT_NONE) {
+                get(b0, z + i * ldz + j);
+                get(b1, z + (i + rows) * ldz + j);
+            }
+            one(a0, b0, i);
+            one(a1, b1, i + rows);
+        }
+        if (i < i1) {
+            Vec a0, b0;
+            get(a0, dy + i * lddy + j);
+            if (ACT != MSPLAT_ACT_NONE) get(b0, z + i * ldz + j);
+            one(a0, b0, i);
+        }
+    }
+    if (!partial) return;
+#pragma unroll
+    for (int q = 0; q < V; ++q) sums[(ry * lanes + cx) * V + q] = sum[q];
     __syncthreads();
-    if (partial && threadIdx.y == 0 && j < n) {
+    for (int c = threadIdx.x; c < lanes * V; c += 256) {
+        const int64_t col = (int64_t)blockIdx.x * lanes * V + c;
+        if (col >= n) break;
         float t = 0.f;
-        for (int q = 0; q < 8; ++q) t += sums[q][threadIdx.x];
-        partial[(int64_t)blockIdx.y * n + j] = t;
+        for (int q = 0; q < rows; ++q) t += sums[q * lanes * V + c];
+        partial[(int64_t)blockIdx.y * n + col] = t;
     }
 }
 
+// Threads of a block: `across` consecutive elements (a power of two) x 256 /
+// across shares of the pieces, whose sums are joined through shared memory. Few
+// elements with many pieces (the column sums, a small dw) thus have as many
+// reads in flight as many elements with few.
 template <typename T>
-__global__ void __launch_bounds__(256) k_slab_sum(int64_t rows, int64_t cols, const float* slab, int64_t ld, int pieces, T* out,
-                                                  int64_t ldo, float alpha, const float* alpha_dev,
-                                                  const int32_t* targets, int64_t labels) {
-    const int64_t n = rows * cols;
+__global__ void __launch_bounds__(256) k_slab_sum(int64_t rows, int64_t cols, const float* slab, int64_t ld, int pieces,
+                                                  T* out, int64_t ldo, float alpha, const float* alpha_dev,
+                                                  const int32_t* targets, int64_t labels, int across) {
+    __shared__ float sums[256];
+    const int64_t n = rows * cols, layer = rows * ld;
     const float a = alpha * (alpha_dev ? *alpha_dev : 1.f);
-    for (int64_t e = blockIdx.x * 256ll + threadIdx.x; e < n; e += gridDim.x * 256ll) {
+    const int ex = threadIdx.x % across, share = threadIdx.x / across, shares = 256 / across;
+    for (int64_t e0 = (int64_t)blockIdx.x * across; e0 < n; e0 += (int64_t)gridDim.x * across) {
+        const int64_t e = e0 + ex, i = e < n ? e / cols : 0, j = e < n ? e - i * cols : 0;
+        const float* at = slab + i * ld + j;
         float t = 0.f;
-        const int64_t i = e / cols;
-        const float* at = slab + i * ld + (e - i * cols);
-        for (int q = 0; q < pieces; ++q) t += at[q * rows * ld];
-        t *= a;
-        if (targets && !(targets[i] >= 0 && targets[i] < labels)) t = 0.f;
-        out[i * ldo + (e - i * cols)] = from_f32<T>(t);
+        if (e < n) {
+            int q = share;
+            for (; q + 3 * shares < pieces; q += 4 * shares) {
+                const float v0 = __ldcs(at + q * layer), v1 = __ldcs(at + (q + shares) * layer),
+                            v2 = __ldcs(at + (q + 2 * shares) * layer), v3 = __ldcs(at + (q + 3 * shares) * layer);
+                t += (v0 + v1) + (v2 + v3);
+            }
+            for (; q < pieces; q += shares) t += __ldcs(at + q * layer);
+        }
+        if (shares > 1) {
+            sums[threadIdx.x] = t;
+            __syncthreads();
+            if (share == 0)
+                for (int q = 1; q < shares; ++q) t += sums[q * across + ex];
+            __syncthreads();
+        }
+        if (share == 0 && e < n) {
+            t *= a;
+            if (targets && !(targets[i] >= 0 && targets[i] < labels)) t = 0.f;
+            out[i * ldo + j] = from_f32<T>(t);
+        }
     }
 }
 
@@ -115,31 +196,46 @@ __global__ void __launch_bounds__(256) k_loss_total(const double* partial, int b
     }
 }
 
-template <typename T>
+template <typename T, int V>
 void dz_typed(int64_t m, int64_t n, const void* z, int64_t ldz, int act, const void* dy, int64_t lddy, void* dz,
               int64_t lddz, float* partial, cudaStream_t s) {
     const int pieces = dz_pieces(m, n);
-    const dim3 grid((unsigned)ceil_div(n, 32), pieces);
+    int lanes = 1;
+    while (lanes < 32 && lanes * V < n) lanes *= 2;
+    const dim3 grid((unsigned)ceil_div(n, (int64_t)lanes * V), pieces);
     note_launches(1);
     auto go = [&](auto kernel) {
-        kernel<<<grid, dim3(32, 8), 0, s>>>(m, n, static_cast<const T*>(z), ldz, static_cast<const T*>(dy), lddy,
-                                            static_cast<T*>(dz), lddz, partial, ceil_div(m, pieces));
+        kernel<<<grid, 256, 0, s>>>(m, n, static_cast<const T*>(z), ldz, static_cast<const T*>(dy), lddy,
+                                    static_cast<T*>(dz), lddz, partial, ceil_div(m, pieces), lanes);
     };
     switch (act) {
-        case MSPLAT_ACT_RELU: go(k_dz<T, MSPLAT_ACT_RELU>); break;
-        case MSPLAT_ACT_GELU: go(k_dz<T, MSPLAT_ACT_GELU>); break;
-        case MSPLAT_ACT_SILU: go(k_dz<T, MSPLAT_ACT_SILU>); break;
-        case MSPLAT_ACT_SIGMOID: go(k_dz<T, MSPLAT_ACT_SIGMOID>); break;
-        default: go(k_dz<T, MSPLAT_ACT_NONE>); break;
+        case MSPLAT_ACT_RELU: go(k_dz<T, MSPLAT_ACT_RELU, V>); break;
+        case MSPLAT_ACT_GELU: go(k_dz<T, MSPLAT_ACT_GELU, V>); break;
+        case MSPLAT_ACT_SILU: go(k_dz<T, MSPLAT_ACT_SILU, V>); break;
+        case MSPLAT_ACT_SIGMOID: go(k_dz<T, MSPLAT_ACT_SIGMOID, V>); break;
+        default: go(k_dz<T, MSPLAT_ACT_NONE, V>); break;
     }
     OPS_CK(cudaGetLastError());
+}
+
+template <typename T>
+void dz_any(int64_t m, int64_t n, const void* z, int64_t ldz, int act, const void* dy, int64_t lddy, void* dz,
+            int64_t lddz, float* partial, cudaStream_t s) {
+    constexpr int V = 16 / sizeof(T);
+    auto ready = [&](const void* p, int64_t ld) {
+        return !p || (reinterpret_cast<uintptr_t>(p) % 16 == 0 && (m <= 1 || ld % V == 0));
+    };
+    if (n >= V && ready(dy, lddy) && ready(dz, lddz) && (act == MSPLAT_ACT_NONE || ready(z, ldz)))
+        dz_typed<T, V>(m, n, z, ldz, act, dy, lddy, dz, lddz, partial, s);
+    else
+        dz_typed<T, 1>(m, n, z, ldz, act, dy, lddy, dz, lddz, partial, s);
 }
 
 }  // namespace
 
 int dz_pieces(int64_t m, int64_t n) {
-    // about eight blocks per SM, at least 64 rows each
-    const int64_t want = ceil_div(kSMs * 8, ceil_div(n, 32));
+    // about eight blocks per SM (of 128 to 256 columns), at least 64 rows each
+    const int64_t want = ceil_div(kSMs * 8, ceil_div(n, 256));
     const int64_t most = ceil_div(m, 64);
     return (int)(want < most ? want : most);
 }
@@ -147,27 +243,30 @@ int dz_pieces(int64_t m, int64_t n) {
 void launch_dz(int64_t m, int64_t n, const void* z, int64_t ldz, int act, const void* dy, int64_t lddy, void* dz,
                int64_t lddz, float* partial, int dtype, cudaStream_t s) {
     if (dtype == MSPLAT_DTYPE_F32)
-        dz_typed<float>(m, n, z, ldz, act, dy, lddy, dz, lddz, partial, s);
+        dz_any<float>(m, n, z, ldz, act, dy, lddy, dz, lddz, partial, s);
     else if (dtype == MSPLAT_DTYPE_F16)
-        dz_typed<__half>(m, n, z, ldz, act, dy, lddy, dz, lddz, partial, s);
+        dz_any<__half>(m, n, z, ldz, act, dy, lddy, dz, lddz, partial, s);
     else
-        dz_typed<__nv_bfloat16>(m, n, z, ldz, act, dy, lddy, dz, lddz, partial, s);
+        dz_any<__nv_bfloat16>(m, n, z, ldz, act, dy, lddy, dz, lddz, partial, s);
 }
 
 void launch_slab_sum(int64_t rows, int64_t cols, const float* slab, int64_t ld, int pieces, void* out, int64_t ldo, float alpha,
                      const float* alpha_dev, const int32_t* targets, int64_t labels, int dtype, cudaStream_t s) {
-    const int64_t ctas = ceil_div(rows * cols, 256);
+    // shares of at least four pieces, as long as the blocks do not fill the SMs
+    int across = 256;
+    while (across > 8 && ceil_div(rows * cols, across) < kSMs * 8 && 256 / across * 4 < pieces) across /= 2;
+    const int64_t ctas = ceil_div(rows * cols, across);
     const unsigned grid = (unsigned)(ctas < kSMs * 8 ? ctas : kSMs * 8);
     note_launches(1);
+    auto go = [&](auto* o) {
+        k_slab_sum<<<grid, 256, 0, s>>>(rows, cols, slab, ld, pieces, o, ldo, alpha, alpha_dev, targets, labels, across);
+    };
     if (dtype == MSPLAT_DTYPE_F32)
-        k_slab_sum<float><<<grid, 256, 0, s>>>(rows, cols, slab, ld, pieces, static_cast<float*>(out), ldo, alpha,
-                                               alpha_dev, targets, labels);
+        go(static_cast<float*>(out));
     else if (dtype == MSPLAT_DTYPE_F16)
-        k_slab_sum<__half><<<grid, 256, 0, s>>>(rows, cols, slab, ld, pieces, static_cast<__half*>(out), ldo, alpha,
-                                                alpha_dev, targets, labels);
+        go(static_cast<__half*>(out));
     else
-        k_slab_sum<__nv_bfloat16><<<grid, 256, 0, s>>>(rows, cols, slab, ld, pieces, static_cast<__nv_bfloat16*>(out),
-                                                       ldo, alpha, alpha_dev, targets, labels);
+        go(static_cast<__nv_bfloat16*>(out));
     OPS_CK(cudaGetLastError());
 }
 

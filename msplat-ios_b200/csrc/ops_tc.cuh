@@ -441,14 +441,14 @@ __device__ __forceinline__ void row_end(const Product& p, const RowState& r, int
     if (EPI == kEpiStats && r.in) p.stats[(p.stats_block0 + block) * p.stats_ld + r.i] = make_float2(r.top, r.sum);
 }
 
-// Columns of a tile: the widest that still gives every SM one, and for the
+// Columns of a tile: the widest that still gives three SMs of four one, and for the
 // label statistics a function of the columns alone (stats_block).
 inline int tile_columns(const Product& p, int widest) {
     const int need = p.N > 128 ? 256 : p.N > 64 ? 128 : 64;
     int bn = need < widest ? need : widest;
     if (p.epi == kEpiStats) return bn;
     const int64_t tm = ceil_div(p.M, kBM) * (p.epi == kEpiSlab ? p.splits : 1);
-    while (bn > 64 && tm * ceil_div(p.N, bn) < kSMs) bn /= 2;
+    while (bn > 64 && tm * ceil_div(p.N, bn) < kSMs * 3 / 4) bn /= 2;
     return bn;
 }
 
