@@ -141,6 +141,7 @@ struct Product {
     // are read as zeros of B
     const int32_t* targets;
     int64_t labels;     // number of labels
+    const uint32_t* unlabelled;  // label_reduces: bit r % 32 of word r / 32 is set when r has no label
     int label_reduces;
     int64_t col0;       // label of column 0 of this piece
     float logit_scale;
@@ -186,6 +187,7 @@ struct JoinArgs {
     int64_t labels;
     float* lse;
     float* row_loss;
+    uint32_t* unlabelled; // [ceil(m / 32)] bits
     double* partial;      // [join_blocks(m)][2]
 };
 int join_blocks(int64_t m);

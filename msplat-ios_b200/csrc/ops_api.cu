@@ -140,6 +140,7 @@ struct LossPlan {
     float *lse, *label_logit, *alpha;
     double* partial;
     float2* stats;
+    uint32_t* unlabelled;
     char* g = nullptr;
     float *slab_x = nullptr, *slab_w = nullptr;
     LossPlan(Arena& a, int64_t m, int64_t v, int64_t d, bool grad, int dtype) {
@@ -149,6 +150,7 @@ struct LossPlan {
         alpha = a.take<float>(1);
         lse = a.take<float>(m);
         label_logit = a.take<float>(m);
+        unlabelled = a.take<uint32_t>(ceil_div(m, 64) * 2);
         partial = a.take<double>(2 * ceil_div(m, stats_rows) * join_blocks(stats_rows));
         stats = a.take<float2>(blocks * stats_rows);
         if (!grad) return;
@@ -415,6 +417,7 @@ int msplat_loss_cross_entropy(int64_t m, int64_t v, int64_t d, const void* x, in
             j.targets = targets + r0; j.labels = v;
             j.lse = plan.lse + r0;
             j.row_loss = row_loss ? row_loss + r0 : nullptr;
+            j.unlabelled = plan.unlabelled + r0 / 32;
             j.partial = plan.partial + 2 * joined;
             launch_join(j, s);
             joined += join_blocks(rows);
@@ -454,6 +457,7 @@ int msplat_loss_cross_entropy(int64_t m, int64_t v, int64_t d, const void* x, in
                 q.B = p.A; q.ldb = ldx; q.b_mn = true;
                 q.targets = p.targets;
                 q.label_reduces = 1;
+                q.unlabelled = plan.unlabelled + r0 / 32;
                 launch_gradient(q, plan, plan.slab_w, plan.sw, plan.by_rows, first, last, at(dw, l0 * lddw, es),
                                 lddw, v, dtype, s);
             }

@@ -130,45 +130,70 @@ __global__ void __launch_bounds__(256) k_slab_sum(int64_t rows, int64_t cols, co
     }
 }
 
-__global__ void __launch_bounds__(256) k_join(JoinArgs a) {
-    __shared__ double ssum[256], scount[256];
+// Each warp takes 32 rows (its lanes) and one share of the column blocks;
+// `shares` warps (a power of two) join theirs through shared memory.
+__global__ void __launch_bounds__(1024) k_join(JoinArgs a, int shares) {
+    __shared__ float tops[32][33], sums[32][33];
+    const int lane = threadIdx.x, warp = threadIdx.y, share = warp % shares;
+    const int64_t rows = 32 * (32 / shares);
     double sum = 0, count = 0;
-    for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < a.m; i += gridDim.x * 256ll) {
+    for (int64_t g0 = blockIdx.x * rows; g0 < a.m; g0 += gridDim.x * rows) {
+        const int64_t i0 = g0 + warp / shares * 32, i = i0 + lane;
         // a block whose sum is 0 (columns beyond the last, or logits of -inf
         // only) has no reference; a sum of NaN counts
-        float top = -INFINITY;
-        for (int64_t b = 0; b < a.blocks; ++b) {
-            const float2 v = a.stats[b * a.stats_ld + i];
-            if (v.y != 0.f) top = fmaxf(top, v.x);
+        float top = -INFINITY, total = 0.f;
+        if (i < a.m)
+            for (int64_t b = share; b < a.blocks; b += shares) {
+                const float2 v = __ldcs(a.stats + b * a.stats_ld + i);
+                if (v.y == 0.f) continue;
+                const float t = fmaxf(top, v.x);
+                total = (total == 0.f ? 0.f : total * exp2f(top - t)) + v.y * exp2f(v.x - t);
+                top = t;
+            }
+        tops[warp][lane] = top;
+        sums[warp][lane] = total;
+        if (shares > 1) __syncthreads();
+        if (share == 0) {
+            for (int q = warp + 1; q < warp + shares; ++q) {
+                const float t = fmaxf(top, tops[q][lane]);
+                if (sums[q][lane] == 0.f) continue;
+                total = (total == 0.f ? 0.f : total * exp2f(top - t)) + sums[q][lane] * exp2f(tops[q][lane] - t);
+                top = t;
+            }
+            const int32_t t = i < a.m ? a.targets[i] : -1;
+            const bool has = t >= 0 && t < a.labels;
+            const uint32_t off = __ballot_sync(~0u, !has);
+            if (i < a.m) {
+                const float lse = top + log2f(total);
+                const float row = has ? (lse - a.label_logit[i]) * kLn2 : 0.f;
+                a.lse[i] = lse;
+                if (a.row_loss) a.row_loss[i] = row;
+                if (lane == 0) a.unlabelled[i0 / 32] = off;
+                if (has) {
+                    sum += row;
+                    count += 1;
+                }
+            }
         }
-        float total = 0.f;
-        for (int64_t b = 0; b < a.blocks; ++b) {
-            const float2 v = a.stats[b * a.stats_ld + i];
-            if (v.y != 0.f) total += v.y * exp2f(v.x - top);
-        }
-        const float lse = top + log2f(total);
-        const int32_t t = a.targets[i];
-        const bool has = t >= 0 && t < a.labels;
-        const float row = has ? (lse - a.label_logit[i]) * kLn2 : 0.f;
-        a.lse[i] = lse;
-        if (a.row_loss) a.row_loss[i] = row;
-        if (has) {
-            sum += row;
-            count += 1;
-        }
+        if (shares > 1) __syncthreads();
     }
-    ssum[threadIdx.x] = sum;
-    scount[threadIdx.x] = count;
-    for (int o = 128; o; o >>= 1) {
-        __syncthreads();
-        if (threadIdx.x < o) {
-            ssum[threadIdx.x] += ssum[threadIdx.x + o];
-            scount[threadIdx.x] += scount[threadIdx.x + o];
-        }
+    __shared__ double ssum[32], scount[32];
+    for (int o = 16; o; o >>= 1) {
+        sum += __shfl_xor_sync(~0u, sum, o);
+        count += __shfl_xor_sync(~0u, count, o);
     }
-    if (threadIdx.x == 0) {
-        a.partial[2 * blockIdx.x] = ssum[0];
-        a.partial[2 * blockIdx.x + 1] = scount[0];
+    if (lane == 0) {
+        ssum[warp] = sum;
+        scount[warp] = count;
+    }
+    __syncthreads();
+    if (warp == 0 && lane == 0) {
+        for (int q = 1; q < 32; ++q) {
+            sum += ssum[q];
+            count += scount[q];
+        }
+        a.partial[2 * blockIdx.x] = sum;
+        a.partial[2 * blockIdx.x + 1] = count;
     }
 }
 
@@ -271,13 +296,15 @@ void launch_slab_sum(int64_t rows, int64_t cols, const float* slab, int64_t ld, 
 }
 
 int join_blocks(int64_t m) {
-    const int64_t b = ceil_div(m, 256);
-    return (int)(b < kSMs * 4 ? b : kSMs * 4);
+    const int64_t b = ceil_div(m, 32);
+    return (int)(b < kSMs * 2 ? b : kSMs * 2);
 }
 
 void launch_join(const JoinArgs& a, cudaStream_t s) {
     note_launches(1);
-    k_join<<<join_blocks(a.m), 256, 0, s>>>(a);
+    int shares = 1;
+    while (shares < 32 && shares < a.blocks) shares *= 2;
+    k_join<<<join_blocks(a.m), dim3(32, 32), 0, s>>>(a, shares);
     OPS_CK(cudaGetLastError());
 }
 

@@ -1,6 +1,7 @@
 // ops_tc.cuh — the pieces of the tensor-core kernels: barriers, TMA, tcgen05,
 // and the ends of a product (ops.cuh) for accumulators that live in TMEM.
 #pragma once
+#include <atomic>
 #include <cuda.h>
 
 #include "ops_epilogue.cuh"
@@ -200,6 +201,10 @@ __device__ __forceinline__ void tile_of(const Product& p, const Tiles& tl, int w
         r1 = min(p.R, r0 + p.split_len);
     }
 }
+
+// Dynamic shared memory for stages and boxes: without the static part (2048)
+// and, in kBlockBytes + 1024, with room to align the stages.
+constexpr int kBlockBytes = 227 * 1024 - 2048 - 1024;
 
 // A warp's boxes. A box holds 32 rows of 32 columns, 128 or 64 bytes per row, in
 // TMA's 128- or 64-byte swizzle: a thread writes its row's 16-byte pieces
@@ -402,34 +407,50 @@ __device__ __forceinline__ bool columns32(const Product& p, const Tiles& tl, con
                                           RowState& r, float (&v)[32], int64_t i0, int64_t j0, int64_t j_next,
                                           int split, int lane, volatile int* gave_up) {
     if (EPI == kEpiStats) {
-        const int n = (int)min((int64_t)32, p.N - j0);
         const float to2 = p.logit_scale * kLog2e;
         float top = r.top;
 #pragma unroll
-        for (int q = 0; q < 32; ++q) {
-            v[q] = __fmul_rn(v[q], to2);
-            if (q < n) top = fmaxf(top, v[q]);
+        for (int q = 0; q < 32; ++q) v[q] = __fmul_rn(v[q], to2);
+        if (j0 + 32 > p.N) {
+            const int n = (int)(p.N - j0);
+#pragma unroll
+            for (int q = 0; q < 32; ++q) v[q] = q < n ? v[q] : -INFINITY;
+        }
+#pragma unroll
+        for (int q = 0; q < 32; ++q) top = fmaxf(top, v[q]);
+        const int64_t at = r.target - p.col0 - j0;
+        if (__any_sync(~0u, r.in && at >= 0 && at < 32)) {
+#pragma unroll
+            for (int q = 0; q < 32; ++q)
+                if (q == at && r.in) p.label_logit[r.i] = v[q];
         }
         const float ref = top == -INFINITY ? 0.f : top;
-        float sum = r.sum * (r.top == -INFINITY ? 0.f : exp2f(r.top - ref));
-        if (r.top == -INFINITY && r.sum != 0.f) sum = r.sum;  // NaN stays
-        const int64_t at = r.target - p.col0 - j0;
+        float sum = r.top == -INFINITY ? r.sum : r.sum * exp2_fast(r.top - ref);  // a NaN stays
+        float more[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int q = 0; q < 32; ++q) {
-            if (q < n) sum += exp2f(v[q] - ref);
-            if (q == at && r.in) p.label_logit[r.i] = v[q];
-        }
+        for (int q = 0; q < 32; ++q) more[q % 4] += exp2_fast(v[q] - ref);
         r.top = top;
-        r.sum = sum;
+        r.sum = sum + ((more[0] + more[1]) + (more[2] + more[3]));
         return true;
     }
     if (EPI == kEpiGrad) {
         const float to2 = p.logit_scale * kLog2e;
-        const int64_t at = r.target - p.col0 - j0;
-        const bool has = r.in && r.target >= 0 && r.target < p.labels;
 #pragma unroll
-        for (int q = 0; q < 32; ++q)
-            v[q] = has ? epi_grad(__fmul_rn(v[q], to2), r.lse, q == at, p.g_scale) : 0.f;
+        for (int q = 0; q < 32; ++q) {
+            v[q] = exp2_fast(__fmul_rn(v[q], to2) - r.lse);
+            if (sizeof(T) == 2) v[q] *= p.g_scale;
+        }
+        const int64_t at = r.target - p.col0 - j0;
+        if (__any_sync(~0u, at >= 0 && at < 32)) {
+#pragma unroll
+            for (int q = 0; q < 32; ++q)
+                if (q == at) v[q] -= p.g_scale;
+        }
+        const bool has = r.in && r.target >= 0 && r.target < p.labels;
+        if (__any_sync(~0u, !has)) {
+#pragma unroll
+            for (int q = 0; q < 32; ++q) v[q] = has ? v[q] : 0.f;
+        }
     }
     if (EPI == kEpiSlab || (EPI == kEpiLinear && sizeof(T) == 2 && p.out_dtype == MSPLAT_DTYPE_F32))
         return write32<T, float, EPI>(p, tl, maps, o, r, v, i0, j0, j_next, split, lane, gave_up);
@@ -439,6 +460,19 @@ __device__ __forceinline__ bool columns32(const Product& p, const Tiles& tl, con
 template <int EPI>
 __device__ __forceinline__ void row_end(const Product& p, const RowState& r, int64_t block) {
     if (EPI == kEpiStats && r.in) p.stats[(p.stats_block0 + block) * p.stats_ld + r.i] = make_float2(r.top, r.sum);
+}
+
+// Lets a kernel use all of a block's shared memory, once per kernel (KEY) and
+// device.
+template <typename KEY, typename K>
+void allow_shared(K kernel) {
+    static std::atomic<uint64_t> done{0};
+    int dev = 0;
+    OPS_CK(cudaGetDevice(&dev));
+    const uint64_t bit = 1ull << (dev & 63);
+    if (done.load(std::memory_order_acquire) & bit) return;
+    OPS_CK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kBlockBytes + 1024));
+    done.fetch_or(bit, std::memory_order_release);
 }
 
 // Columns of a tile: the widest that still gives three SMs of four one, and for the
@@ -479,7 +513,6 @@ inline void set_outputs(const Product& p, Tiles& tl, OutMaps& maps) {
 
 // Shares the block's memory between the stages and `warps` warps' boxes: two
 // boxes per output where that leaves least_stages. Returns the dynamic bytes.
-constexpr int kBlockBytes = 227 * 1024 - 2048;  // without the static part and the alignment of the stages
 inline int share_memory(const Product& p, Tiles& tl, int warps, int fixed, int least_stages, int most_stages) {
     const int outputs = p.epi == kEpiStats ? 0 : 1 + (p.epi == kEpiLinear && p.preact);
     for (tl.ring = 2;; --tl.ring) {

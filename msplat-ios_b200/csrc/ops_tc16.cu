@@ -31,6 +31,12 @@ struct Smem {
 };
 static_assert(offsetof(Smem, bias) % 16 == 0 && sizeof(Smem) <= 2048, "read as float4; share_memory counts 2048");
 
+// Bits of the rows r .. r + 63 (r a multiple of 64) without a label.
+__device__ __forceinline__ uint64_t unlabelled64(const Product& p, int64_t r) {
+    const uint32_t* w = p.unlabelled + r / 32;
+    return (uint64_t)__ldg(w) | (r + 32 < p.R ? (uint64_t)__ldg(w + 1) << 32 : 0);
+}
+
 template <typename T, int EPI>
 __global__ void __launch_bounds__(kThreads, 1)
     k_product_tc16(const __grid_constant__ Product p, const __grid_constant__ Tiles tl,
@@ -122,24 +128,26 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (!(ok = mbar_wait(smem_u32(&sm.acc_empty[acc]), acc_phase ^ 1, gave_up))) break;
             tc_fence_after();
             const uint32_t d = tmem + acc * tl.bn;
+            uint64_t off_next = p.label_reduces ? unlabelled64(p, r0) : 0;
             for (int64_t r = r0; r < r1; r += kBR) {
-                // unlabelled rows of x must not reach dw: bit q stands for row r + q
-                uint32_t off0 = 0, off1 = 0;
+                // unlabelled rows of x must not reach dw, even as 0 x NaN: their rows of
+                // the stage are cleared before the products read it
+                uint64_t off = 0;
                 if (p.label_reduces) {
-                    const int64_t a = r + lane, b = a + 32;
-                    off0 = __ballot_sync(~0u, a < p.R && !labelled(p, a));
-                    off1 = __ballot_sync(~0u, b < p.R && !labelled(p, b));
+                    off = off_next;
+                    if (r + kBR < r1) off_next = unlabelled64(p, r + kBR);
                 }
                 if (!(ok = mbar_wait(smem_u32(&sm.full[stage]), phase, gave_up))) break;
                 uint8_t* sa = tiles + (size_t)stage * tl.stage_bytes;
-                if (off0 | off1) {
+                if (off) {
                     uint8_t* sb = sa + kBM * 128;
-                    for (int q = 0; q < kBR; ++q) {
-                        if (!((q < 32 ? off0 >> q : off1 >> (q - 32)) & 1)) continue;
-                        for (int c = lane; c < tl.bn / 8; c += 32)
-                            *reinterpret_cast<uint4*>(sb + (c / 8) * 8192 + q * 128 + (c % 8) * 16) = make_uint4(0, 0, 0, 0);
+                    // eight lanes clear a row's 128 bytes, four column groups at a time
+                    for (; off; off &= off - 1) {
+                        const int q = __ffsll(off) - 1;
+                        for (int g = lane / 8; g < tl.bn / 64; g += 4)
+                            *reinterpret_cast<uint4*>(sb + g * 8192 + q * 128 + lane % 8 * 16) = make_uint4(0, 0, 0, 0);
                     }
-                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    fence_async();
                     __syncwarp();
                 }
                 tc_fence_after();
@@ -241,6 +249,9 @@ EncodeFn encoder() {
     return fn;
 }
 
+template <typename T, int EPI>
+struct Here;  // one kernel
+
 struct Maps {
     CUtensorMap a, b;
     OutMaps out;
@@ -248,7 +259,7 @@ struct Maps {
 
 template <typename T, int EPI>
 void run(const Product& p, const Tiles& tl, const Maps& m, int bytes, cudaStream_t s) {
-    OPS_CK(cudaFuncSetAttribute(k_product_tc16<T, EPI>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    allow_shared<Here<T, EPI>>(k_product_tc16<T, EPI>);
     note_launches(1);
     k_product_tc16<T, EPI><<<std::min(tl.total, kSMs), kThreads, bytes, s>>>(p, tl, m.a, m.b, m.out);
     OPS_CK(cudaGetLastError());

@@ -329,12 +329,15 @@ bool vectors(const void* q, int64_t ld, int64_t rows) {
 }
 
 template <typename T, int EPI, int BN>
+struct Here;  // one kernel
+
+template <typename T, int EPI, int BN>
 void run(const Product& p, Tiles tl, cudaStream_t s) {
     OutMaps maps{};
     set_outputs(p, tl, maps);
     tl.stage_bytes = planes<T>() * (kBM + BN) * 128;
     const int bytes = share_memory(p, tl, kEpiWarps, 0, 2, kMaxStages);
-    OPS_CK(cudaFuncSetAttribute(k_product_tcv<T, EPI, BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    allow_shared<Here<T, EPI, BN>>(k_product_tcv<T, EPI, BN>);
     note_launches(1);
     k_product_tcv<T, EPI, BN><<<std::min(tl.total, kSMs), kThreads, bytes, s>>>(
         p, tl, maps, vectors<T>(p.A, p.lda, p.a_mn ? p.R : p.M), vectors<T>(p.B, p.ldb, p.b_mn ? p.R : p.N));

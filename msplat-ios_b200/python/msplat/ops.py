@@ -63,21 +63,20 @@ def _matrix(t, name, device, dtype, rows=None, cols=None):
     """(address, row stride) of a matrix argument, or (None, 0) for None."""
     if t is None:
         return None, 0
-    if t.device != device or t.device.type != "cuda":
-        _refuse(f"{name} must be on {device}")
     if t.dtype != dtype:
         _refuse(f"{name} must be {dtype}")
-    if t.dim() != 2 or (rows is not None and t.shape != (rows, cols)):
+    if t.device != device:
+        _refuse(f"{name} must be on {device}")
+    shape = t.shape
+    if len(shape) != 2 or (rows is not None and (shape[0] != rows or shape[1] != cols)):
         _refuse(f"{name} must have the shape ({rows}, {cols})" if rows is not None else f"{name} must be a matrix")
-    r, c = t.shape
     s0, s1 = t.stride()
-    if c > 1 and s1 != 1:
+    if s1 != 1 and shape[1] > 1:
         _refuse(f"the columns of {name} must be contiguous")
-    if r > 1:
-        if s0 < c:
+    if s0 < shape[1]:
+        if shape[0] > 1:
             _refuse(f"the rows of {name} overlap")
-    else:
-        s0 = max(s0, c)
+        s0 = shape[1]
     return t.data_ptr(), s0
 
 
@@ -90,11 +89,12 @@ def _vector(t, name, device, dtype, size):
 
 
 def _dtype(x):
-    if not isinstance(x, torch.Tensor) or x.dtype not in _DTYPES:
+    code = _DTYPES.get(x.dtype) if isinstance(x, torch.Tensor) else None
+    if code is None:
         _refuse("float32, float16 or bfloat16 tensors are needed")
-    if x.device.type != "cuda":
+    if not x.is_cuda:
         _refuse("CUDA tensors are needed")
-    return _DTYPES[x.dtype]
+    return code
 
 
 def _act(name):
@@ -102,30 +102,50 @@ def _act(name):
     return code if code is not None else _refuse(f"unknown activation {name!r}")
 
 
-class _On:
-    """The device and stream of a call: makes them current, so that what is
-    allocated belongs to the stream, when they are not."""
+def _enter(device, stream):
+    """Makes the call's device and stream current, where they are not, so that
+    what is allocated belongs to the stream: the contexts to leave again."""
+    entered = []
+    if device.index != torch.cuda.current_device():
+        entered.append(torch.cuda.device(device))
+    if stream is not None:
+        if stream.device != device:
+            _refuse("the stream belongs to another device than the tensors")
+        entered.append(torch.cuda.stream(stream))
+    for c in entered:
+        c.__enter__()
+    return entered
 
-    __slots__ = ("handle", "_ctx")
+
+class _On:
+    """The device and stream of a call. `handle` is the stream's address."""
+
+    __slots__ = ("handle", "_entered")
 
     def __init__(self, device, stream):
-        self._ctx = []
-        if device.index != torch.cuda.current_device():
-            self._ctx.append(torch.cuda.device(device))
-        if stream is not None:
-            if stream.device != device:
-                _refuse("the stream belongs to another device than the tensors")
-            self._ctx.append(torch.cuda.stream(stream))
+        self._entered = _enter(device, stream) if stream is not None or _current_device() != device.index else None
+        self.handle = _raw_stream(device.index)
 
     def __enter__(self):
-        for c in self._ctx:
-            c.__enter__()
-        self.handle = torch.cuda.current_stream().cuda_stream
         return self
 
     def __exit__(self, *a):
-        for c in reversed(self._ctx):
-            c.__exit__(*a)
+        if self._entered:
+            for c in reversed(self._entered):
+                c.__exit__(*a)
+
+
+def _current_device():
+    return torch.cuda.current_device()
+
+
+def _raw_stream(index):
+    return torch.cuda.current_stream(index).cuda_stream
+
+
+# the same without the objects around them, where torch has that
+_current_device = getattr(torch._C, "_cuda_getDevice", _current_device)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _raw_stream)
 
 
 def _workspace(size_fn, device, *args):
