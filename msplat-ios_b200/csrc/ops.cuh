@@ -156,7 +156,7 @@ struct Product {
 // Column blocks that a kEpiStats product leaves statistics of; at most
 // stats_blocks_most(N) for any type and alignment.
 int64_t stats_blocks(const Product& p);
-inline int64_t stats_blocks_most(int64_t n) { return 2 * ceil_div(n, 128); }
+inline int64_t stats_blocks_most(int64_t n) { return 2 * ceil_div(n, 64); }
 
 void launch_product(const Product& p, cudaStream_t s);
 // 16-bit matrices that TMA can address (ops_tc16.cu); everything else (ops_tcv.cu).

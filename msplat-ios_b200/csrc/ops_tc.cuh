@@ -174,7 +174,7 @@ struct Tiles {
     int total;           // with the splits of the reduction
     int stages, stage_bytes;
     uint32_t idesc;
-    int resident;        // the block's columns stay the same (ops_tcv.cu)
+    int resident;        // stages of B that stay in shared memory (ops_tcv.cu)
     // the outputs' boxes of 32 x 32 in shared memory
     int tma_out;         // they move by TMA (16-byte aligned outputs), else element by element
     int ring;            // boxes per output and warp, 1 or 2
@@ -518,8 +518,8 @@ inline int share_memory(const Product& p, Tiles& tl, int warps, int fixed, int l
     for (tl.ring = 2;; --tl.ring) {
         tl.warp_bytes = tl.ring * outputs * tl.box_bytes;
         const int rest = kBlockBytes - fixed - warps * tl.warp_bytes;
-        tl.stages = std::min(most_stages, rest / tl.stage_bytes);
-        if (tl.stages >= least_stages || tl.ring == 1) break;
+        tl.stages = rest > 0 ? std::min(most_stages, rest / tl.stage_bytes) : 0;
+        if ((rest > 0 && tl.stages >= least_stages) || tl.ring == 1) break;
     }
     return 1024 + fixed + tl.stages * tl.stage_bytes + warps * tl.warp_bytes;
 }

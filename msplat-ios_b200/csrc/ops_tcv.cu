@@ -13,9 +13,11 @@
 // rounding at the end.
 //
 // A block owns 128 x bn tiles (bn 64 or 128) and walks its share of them. Warps
-// 8-15 load, split and store the stages (the layout is TMA's 128-byte swizzle,
-// 64 elements of the reduction per stage), warp 0 issues the products, warps 4-7
-// do the ends of the finished tile from TMEM meanwhile.
+// 12-19 load, split and store the stages (the layout is TMA's 128-byte swizzle,
+// 64 elements of the reduction per stage), warp 0 issues the products, warps
+// 4-11 do the ends of the finished tile from TMEM meanwhile. When the parts of B
+// for a tile's columns fit beside the stages (a layer's weights for many rows), a
+// block keeps to one column of tiles and loads them once (resident).
 #include <cstddef>
 
 #include "ops_tc.cuh"
@@ -24,9 +26,14 @@ namespace msplat {
 namespace ops {
 namespace {
 
-constexpr int kThreads = 512;
+constexpr int kThreads = 640;
 constexpr int kLoaders = 256;
-constexpr int kEpiWarps = 4;
+constexpr int kEpiWarps = 8;
+constexpr int kLoadWarp = 12;  // the first of the loaders
+// Registers per thread of the three kinds of warps, out of the launch's 96 x
+// 640: 128 x 40 + 256 x 128 + 256 x 88 = 60416 of 61440.
+constexpr int kIssueRegs = 40, kEpiRegs = 128, kLoadRegs = 88;
+static_assert(128 * kIssueRegs + 256 * kEpiRegs + 256 * kLoadRegs <= kThreads * 96, "setmaxnreg would wait forever");
 constexpr int kMaxStages = 8;
 constexpr int kGroup = 8;  // stages (of 64) that one accumulator takes
 
@@ -140,11 +147,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     // accumulators of one tile: the groups' and, for split factors, the corrections'
     constexpr int kGroups = 512 / 2 / BN - (P > 1 ? 1 : 0);
     constexpr int kTileCols = 256;
+    const int stage_bytes = tl.stage_bytes;  // A, and B unless it is resident
     extern __shared__ __align__(1024) uint8_t dyn[];
     __shared__ Smem sm;
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     uint8_t* tiles = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(dyn) + 1023) & ~(uintptr_t)1023);
-    uint8_t* boxes = tiles + (size_t)tl.stages * (kA + kB);
+    uint8_t* resident = tiles + (size_t)tl.stages * stage_bytes;
+    uint8_t* boxes = resident + (size_t)tl.resident * kB;
 
     if (threadIdx.x == 0) {
         for (int q = 0; q < tl.stages; ++q) {
@@ -153,7 +162,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         for (int q = 0; q < 2; ++q) {
             mbar_init(smem_u32(&sm.acc_full[q]), 1);
-            mbar_init(smem_u32(&sm.acc_empty[q]), 4);
+            mbar_init(smem_u32(&sm.acc_empty[q]), kEpiWarps);
         }
         mbar_init(smem_u32(&sm.drain), 1);
         for (int q = 0; q < 2 * kEpiWarps; ++q) mbar_init(smem_u32(&sm.residual[q / 2][q % 2]), 1);
@@ -167,12 +176,18 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t tmem = sm.tmem;
     volatile int* gave_up = &sm.gave_up;
 
-    if (warp >= 8) {
-        const int t = threadIdx.x - 256;
+    if (warp >= kLoadWarp) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kLoadRegs));
+        const int t = threadIdx.x - kLoadWarp * 32;
         const Operand<T> oa{static_cast<const T*>(p.A), p.lda, p.a_mn ? p.R : p.M, p.a_mn ? p.M : p.R, p.a_mn, vec_a,
                             nullptr};
         const Operand<T> ob{static_cast<const T*>(p.B), p.ldb, p.b_mn ? p.R : p.N, p.b_mn ? p.N : p.R, p.b_mn, vec_b,
                             p.label_reduces ? &p : nullptr};
+        for (int q = 0; q < tl.resident; ++q) {
+            Chunk<T> b[BN / 32];
+            load_tile<T, BN>(ob, (int64_t)(blockIdx.x % tl.tiles_n) * BN, (int64_t)q * kBR, t, b);
+            store_tile<T, BN>(resident + (size_t)q * kB, t, b);
+        }
         int stage = 0;
         uint32_t phase = 0;
         bool ok = true;
@@ -183,12 +198,12 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int64_t r = r0; r < r1; r += kBR) {
                 Chunk<T> a[kBM / 32], b[BN / 32];
                 load_tile<T, kBM>(oa, (int64_t)tm * kBM, r, t, a);
-                load_tile<T, BN>(ob, (int64_t)tn * BN, r, t, b);
+                if (!tl.resident) load_tile<T, BN>(ob, (int64_t)tn * BN, r, t, b);
                 if (!(ok = mbar_wait(smem_u32(&sm.empty[stage]), phase ^ 1, gave_up))) break;
-                uint8_t* s = tiles + (size_t)stage * (kA + kB);
+                uint8_t* s = tiles + (size_t)stage * stage_bytes;
                 store_tile<T, kBM>(s, t, a);
-                store_tile<T, BN>(s + kA, t, b);
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                if (!tl.resident) store_tile<T, BN>(s + kA, t, b);
+                fence_async();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(smem_u32(&sm.full[stage]));
                 if (++stage == tl.stages) {
@@ -197,11 +212,12 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
             }
         }
-    } else if (warp == 0) {
+    } else if (warp < 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssueRegs));
         int stage = 0, acc = 0;
         uint32_t phase = 0, acc_phase = 0;
         bool ok = true;
-        for (int w = blockIdx.x; w < tl.total && ok; w += gridDim.x) {
+        for (int w = blockIdx.x; w < tl.total && ok && warp == 0; w += gridDim.x) {
             int tm, tn, split;
             int64_t r0, r1;
             tile_of(p, tl, w, tm, tn, split, r0, r1);
@@ -213,7 +229,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (!(ok = mbar_wait(smem_u32(&sm.full[stage]), phase, gave_up))) break;
                 tc_fence_after();
                 if (elect_one()) {
-                    const uint32_t a = smem_u32(tiles + (size_t)stage * (kA + kB)), b = a + kA;
+                    const uint32_t a = smem_u32(tiles + (size_t)stage * stage_bytes);
+                    const uint32_t b = tl.resident ? smem_u32(resident) + block * kB : a + kA;
                     const uint32_t step_a = p.a_mn ? 2048 >> 4 : 32 >> 4, step_b = p.b_mn ? 2048 >> 4 : 32 >> 4;
                     uint64_t da[P], db[P];
 #pragma unroll
@@ -223,8 +240,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                     const int group = min(block / kGroup, kGroups - 1);
                     const bool fresh = block % kGroup == 0 && block / kGroup < kGroups;
-#pragma unroll
-                    for (int k = 0; k < kBR / 16; ++k) {
+                    const int steps = (int)min((int64_t)(kBR / 16), (r1 - r + 15) / 16);
+                    for (int k = 0; k < steps; ++k) {
                         if (P > 1) {
                             const int pa[5] = {0, 2, 1, 0, 1}, pb[5] = {2, 0, 1, 1, 0};
 #pragma unroll
@@ -256,7 +273,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             __syncwarp();
         }
-    } else if (warp >= 4) {
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kEpiRegs));
+        const int quarter = warp % 4, half = (warp - 4) / 4;
+        constexpr int kHalf = BN / 2;
         WarpOut o;
         o.y = boxes + (warp - 4) * tl.warp_bytes;
         o.z = o.y + tl.ring * tl.box_bytes;
@@ -271,15 +291,15 @@ __global__ void __launch_bounds__(kThreads, 1)
             int tm, tn, split;
             int64_t r0, r1;
             tile_of(p, tl, w, tm, tn, split, r0, r1);
-            const int64_t i0 = (int64_t)tm * kBM + (warp - 4) * 32, j0 = (int64_t)tn * BN;
-            const int64_t j_end = min(p.N, j0 + BN);
+            const int64_t i0 = (int64_t)tm * kBM + quarter * 32, j0 = (int64_t)tn * BN + half * kHalf;
+            const int64_t j_end = min(p.N, j0 + kHalf);
             const int groups = (int)min((int64_t)kGroups, (r1 - r0 + kGroup * kBR - 1) / (kGroup * kBR));
             RowState row = row_begin<EPI>(p, i0, lane);
-            if (EPI == kEpiLinear) fetch_residual(p, tl, maps, o, i0, j0, lane);
+            if (EPI == kEpiLinear && j0 < j_end) fetch_residual(p, tl, maps, o, i0, j0, lane);
             if (!(ok = mbar_wait(smem_u32(&sm.acc_full[acc]), acc_phase, gave_up))) break;
             tc_fence_after();
             if (i0 < p.M) {
-                const uint32_t d = tmem + ((uint32_t)(warp - 4) << 21) + acc * kTileCols;
+                const uint32_t d = tmem + ((uint32_t)quarter << 21) + acc * kTileCols + half * kHalf;
                 for (int64_t j = j0; j < j_end && ok; j += 32) {
                     const uint32_t c = (uint32_t)(j - j0);
                     uint32_t raw[32];
@@ -302,7 +322,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     ok = columns32<T, EPI>(p, tl, maps, o, row, v, i0, j, j + 32 < j_end ? j + 32 : p.N, split, lane,
                                            gave_up);
                 }
-                row_end<EPI>(p, row, tn);
+                row_end<EPI>(p, row, 2 * tn + half);
             }
             tc_fence_before();
             __syncwarp();
@@ -335,11 +355,26 @@ template <typename T, int EPI, int BN>
 void run(const Product& p, Tiles tl, cudaStream_t s) {
     OutMaps maps{};
     set_outputs(p, tl, maps);
-    tl.stage_bytes = planes<T>() * (kBM + BN) * 128;
-    const int bytes = share_memory(p, tl, kEpiWarps, 0, 2, kMaxStages);
+    constexpr int a_bytes = planes<T>() * kBM * 128, b_bytes = planes<T>() * BN * 128;
+    // B's parts stay when a block has several tiles and they leave two stages of A
+    const int64_t blocks = ceil_div(p.R, kBR);
+    tl.resident = 0;
+    int grid = std::min(tl.total, kSMs), bytes = 0;
+    if (EPI != kEpiSlab && tl.total > kSMs && tl.tiles_n <= kSMs && blocks * b_bytes <= kBlockBytes) {
+        tl.stage_bytes = a_bytes;
+        bytes = share_memory(p, tl, kEpiWarps, (int)blocks * b_bytes, 2, kMaxStages);
+        if (tl.stages >= 2) {
+            tl.resident = (int)blocks;
+            grid = kSMs / tl.tiles_n * tl.tiles_n;
+        }
+    }
+    if (!tl.resident) {
+        tl.stage_bytes = a_bytes + b_bytes;
+        bytes = share_memory(p, tl, kEpiWarps, 0, 2, kMaxStages);
+    }
     allow_shared<Here<T, EPI, BN>>(k_product_tcv<T, EPI, BN>);
     note_launches(1);
-    k_product_tcv<T, EPI, BN><<<std::min(tl.total, kSMs), kThreads, bytes, s>>>(
+    k_product_tcv<T, EPI, BN><<<grid, kThreads, bytes, s>>>(
         p, tl, maps, vectors<T>(p.A, p.lda, p.a_mn ? p.R : p.M), vectors<T>(p.B, p.ldb, p.b_mn ? p.R : p.N));
     OPS_CK(cudaGetLastError());
 }
@@ -374,7 +409,8 @@ int columns_tcv(const Product& p) {
 
 bool gave_up_tcv(cudaStream_t s) { return take_gave_up(s); }
 
-int64_t stats_blocks_tcv(const Product& p) { return ceil_div(p.N, columns_tcv(p)); }
+// the halves of the tiles
+int64_t stats_blocks_tcv(const Product& p) { return 2 * ceil_div(p.N, columns_tcv(p)); }
 
 void launch_product_tcv(const Product& p, cudaStream_t s) {
     Tiles tl{};
