@@ -53,6 +53,21 @@ __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { retu
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
+// 2^x with the special function unit alone (2 units in the last place; results
+// below 2^-126 are 0).
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// 1 / x with the special function unit alone (1 unit in the last place).
+__device__ __forceinline__ float recip_fast(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
 // The Gaussian distribution function through the error function's
 // approximation 7.1.26 of Abramowitz and Stegun, Handbook of Mathematical
 // Functions: erfc(x) = t (a1 + t (a2 + ...)) exp(-x^2), t = 1 / (1 + p x), off by
@@ -60,8 +75,8 @@ constexpr float kLn2 = 0.6931471805599453f;
 // polynomials. *density: exp(-z^2 / 2).
 __device__ __forceinline__ float normal_cdf(float z, float* density) {
     const float x = fabsf(z) * 0.70710678118654752f;
-    const float t = __fdividef(1.f, fmaf(0.3275911f, x, 1.f));
-    const float e = exp2f(-kLog2e * x * x);
+    const float t = recip_fast(fmaf(0.3275911f, x, 1.f));
+    const float e = exp2_fast(-kLog2e * x * x);
     float q = fmaf(1.061405429f, t, -1.453152027f);
     q = fmaf(q, t, 1.421413741f);
     q = fmaf(q, t, -0.284496736f);
@@ -70,7 +85,7 @@ __device__ __forceinline__ float normal_cdf(float z, float* density) {
     *density = e;
     return z < 0.f ? q : 1.f - q;
 }
-__device__ __forceinline__ float logistic(float z) { return __fdividef(1.f, 1.f + exp2f(-kLog2e * z)); }
+__device__ __forceinline__ float logistic(float z) { return recip_fast(1.f + exp2_fast(-kLog2e * z)); }
 
 __device__ __forceinline__ float act_relu(float z) { return z < 0.f ? 0.f : z; }
 __device__ __forceinline__ float act_gelu(float z) {

@@ -337,6 +337,11 @@ __device__ __forceinline__ void fetch_residual(const Product& p, const Tiles& tl
     tma_load3(smem_u32(o.y + b * tl.box_bytes), &maps.r, (int)j0, (int)i0, o.bar + 8 * b);
 }
 
+__device__ __forceinline__ void boxes_free(const Tiles& tl, int lane) {
+    if (lane == 0) bulk_wait_read(tl.ring - 1);
+    __syncwarp();
+}
+
 // The end of a product for 32 x 32 results, one row per thread, through the
 // warp's boxes. j_next: the tile's next columns (N or above: none).
 template <typename T, typename TO, int EPI>
@@ -346,6 +351,9 @@ __device__ __forceinline__ bool write32(const Product& p, const Tiles& tl, const
     const int b = o.k % tl.ring;
     uint8_t* y = o.y + b * tl.box_bytes;
     uint8_t* z = o.z + b * tl.box_bytes;
+    // the boxes are free once the store of `ring` boxes ago has read them; with a
+    // residual that wait came before its fetch
+    const bool free_now = EPI == kEpiLinear && p.residual;
     if (EPI == kEpiLinear) {
         if (p.bias) {
             o.bias[lane] = j0 + lane < p.N ? to_f32(static_cast<const T*>(p.bias)[j0 + lane]) : 0.f;
@@ -366,7 +374,10 @@ __device__ __forceinline__ bool write32(const Product& p, const Tiles& tl, const
 #pragma unroll
             for (int q = 0; q < 32; ++q) v[q] = 0.f;
         }
-        if (p.preact) box_write<TO>(z, lane, v);
+        if (p.preact) {
+            if (tl.tma_out && !free_now) boxes_free(tl, lane);
+            box_write<TO>(z, lane, v);
+        }
         activate32(v, p.act);
         if (p.residual) {
             if (tl.tma_out) {
@@ -379,6 +390,7 @@ __device__ __forceinline__ bool write32(const Product& p, const Tiles& tl, const
             box_add<TO>(y, lane, v);
         }
     }
+    if (tl.tma_out && !free_now && !(EPI == kEpiLinear && p.preact)) boxes_free(tl, lane);
     box_write<TO>(y, lane, v);
     if (tl.tma_out) {
         fence_async();
@@ -387,7 +399,7 @@ __device__ __forceinline__ bool write32(const Product& p, const Tiles& tl, const
             if (EPI == kEpiLinear && p.preact) tma_store(&maps.z, smem_u32(z), (int)j0, (int)i0, 0, false);
             tma_store(&maps.y, smem_u32(y), (int)j0, (int)i0, split, EPI == kEpiSlab && p.accumulate);
             bulk_commit();
-            bulk_wait_read(tl.ring - 1);
+            if (free_now) bulk_wait_read(tl.ring - 1);
         }
     } else {
         __syncwarp();
@@ -409,6 +421,8 @@ __device__ __forceinline__ bool columns32(const Product& p, const Tiles& tl, con
     if (EPI == kEpiStats) {
         const float to2 = p.logit_scale * kLog2e;
         float top = r.top;
+        // rounded products here and in the gradient, never part of a fused
+        // multiply-add: at large logits one bit of them is a large difference
 #pragma unroll
         for (int q = 0; q < 32; ++q) v[q] = __fmul_rn(v[q], to2);
         if (j0 + 32 > p.N) {
