@@ -175,10 +175,9 @@ struct Tiles {
     int stages, stage_bytes;
     uint32_t idesc;
     int resident;        // stages of B that stay in shared memory (ops_tcv.cu)
-    // the outputs' boxes of 32 x 32 in shared memory
+    // the outputs' boxes in shared memory
     int tma_out;         // they move by TMA (16-byte aligned outputs), else element by element
     int ring;            // boxes per output and warp, 1 or 2
-    int box_bytes;       // 2048 or 4096
     int warp_bytes;      // what a warp needs: boxes of y and preact
 };
 
@@ -206,10 +205,12 @@ __device__ __forceinline__ void tile_of(const Product& p, const Tiles& tl, int w
 // and, in kBlockBytes + 1024, with room to align the stages.
 constexpr int kBlockBytes = 227 * 1024 - 2048 - 1024;
 
-// A warp's boxes. A box holds 32 rows of 32 columns, 128 or 64 bytes per row, in
-// TMA's 128- or 64-byte swizzle: a thread writes its row's 16-byte pieces
-// without bank conflicts and one instruction stores the box, clipped at the
-// matrix' edges.
+// A warp's boxes. A box holds 32 rows of 128 bytes (32 or 64 columns) in TMA's
+// 128-byte swizzle: a thread writes its row's 16-byte pieces without bank
+// conflicts and one instruction stores the box, clipped at the matrix' edges.
+// (Rows of 64 bytes halve what the TMA unit stores per clock: 65536 x 1024 bf16
+// from a reduction of 64 took 53 us with them.)
+constexpr int kBoxBytes = 32 * 128;
 struct WarpOut {
     uint8_t* y;       // ring boxes
     uint8_t* z;       // ring boxes, with preact
@@ -219,54 +220,81 @@ struct WarpOut {
     int k;            // boxes done
 };
 
+__device__ __forceinline__ uint32_t box_piece(int row, int piece) { return row * 128 + ((piece ^ (row & 7)) << 4); }
+// Two values rounded into one 32-bit word of a 16-bit type, and back.
 template <typename TO>
-__device__ __forceinline__ uint32_t box_piece(int row, int piece) {
-    return sizeof(TO) == 4 ? row * 128 + ((piece ^ (row & 7)) << 4) : row * 64 + ((piece ^ (row >> 1 & 3)) << 4);
+__device__ __forceinline__ uint32_t pack2(float a, float b);
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
 }
 template <typename TO>
-__device__ __forceinline__ TO* box_at(uint8_t* box, int row, int col) {
-    constexpr int n = 16 / sizeof(TO);
-    return reinterpret_cast<TO*>(box + box_piece<TO>(row, col / n)) + col % n;
+__device__ __forceinline__ float2 unpack2(uint32_t w);
+template <>
+__device__ __forceinline__ float2 unpack2<__half>(uint32_t w) {
+    return __half22float2(*reinterpret_cast<const __half2*>(&w));
 }
+template <>
+__device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t w) {
+    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
+}
+// 32 columns of a row from piece `first` on
 template <typename TO>
-struct Piece {
-    union {
-        uint4 w;
-        TO t[16 / sizeof(TO)];
-    };
-    __device__ __forceinline__ Piece() {}
-};
-template <typename TO>
-__device__ __forceinline__ void box_write(uint8_t* box, int row, const float (&v)[32]) {
-    constexpr int n = 16 / sizeof(TO);
+__device__ __forceinline__ void box_write(uint8_t* box, int row, int first, const float (&v)[32]) {
+    if constexpr (sizeof(TO) == 4) {
 #pragma unroll
-    for (int q = 0; q < 32 / n; ++q) {
-        Piece<TO> o;
+        for (int q = 0; q < 8; ++q)
+            *reinterpret_cast<float4*>(box + box_piece(row, first + q)) =
+                make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+    } else {
 #pragma unroll
-        for (int e = 0; e < n; ++e) o.t[e] = from_f32<TO>(v[q * n + e]);
-        *reinterpret_cast<uint4*>(box + box_piece<TO>(row, q)) = o.w;
+        for (int q = 0; q < 4; ++q)
+            *reinterpret_cast<uint4*>(box + box_piece(row, first + q)) =
+                make_uint4(pack2<TO>(v[8 * q], v[8 * q + 1]), pack2<TO>(v[8 * q + 2], v[8 * q + 3]),
+                           pack2<TO>(v[8 * q + 4], v[8 * q + 5]), pack2<TO>(v[8 * q + 6], v[8 * q + 7]));
     }
 }
 template <typename TO>
-__device__ __forceinline__ void box_add(const uint8_t* box, int row, float (&v)[32]) {
-    constexpr int n = 16 / sizeof(TO);
+__device__ __forceinline__ void box_add(const uint8_t* box, int row, int first, float (&v)[32]) {
+    if constexpr (sizeof(TO) == 4) {
 #pragma unroll
-    for (int q = 0; q < 32 / n; ++q) {
-        Piece<TO> o;
-        o.w = *reinterpret_cast<const uint4*>(box + box_piece<TO>(row, q));
+        for (int q = 0; q < 8; ++q) {
+            const float4 f = *reinterpret_cast<const float4*>(box + box_piece(row, first + q));
+            v[4 * q] += f.x;
+            v[4 * q + 1] += f.y;
+            v[4 * q + 2] += f.z;
+            v[4 * q + 3] += f.w;
+        }
+    } else {
 #pragma unroll
-        for (int e = 0; e < n; ++e) v[q * n + e] += to_f32(o.t[e]);
+        for (int q = 0; q < 4; ++q) {
+            const uint4 w = *reinterpret_cast<const uint4*>(box + box_piece(row, first + q));
+            const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float2 f = unpack2<TO>(u[e]);
+                v[8 * q + 2 * e] += f.x;
+                v[8 * q + 2 * e + 1] += f.y;
+            }
+        }
     }
 }
-// Element by element between a box and rows i0 .., columns j0 .. of a matrix:
-// consecutive lanes take consecutive elements.
+// Element by element between 32 columns of a box and rows i0 .., columns j0 ..
+// of a matrix: consecutive lanes take consecutive elements.
 template <typename TO, bool IN>
-__device__ __forceinline__ void box_copy(uint8_t* box, TO* g, int64_t ld, int64_t i0, int64_t j0, int64_t M, int64_t N,
-                                         int lane) {
+__device__ __forceinline__ void box_copy(uint8_t* box, int first, TO* g, int64_t ld, int64_t i0, int64_t j0, int64_t M,
+                                         int64_t N, int lane) {
+    constexpr int per = 16 / sizeof(TO);
     const int n = (int)min((int64_t)32, N - j0), rows = (int)min((int64_t)32, M - i0);
     for (int e = lane; e < rows * n; e += 32) {
         const int r = e / n, c = e - r * n;
-        TO* b = box_at<TO>(box, r, c);
+        TO* b = reinterpret_cast<TO*>(box + box_piece(r, first + c / per)) + c % per;
         TO* m = g + (i0 + r) * ld + j0 + c;
         if (IN)
             *b = *m;
@@ -333,8 +361,8 @@ __device__ __forceinline__ void fetch_residual(const Product& p, const Tiles& tl
                                                int64_t i0, int64_t j0, int lane) {
     if (!p.residual || !tl.tma_out || j0 >= p.N || i0 >= p.M || lane != 0) return;
     const int b = o.k % tl.ring;
-    mbar_expect(o.bar + 8 * b, tl.box_bytes);
-    tma_load3(smem_u32(o.y + b * tl.box_bytes), &maps.r, (int)j0, (int)i0, o.bar + 8 * b);
+    mbar_expect(o.bar + 8 * b, kBoxBytes);
+    tma_load3(smem_u32(o.y + b * kBoxBytes), &maps.r, (int)j0, (int)i0, o.bar + 8 * b);
 }
 
 __device__ __forceinline__ void boxes_free(const Tiles& tl, int lane) {
@@ -343,14 +371,20 @@ __device__ __forceinline__ void boxes_free(const Tiles& tl, int lane) {
 }
 
 // The end of a product for 32 x 32 results, one row per thread, through the
-// warp's boxes. j_next: the tile's next columns (N or above: none).
+// warp's boxes. j_begin: the warp's first columns of the tile; j_next: the tile's next columns (N or above: none).
 template <typename T, typename TO, int EPI>
 __device__ __forceinline__ bool write32(const Product& p, const Tiles& tl, const OutMaps& maps, WarpOut& o,
-                                        const RowState& r, float (&v)[32], int64_t i0, int64_t j0, int64_t j_next,
+                                        const RowState& r, float (&v)[32], int64_t i0, int64_t j_begin, int64_t j0,
+                                          int64_t j_next,
                                         int split, int lane, volatile int* gave_up) {
+    // 16-bit boxes take two calls: the second fills and sends the box
+    constexpr bool kTwo = sizeof(TO) == 2;
+    const bool second = kTwo && ((j0 - j_begin) & 32);
+    const bool send = !kTwo || second || j_next >= p.N;
+    const int first = second ? 4 : 0;
     const int b = o.k % tl.ring;
-    uint8_t* y = o.y + b * tl.box_bytes;
-    uint8_t* z = o.z + b * tl.box_bytes;
+    uint8_t* y = o.y + b * kBoxBytes;
+    uint8_t* z = o.z + b * kBoxBytes;
     // the boxes are free once the store of `ring` boxes ago has read them; with a
     // residual that wait came before its fetch
     const bool free_now = EPI == kEpiLinear && p.residual;
@@ -370,41 +404,44 @@ __device__ __forceinline__ bool write32(const Product& p, const Tiles& tl, const
 #pragma unroll
             for (int q = 0; q < 32; ++q) v[q] *= r.alpha;
         }
-        if (r.zero) {
+        if (p.targets && __any_sync(~0u, r.zero)) {
 #pragma unroll
-            for (int q = 0; q < 32; ++q) v[q] = 0.f;
+            for (int q = 0; q < 32; ++q) v[q] = r.zero ? 0.f : v[q];
         }
         if (p.preact) {
-            if (tl.tma_out && !free_now) boxes_free(tl, lane);
-            box_write<TO>(z, lane, v);
+            if (tl.tma_out && !free_now && !second) boxes_free(tl, lane);
+            box_write<TO>(z, lane, first, v);
         }
         activate32(v, p.act);
         if (p.residual) {
             if (tl.tma_out) {
-                if (!mbar_wait(o.bar + 8 * b, o.phase >> b & 1, gave_up)) return false;
-                o.phase ^= 1u << b;
+                if (!second) {
+                    if (!mbar_wait(o.bar + 8 * b, o.phase >> b & 1, gave_up)) return false;
+                    o.phase ^= 1u << b;
+                }
             } else {
-                box_copy<TO, true>(y, const_cast<TO*>(static_cast<const TO*>(p.residual)), p.ldr, i0, j0, p.M, p.N, lane);
+                box_copy<TO, true>(y, first, const_cast<TO*>(static_cast<const TO*>(p.residual)), p.ldr, i0, j0, p.M, p.N, lane);
                 __syncwarp();
             }
-            box_add<TO>(y, lane, v);
+            box_add<TO>(y, lane, first, v);
         }
     }
-    if (tl.tma_out && !free_now && !(EPI == kEpiLinear && p.preact)) boxes_free(tl, lane);
-    box_write<TO>(y, lane, v);
+    if (tl.tma_out && !free_now && !second && !(EPI == kEpiLinear && p.preact)) boxes_free(tl, lane);
+    box_write<TO>(y, lane, first, v);
     if (tl.tma_out) {
+        if (!send) return true;
         fence_async();
         __syncwarp();
         if (lane == 0) {
-            if (EPI == kEpiLinear && p.preact) tma_store(&maps.z, smem_u32(z), (int)j0, (int)i0, 0, false);
-            tma_store(&maps.y, smem_u32(y), (int)j0, (int)i0, split, EPI == kEpiSlab && p.accumulate);
+            if (EPI == kEpiLinear && p.preact) tma_store(&maps.z, smem_u32(z), (int)(second ? j0 - 32 : j0), (int)i0, 0, false);
+            tma_store(&maps.y, smem_u32(y), (int)(second ? j0 - 32 : j0), (int)i0, split, EPI == kEpiSlab && p.accumulate);
             bulk_commit();
             if (free_now) bulk_wait_read(tl.ring - 1);
         }
     } else {
         __syncwarp();
-        if (p.preact) box_copy<TO, false>(z, static_cast<TO*>(p.preact), p.ldz, i0, j0, p.M, p.N, lane);
-        box_copy<TO, false>(y, static_cast<TO*>(p.out), p.ldo, i0, j0, p.M, p.N, lane);
+        if (p.preact) box_copy<TO, false>(z, first, static_cast<TO*>(p.preact), p.ldz, i0, j0, p.M, p.N, lane);
+        box_copy<TO, false>(y, first, static_cast<TO*>(p.out), p.ldo, i0, j0, p.M, p.N, lane);
     }
     ++o.k;
     fetch_residual(p, tl, maps, o, i0, j_next, lane);
@@ -416,7 +453,8 @@ __device__ __forceinline__ bool write32(const Product& p, const Tiles& tl, const
 // gave up.
 template <typename T, int EPI>
 __device__ __forceinline__ bool columns32(const Product& p, const Tiles& tl, const OutMaps& maps, WarpOut& o,
-                                          RowState& r, float (&v)[32], int64_t i0, int64_t j0, int64_t j_next,
+                                          RowState& r, float (&v)[32], int64_t i0, int64_t j_begin, int64_t j0,
+                                          int64_t j_next,
                                           int split, int lane, volatile int* gave_up) {
     if (EPI == kEpiStats) {
         const float to2 = p.logit_scale * kLog2e;
@@ -467,8 +505,8 @@ __device__ __forceinline__ bool columns32(const Product& p, const Tiles& tl, con
         }
     }
     if (EPI == kEpiSlab || (EPI == kEpiLinear && sizeof(T) == 2 && p.out_dtype == MSPLAT_DTYPE_F32))
-        return write32<T, float, EPI>(p, tl, maps, o, r, v, i0, j0, j_next, split, lane, gave_up);
-    return write32<T, T, EPI>(p, tl, maps, o, r, v, i0, j0, j_next, split, lane, gave_up);
+        return write32<T, float, EPI>(p, tl, maps, o, r, v, i0, j_begin, j0, j_next, split, lane, gave_up);
+    return write32<T, T, EPI>(p, tl, maps, o, r, v, i0, j_begin, j0, j_next, split, lane, gave_up);
 }
 
 template <int EPI>
@@ -511,7 +549,6 @@ bool tma_ready(const void* p, int64_t ld, int64_t rows, int elem);
 inline void set_outputs(const Product& p, Tiles& tl, OutMaps& maps) {
     if (p.epi == kEpiStats) return;
     const int dtype = p.epi == kEpiSlab ? MSPLAT_DTYPE_F32 : p.out_dtype, es = dtype_size(dtype);
-    tl.box_bytes = 32 * 32 * es;
     tl.tma_out = 1;
     if (p.epi == kEpiSlab) {
         maps.y = map_output(p.slab, p.M, p.N, slab_ld(p.N), p.splits, dtype);
@@ -530,13 +567,16 @@ inline void set_outputs(const Product& p, Tiles& tl, OutMaps& maps) {
 inline int share_memory(const Product& p, Tiles& tl, int warps, int fixed, int least_stages, int most_stages) {
     const int outputs = p.epi == kEpiStats ? 0 : 1 + (p.epi == kEpiLinear && p.preact);
     for (tl.ring = 2;; --tl.ring) {
-        tl.warp_bytes = tl.ring * outputs * tl.box_bytes;
+        tl.warp_bytes = tl.ring * outputs * kBoxBytes;
         const int rest = kBlockBytes - fixed - warps * tl.warp_bytes;
         tl.stages = rest > 0 ? std::min(most_stages, rest / tl.stage_bytes) : 0;
         if ((rest > 0 && tl.stages >= least_stages) || tl.ring == 1) break;
     }
     return 1024 + fixed + tl.stages * tl.stage_bytes + warps * tl.warp_bytes;
 }
+
+// Column blocks of the label statistics: tiles of 64 columns, halves of wider ones.
+inline int64_t stats_blocks_of(const Product& p, int bn) { return ceil_div(p.N, bn) * (bn == 64 ? 1 : 2); }
 
 inline void set_tiles(const Product& p, Tiles& tl) {
     const int64_t tm = ceil_div(p.M, kBM), tn = ceil_div(p.N, tl.bn);

@@ -56,7 +56,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         for (int q = 0; q < 2; ++q) {
             mbar_init(smem_u32(&sm.acc_full[q]), 1);
-            mbar_init(smem_u32(&sm.acc_empty[q]), kEpiWarps);
+            mbar_init(smem_u32(&sm.acc_empty[q]), tl.bn == 64 ? kEpiWarps / 2 : kEpiWarps);
         }
         mbar_init(smem_u32(&sm.drain), 1);
         for (int q = 0; q < 2 * kEpiWarps; ++q) mbar_init(smem_u32(&sm.residual[q / 2][q % 2]), 1);
@@ -181,10 +181,14 @@ __global__ void __launch_bounds__(kThreads, 1)
             __syncwarp();
         }
     } else if (warp >= 4) {
-        const int quarter = warp % 4, half = (warp - 4) / 4;
+        // tiles of 64 columns: the two groups of warps take every other tile;
+        // wider ones: each takes half of the columns
+        const int quarter = warp % 4, group = (warp - 4) / 4;
+        const bool by_tile = tl.bn == 64;
+        const int half = by_tile ? 0 : group, columns = by_tile ? 64 : tl.bn / 2;
         WarpOut o;
         o.y = boxes + (warp - 4) * tl.warp_bytes;
-        o.z = o.y + tl.ring * tl.box_bytes;
+        o.z = o.y + tl.ring * kBoxBytes;
         o.bias = sm.bias[warp - 4];
         o.bar = smem_u32(sm.residual[warp - 4]);
         o.phase = 0;
@@ -193,17 +197,22 @@ __global__ void __launch_bounds__(kThreads, 1)
         uint32_t acc_phase = 0;
         bool ok = true;
         for (int w = blockIdx.x; w < tl.total && ok; w += gridDim.x) {
+            if (by_tile && acc != group) {
+                acc ^= 1;
+                if (acc == 0) acc_phase ^= 1;
+                continue;
+            }
             int tm, tn, split;
             int64_t r0, r1;
             tile_of(p, tl, w, tm, tn, split, r0, r1);
-            const int64_t i0 = (int64_t)tm * kBM + quarter * 32, j0 = (int64_t)tn * tl.bn + half * (tl.bn / 2);
-            const int64_t j_end = min(p.N, j0 + tl.bn / 2);
+            const int64_t i0 = (int64_t)tm * kBM + quarter * 32, j0 = (int64_t)tn * tl.bn + half * columns;
+            const int64_t j_end = min(p.N, j0 + columns);
             RowState row = row_begin<EPI>(p, i0, lane);
             if (EPI == kEpiLinear && j0 < j_end) fetch_residual(p, tl, maps, o, i0, j0, lane);
             if (!(ok = mbar_wait(smem_u32(&sm.acc_full[acc]), acc_phase, gave_up))) break;
             tc_fence_after();
             if (i0 < p.M) {
-                const uint32_t d = tmem + ((uint32_t)quarter << 21) + acc * tl.bn + half * (tl.bn / 2);
+                const uint32_t d = tmem + ((uint32_t)quarter << 21) + acc * tl.bn + half * columns;
                 for (int64_t j = j0; j < j_end && ok; j += 32) {
                     uint32_t raw[32];
                     tmem_load32(d + (uint32_t)(j - j0), raw);
@@ -211,10 +220,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                     float v[32];
 #pragma unroll
                     for (int q = 0; q < 32; ++q) v[q] = __uint_as_float(raw[q]);
-                    ok = columns32<T, EPI>(p, tl, maps, o, row, v, i0, j, j + 32 < j_end ? j + 32 : p.N, split, lane,
+                    ok = columns32<T, EPI>(p, tl, maps, o, row, v, i0, j0, j, j + 32 < j_end ? j + 32 : p.N, split, lane,
                                            gave_up);
                 }
-                row_end<EPI>(p, row, 2 * tn + half);
+                row_end<EPI>(p, row, by_tile ? tn : 2 * tn + half);
             }
             tc_fence_before();
             __syncwarp();
@@ -296,13 +305,13 @@ CUtensorMap map_output(const void* base, int64_t rows, int64_t cols, int64_t ld,
     const cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)layers};
     const cuuint64_t row = (cuuint64_t)(rows > 1 || layers > 1 ? ld * es : round_up(cols * es, 16));
     const cuuint64_t strides[2] = {row, row * (cuuint64_t)rows};
-    const cuuint32_t box[3] = {32, 32, 1}, step[3] = {1, 1, 1};
+    const cuuint32_t box[3] = {(cuuint32_t)(128 / es), 32, 1}, step[3] = {1, 1, 1};
     const CUresult r = encoder()(
         &m, dtype == MSPLAT_DTYPE_F32    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
             : dtype == MSPLAT_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
                                          : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
         3, const_cast<void*>(base), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
-        es == 4 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) throw Error(MSPLAT_ERR_CUDA, "cuTensorMapEncodeTiled failed");
     return m;
@@ -321,8 +330,7 @@ bool can_product_tc16(const Product& p) {
            tma_ready(p.B, p.ldb, p.b_mn ? p.R : p.N, 2);
 }
 
-// the halves of the tiles
-int64_t stats_blocks_tc16(const Product& p) { return 2 * ceil_div(p.N, tile_columns(p, 256)); }
+int64_t stats_blocks_tc16(const Product& p) { return stats_blocks_of(p, tile_columns(p, 256)); }
 
 void launch_product_tc16(const Product& p, cudaStream_t s) {
     Tiles tl{};

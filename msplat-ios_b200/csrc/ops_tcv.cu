@@ -162,7 +162,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         for (int q = 0; q < 2; ++q) {
             mbar_init(smem_u32(&sm.acc_full[q]), 1);
-            mbar_init(smem_u32(&sm.acc_empty[q]), kEpiWarps);
+            mbar_init(smem_u32(&sm.acc_empty[q]), BN == 64 ? kEpiWarps / 2 : kEpiWarps);
         }
         mbar_init(smem_u32(&sm.drain), 1);
         for (int q = 0; q < 2 * kEpiWarps; ++q) mbar_init(smem_u32(&sm.residual[q / 2][q % 2]), 1);
@@ -275,11 +275,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kEpiRegs));
-        const int quarter = warp % 4, half = (warp - 4) / 4;
-        constexpr int kHalf = BN / 2;
+        // tiles of 64 columns: the two groups of warps take every other tile;
+        // wider ones: each takes half of the columns
+        constexpr bool kByTile = BN == 64;
+        constexpr int kHalf = kByTile ? BN : BN / 2;
+        const int quarter = warp % 4, group = (warp - 4) / 4, half = kByTile ? 0 : group;
         WarpOut o;
         o.y = boxes + (warp - 4) * tl.warp_bytes;
-        o.z = o.y + tl.ring * tl.box_bytes;
+        o.z = o.y + tl.ring * kBoxBytes;
         o.bias = sm.bias[warp - 4];
         o.bar = smem_u32(sm.residual[warp - 4]);
         o.phase = 0;
@@ -288,12 +291,17 @@ __global__ void __launch_bounds__(kThreads, 1)
         uint32_t acc_phase = 0;
         bool ok = true;
         for (int w = blockIdx.x; w < tl.total && ok; w += gridDim.x) {
+            if (kByTile && acc != group) {
+                acc ^= 1;
+                if (acc == 0) acc_phase ^= 1;
+                continue;
+            }
             int tm, tn, split;
             int64_t r0, r1;
             tile_of(p, tl, w, tm, tn, split, r0, r1);
             const int64_t i0 = (int64_t)tm * kBM + quarter * 32, j0 = (int64_t)tn * BN + half * kHalf;
             const int64_t j_end = min(p.N, j0 + kHalf);
-            const int groups = (int)min((int64_t)kGroups, (r1 - r0 + kGroup * kBR - 1) / (kGroup * kBR));
+            const int parts = (int)min((int64_t)kGroups, (r1 - r0 + kGroup * kBR - 1) / (kGroup * kBR));
             RowState row = row_begin<EPI>(p, i0, lane);
             if (EPI == kEpiLinear && j0 < j_end) fetch_residual(p, tl, maps, o, i0, j0, lane);
             if (!(ok = mbar_wait(smem_u32(&sm.acc_full[acc]), acc_phase, gave_up))) break;
@@ -313,16 +321,16 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                         for (int q = 0; q < 32; ++q) v[q] = 0.f;
                     }
-                    for (int g = 0; g < groups; ++g) {
+                    for (int g = 0; g < parts; ++g) {
                         tmem_load32(d + g * BN + c, raw);
                         tmem_wait();
 #pragma unroll
                         for (int q = 0; q < 32; ++q) v[q] += __uint_as_float(raw[q]);
                     }
-                    ok = columns32<T, EPI>(p, tl, maps, o, row, v, i0, j, j + 32 < j_end ? j + 32 : p.N, split, lane,
+                    ok = columns32<T, EPI>(p, tl, maps, o, row, v, i0, j0, j, j + 32 < j_end ? j + 32 : p.N, split, lane,
                                            gave_up);
                 }
-                row_end<EPI>(p, row, 2 * tn + half);
+                row_end<EPI>(p, row, kByTile ? tn : 2 * tn + half);
             }
             tc_fence_before();
             __syncwarp();
@@ -409,8 +417,7 @@ int columns_tcv(const Product& p) {
 
 bool gave_up_tcv(cudaStream_t s) { return take_gave_up(s); }
 
-// the halves of the tiles
-int64_t stats_blocks_tcv(const Product& p) { return 2 * ceil_div(p.N, columns_tcv(p)); }
+int64_t stats_blocks_tcv(const Product& p) { return stats_blocks_of(p, columns_tcv(p)); }
 
 void launch_product_tcv(const Product& p, cudaStream_t s) {
     Tiles tl{};
