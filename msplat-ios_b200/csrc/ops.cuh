@@ -151,13 +151,9 @@ struct Product {
     int splits;
     int64_t split_len;
     int accumulate;
-    // labels: rows (kEpiStats, kEpiGrad, kEpiLinear for dx) without one count
-    // for nothing; with label_reduces the labels belong to r and unlabelled r
-    // are read as zeros of B
+    // labels (kEpiStats, kEpiGrad; kEpiLinear: rows without one become zeros)
     const int32_t* targets;
     int64_t labels;     // number of labels
-    const uint32_t* unlabelled;  // label_reduces: bit r % 32 of word r / 32 is set when r has no label
-    int label_reduces;
     int64_t col0;       // label of column 0 of this piece
     float logit_scale;
     float g_scale;
@@ -202,10 +198,14 @@ struct JoinArgs {
     int64_t labels;
     float* lse;
     float* row_loss;
-    uint32_t* unlabelled; // [ceil(m / 32)] bits
     double* partial;      // [join_blocks(m)][2]
 };
 int join_blocks(int64_t m);
+// The rows of x with a label, zeros in place of the others: what the products
+// read, so that an unlabelled row's NaN or infinity reaches nothing (in dw even
+// a zero gradient times it would).
+void launch_labelled_rows(int64_t m, int64_t d, const void* x, int64_t ldx, const int32_t* targets, int64_t labels,
+                          void* out, int64_t ldo, int dtype, cudaStream_t s);
 void launch_join(const JoinArgs& a, cudaStream_t s);
 // loss = weight * mean, *alpha = factor / number of labelled rows (both 0
 // without any), from all the partial sums.

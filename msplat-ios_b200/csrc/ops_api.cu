@@ -140,8 +140,8 @@ struct LossPlan {
     float *lse, *label_logit, *alpha;
     double* partial;
     float2* stats;
-    uint32_t* unlabelled;
-    char* g = nullptr;
+    char *x = nullptr, *g = nullptr;  // x's labelled rows; a piece of the softmax gradient
+    int64_t ldx;
     float *slab_x = nullptr, *slab_w = nullptr;
     LossPlan(Arena& a, int64_t m, int64_t v, int64_t d, bool grad, int dtype) {
         blocks = stats_blocks_most(v);
@@ -150,11 +150,12 @@ struct LossPlan {
         alpha = a.take<float>(1);
         lse = a.take<float>(m);
         label_logit = a.take<float>(m);
-        unlabelled = a.take<uint32_t>(ceil_div(m, 64) * 2);
         partial = a.take<double>(2 * ceil_div(m, stats_rows) * join_blocks(stats_rows));
         stats = a.take<float2>(blocks * stats_rows);
         if (!grad) return;
         const int es = dtype_size(dtype);
+        ldx = round_up(d, 16 / es);
+        x = a.take<char>(m * ldx * es);
         by_rows = m >= v;
         const int64_t other = round_up(by_rows ? v : m, 16 / es), all = by_rows ? m : v;
         chunk = std::min(all, round_up(std::max<int64_t>(kPieceBytes / (other * es), 1), 128));
@@ -198,7 +199,7 @@ void launch_gradient(Product q, const LossPlan& plan, float* slab, Split split, 
     launch_product(q, s);
     if (!sums || last)
         launch_slab_sum(q.M, q.N, slab, slab_ld(q.N), sums ? split.splits : q.splits, out, ldo, 1.f, plan.alpha,
-                        q.label_reduces ? nullptr : q.targets, labels, dtype, s);
+                        q.targets, labels, dtype, s);
 }
 
 const char* at(const void* p, int64_t elements, int es) { return static_cast<const char*>(p) + elements * es; }
@@ -399,6 +400,11 @@ int msplat_loss_cross_entropy(int64_t m, int64_t v, int64_t d, const void* x, in
         logits.logit_scale = logit_scale;
         logits.g_scale = dtype == MSPLAT_DTYPE_F16 ? 16384.f : 1.f;
 
+        if (grad) {
+            launch_labelled_rows(m, d, x, ldx, targets, v, plan.x, plan.ldx, dtype, s);
+            logits.A = x = plan.x;
+            logits.lda = ldx = plan.ldx;
+        }
         int joined = 0;
         for (int64_t r0 = 0; r0 < m; r0 += plan.stats_rows) {
             const int64_t rows = std::min(plan.stats_rows, m - r0);
@@ -417,7 +423,6 @@ int msplat_loss_cross_entropy(int64_t m, int64_t v, int64_t d, const void* x, in
             j.targets = targets + r0; j.labels = v;
             j.lse = plan.lse + r0;
             j.row_loss = row_loss ? row_loss + r0 : nullptr;
-            j.unlabelled = plan.unlabelled + r0 / 32;
             j.partial = plan.partial + 2 * joined;
             launch_join(j, s);
             joined += join_blocks(rows);
@@ -455,9 +460,6 @@ int msplat_loss_cross_entropy(int64_t m, int64_t v, int64_t d, const void* x, in
                 q.M = cols; q.N = d; q.R = rows;
                 q.A = plan.g; q.lda = plan.ldg; q.a_mn = true;
                 q.B = p.A; q.ldb = ldx; q.b_mn = true;
-                q.targets = p.targets;
-                q.label_reduces = 1;
-                q.unlabelled = plan.unlabelled + r0 / 32;
                 launch_gradient(q, plan, plan.slab_w, plan.sw, plan.by_rows, first, last, at(dw, l0 * lddw, es),
                                 lddw, v, dtype, s);
             }

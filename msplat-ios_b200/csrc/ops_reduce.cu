@@ -162,13 +162,11 @@ __global__ void __launch_bounds__(1024) k_join(JoinArgs a, int shares) {
             }
             const int32_t t = i < a.m ? a.targets[i] : -1;
             const bool has = t >= 0 && t < a.labels;
-            const uint32_t off = __ballot_sync(~0u, !has);
             if (i < a.m) {
                 const float lse = top + log2f(total);
                 const float row = has ? (lse - a.label_logit[i]) * kLn2 : 0.f;
                 a.lse[i] = lse;
                 if (a.row_loss) a.row_loss[i] = row;
-                if (lane == 0) a.unlabelled[i0 / 32] = off;
                 if (has) {
                     sum += row;
                     count += 1;
@@ -219,6 +217,42 @@ __global__ void __launch_bounds__(256) k_loss_total(const double* partial, int b
         if (loss) *loss = any ? (float)(weight * ssum[0] / scount[0]) : 0.f;
         *alpha = any ? (float)(factor / scount[0]) : 0.f;
     }
+}
+
+// One thread per vector of V elements.
+template <typename T, int V>
+__global__ void __launch_bounds__(256) k_labelled_rows(int64_t m, int64_t d, const T* x, int64_t ldx,
+                                                       const int32_t* targets, int64_t labels, T* out, int64_t ldo) {
+    const int64_t per = (d + V - 1) / V;
+    for (int64_t e = blockIdx.x * 256ll + threadIdx.x; e < m * per; e += gridDim.x * 256ll) {
+        const int64_t i = e / per, j = (e - i * per) * V;
+        const int32_t t = __ldg(targets + i);
+        const bool has = t >= 0 && t < labels;
+        const T* from = x + i * ldx + j;
+        T* to = out + i * ldo + j;
+        if (V > 1) {
+            *reinterpret_cast<uint4*>(to) = has ? __ldg(reinterpret_cast<const uint4*>(from)) : make_uint4(0, 0, 0, 0);
+        } else {
+            *to = has ? *from : from_f32<T>(0.f);
+        }
+    }
+}
+
+template <typename T>
+void labelled_typed(int64_t m, int64_t d, const void* x, int64_t ldx, const int32_t* targets, int64_t labels, void* out,
+                    int64_t ldo, cudaStream_t s) {
+    constexpr int V = 16 / sizeof(T);
+    const bool vec = reinterpret_cast<uintptr_t>(x) % 16 == 0 && (m <= 1 || ldx % V == 0) && d % V == 0;
+    const int64_t ctas = ceil_div(m * ceil_div(d, vec ? V : 1), 256);
+    const unsigned grid = (unsigned)std::min<int64_t>(ctas, kSMs * 16);
+    note_launches(1);
+    if (vec)
+        k_labelled_rows<T, V><<<grid, 256, 0, s>>>(m, d, static_cast<const T*>(x), ldx, targets, labels,
+                                                   static_cast<T*>(out), ldo);
+    else
+        k_labelled_rows<T, 1><<<grid, 256, 0, s>>>(m, d, static_cast<const T*>(x), ldx, targets, labels,
+                                                   static_cast<T*>(out), ldo);
+    OPS_CK(cudaGetLastError());
 }
 
 template <typename T, int V>
@@ -293,6 +327,16 @@ void launch_slab_sum(int64_t rows, int64_t cols, const float* slab, int64_t ld, 
     else
         go(static_cast<__nv_bfloat16*>(out));
     OPS_CK(cudaGetLastError());
+}
+
+void launch_labelled_rows(int64_t m, int64_t d, const void* x, int64_t ldx, const int32_t* targets, int64_t labels,
+                          void* out, int64_t ldo, int dtype, cudaStream_t s) {
+    if (dtype == MSPLAT_DTYPE_F32)
+        labelled_typed<float>(m, d, x, ldx, targets, labels, out, ldo, s);
+    else if (dtype == MSPLAT_DTYPE_F16)
+        labelled_typed<__half>(m, d, x, ldx, targets, labels, out, ldo, s);
+    else
+        labelled_typed<__nv_bfloat16>(m, d, x, ldx, targets, labels, out, ldo, s);
 }
 
 int join_blocks(int64_t m) {

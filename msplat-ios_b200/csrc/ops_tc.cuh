@@ -350,7 +350,7 @@ __device__ __forceinline__ RowState row_begin(const Product& p, int64_t i0, int 
     }
     if (EPI == kEpiLinear) {
         if (p.alpha_dev) r.alpha *= __ldg(p.alpha_dev);
-        if (p.targets && !p.label_reduces) r.zero = r.in && !labelled(p, r.i);
+        if (p.targets) r.zero = r.in && !labelled(p, r.i);
     }
     return r;
 }

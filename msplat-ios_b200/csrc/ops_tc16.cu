@@ -31,12 +31,6 @@ struct Smem {
 };
 static_assert(offsetof(Smem, bias) % 16 == 0 && sizeof(Smem) <= 2048, "read as float4; share_memory counts 2048");
 
-// Bits of the rows r .. r + 63 (r a multiple of 64) without a label.
-__device__ __forceinline__ uint64_t unlabelled64(const Product& p, int64_t r) {
-    const uint32_t* w = p.unlabelled + r / 32;
-    return (uint64_t)__ldg(w) | (r + 32 < p.R ? (uint64_t)__ldg(w + 1) << 32 : 0);
-}
-
 template <typename T, int EPI>
 __global__ void __launch_bounds__(kThreads, 1)
     k_product_tc16(const __grid_constant__ Product p, const __grid_constant__ Tiles tl,
@@ -128,31 +122,11 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (!(ok = mbar_wait(smem_u32(&sm.acc_empty[acc]), acc_phase ^ 1, gave_up))) break;
             tc_fence_after();
             const uint32_t d = tmem + acc * tl.bn;
-            uint64_t off_next = p.label_reduces ? unlabelled64(p, r0) : 0;
             for (int64_t r = r0; r < r1; r += kBR) {
-                // unlabelled rows of x must not reach dw, even as 0 x NaN: their rows of
-                // the stage are cleared before the products read it
-                uint64_t off = 0;
-                if (p.label_reduces) {
-                    off = off_next;
-                    if (r + kBR < r1) off_next = unlabelled64(p, r + kBR);
-                }
                 if (!(ok = mbar_wait(smem_u32(&sm.full[stage]), phase, gave_up))) break;
-                uint8_t* sa = tiles + (size_t)stage * tl.stage_bytes;
-                if (off) {
-                    uint8_t* sb = sa + kBM * 128;
-                    // eight lanes clear a row's 128 bytes, four column groups at a time
-                    for (; off; off &= off - 1) {
-                        const int q = __ffsll(off) - 1;
-                        for (int g = lane / 8; g < tl.bn / 64; g += 4)
-                            *reinterpret_cast<uint4*>(sb + g * 8192 + q * 128 + lane % 8 * 16) = make_uint4(0, 0, 0, 0);
-                    }
-                    fence_async();
-                    __syncwarp();
-                }
                 tc_fence_after();
                 if (elect_one()) {
-                    const uint32_t a = smem_u32(sa), b = a + kBM * 128;
+                    const uint32_t a = smem_u32(tiles + (size_t)stage * tl.stage_bytes), b = a + kBM * 128;
                     const uint64_t da = smem_desc(a, p.a_mn ? 8192 : 16), db = smem_desc(b, p.b_mn ? 8192 : 16);
                     const uint32_t step_a = p.a_mn ? 2048 >> 4 : 32 >> 4, step_b = p.b_mn ? 2048 >> 4 : 32 >> 4;
 #pragma unroll

@@ -49,52 +49,85 @@ static_assert(offsetof(Smem, bias) % 16 == 0 && sizeof(Smem) <= 2048, "read as f
 template <typename T>
 constexpr int planes() { return sizeof(T) == 4 ? 3 : 1; }
 
-// Eight consecutive elements on their way to shared memory.
-template <typename T>
-struct Chunk;
-template <>
-struct Chunk<float> {
-    float v[8];
-    __device__ __forceinline__ void zero() {
-#pragma unroll
-        for (int q = 0; q < 8; ++q) v[q] = 0.f;
-    }
-    __device__ __forceinline__ void load(const float* g) {
-        const float4 a = __ldg(reinterpret_cast<const float4*>(g)), b = __ldg(reinterpret_cast<const float4*>(g) + 1);
-        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-    }
-    __device__ __forceinline__ void set(int q, float x) { v[q] = x; }
-    // the three parts, `plane` bytes apart
-    __device__ __forceinline__ void store(uint8_t* s, uint32_t plane) const {
-        uint32_t w[3][4];
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            float a = v[2 * q], b = v[2 * q + 1];
-#pragma unroll
-            for (int k = 0; k < 3; ++k) {
-                const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-                w[k][q] = *reinterpret_cast<const uint32_t*>(&h);
-                if (k < 2) {
-                    a -= __uint_as_float(w[k][q] << 16);
-                    b -= __uint_as_float(w[k][q] & 0xFFFF0000u);
-                }
-            }
-        }
-#pragma unroll
-        for (int k = 0; k < 3; ++k)
-            *reinterpret_cast<uint4*>(s + k * plane) = make_uint4(w[k][0], w[k][1], w[k][2], w[k][3]);
-    }
-};
+// Eight consecutive elements on their way to shared memory, as 32-bit words.
 template <typename T>
 struct Chunk {
-    uint4 w;
-    __device__ __forceinline__ void zero() { w = make_uint4(0, 0, 0, 0); }
-    __device__ __forceinline__ void load(const T* g) { w = __ldg(reinterpret_cast<const uint4*>(g)); }
-    __device__ __forceinline__ void set(int q, T x) {
-        const uint32_t bits = (uint32_t)*reinterpret_cast<const uint16_t*>(&x) << 16 * (q & 1);
-        (q < 2 ? w.x : q < 4 ? w.y : q < 6 ? w.z : w.w) |= bits;
+    static constexpr int kWords = 8 * sizeof(T) / 4;
+    uint32_t w[kWords];
+
+    __device__ __forceinline__ void zero() {
+#pragma unroll
+        for (int q = 0; q < kWords; ++q) w[q] = 0;
     }
-    __device__ __forceinline__ void store(uint8_t* s, uint32_t) const { *reinterpret_cast<uint4*>(s) = w; }
+    // Element by element: the first n.
+    __device__ __forceinline__ void load_each(const T* g, int n) {
+        zero();
+#pragma unroll
+        for (int q = 0; q < 8; ++q)
+            if (q < n) {
+                if constexpr (sizeof(T) == 4)
+                    w[q] = __ldg(reinterpret_cast<const uint32_t*>(g) + q);
+                else
+                    w[q / 2] |= (uint32_t)__ldg(reinterpret_cast<const uint16_t*>(g) + q) << 16 * (q & 1);
+            }
+    }
+    // From a 16-byte boundary.
+    __device__ __forceinline__ void load_aligned(const T* g) {
+#pragma unroll
+        for (int q = 0; q < kWords / 4; ++q) {
+            const uint4 v = __ldg(reinterpret_cast<const uint4*>(g) + q);
+            w[4 * q] = v.x; w[4 * q + 1] = v.y; w[4 * q + 2] = v.z; w[4 * q + 3] = v.w;
+        }
+    }
+    // From any element: the 16-byte pieces around it, shifted into place.
+    __device__ __forceinline__ void load_around(const T* g) {
+        const uintptr_t a = reinterpret_cast<uintptr_t>(g);
+        const uint32_t off = (uint32_t)(a & 15);
+        const uint4* at = reinterpret_cast<const uint4*>(a & ~(uintptr_t)15);
+        uint32_t r[kWords + 4];
+#pragma unroll
+        for (int q = 0; q < kWords / 4 + 1; ++q) {
+            const uint4 v = q < kWords / 4 || off ? __ldg(at + q) : make_uint4(0, 0, 0, 0);
+            r[4 * q] = v.x; r[4 * q + 1] = v.y; r[4 * q + 2] = v.z; r[4 * q + 3] = v.w;
+        }
+#pragma unroll
+        for (int q = 0; q < kWords + 2; ++q) r[q] = off & 8 ? r[q + 2] : r[q];
+#pragma unroll
+        for (int q = 0; q < kWords + 1; ++q) r[q] = off & 4 ? r[q + 1] : r[q];
+#pragma unroll
+        for (int q = 0; q < kWords; ++q) w[q] = sizeof(T) == 4 ? r[q] : __funnelshift_r(r[q], r[q + 1], (off & 2) * 8);
+    }
+    // Zeros behind the first n elements.
+    __device__ __forceinline__ void keep(int n) {
+#pragma unroll
+        for (int q = 0; q < kWords; ++q) {
+            if constexpr (sizeof(T) == 4)
+                w[q] = q < n ? w[q] : 0;
+            else
+                w[q] = 2 * q + 1 < n ? w[q] : 2 * q < n ? w[q] & 0xFFFF : 0;
+        }
+    }
+    // The parts, `plane` bytes apart.
+    __device__ __forceinline__ void store(uint8_t* s, uint32_t plane) const {
+        if constexpr (sizeof(T) == 4) {
+            uint32_t o[3][4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                float a = __uint_as_float(w[2 * q]), b = __uint_as_float(w[2 * q + 1]);
+#pragma unroll
+                for (int k = 0; k < 3; ++k) {
+                    o[k][q] = pack2<__nv_bfloat16>(a, b);
+                    a -= __uint_as_float(o[k][q] << 16);
+                    b -= __uint_as_float(o[k][q] & 0xFFFF0000u);
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < 3; ++k)
+                *reinterpret_cast<uint4*>(s + k * plane) = make_uint4(o[k][0], o[k][1], o[k][2], o[k][3]);
+        } else {
+            *reinterpret_cast<uint4*>(s) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+    }
 };
 
 // One operand as rows of consecutive elements: [i][r], or [r][i] when mn.
@@ -103,8 +136,14 @@ struct Operand {
     const T* p;
     int64_t ld, rows, cols;
     bool mn, vec;
-    const Product* masked;  // rows without a label read as zeros
+    const T* end;  // behind the last element
 };
+template <typename T>
+__device__ __forceinline__ Operand<T> operand(const void* p, int64_t ld, int64_t I, int64_t R, bool mn, bool vec) {
+    Operand<T> o{static_cast<const T*>(p), ld, mn ? R : I, mn ? I : R, mn, vec, nullptr};
+    o.end = o.p + (o.rows - 1) * ld + o.cols;
+    return o;
+}
 
 // The stage's tile of an operand: WIDE / 32 chunks of eight per thread, thread
 // t taking chunk t % 8 of row t / 8 + 32 q (eight lanes read one row's 64
@@ -117,15 +156,22 @@ __device__ __forceinline__ void load_tile(const Operand<T>& o, int64_t i0, int64
         // mn: 64 rows of r per group of 64 i
         const int64_t row = o.mn ? r0 + line % 64 : i0 + line;
         const int64_t col = (o.mn ? i0 + line / 64 * 64 : r0) + t % 8 * 8;
-        c[q].zero();
-        if (row >= o.rows || col >= o.cols || (o.masked && !labelled(*o.masked, row))) continue;
+        if (row >= o.rows || col >= o.cols) {
+            c[q].zero();
+            continue;
+        }
         const T* g = o.p + row * o.ld + col;
-        if (o.vec && col + 8 <= o.cols) {
-            c[q].load(g);
+        const int n = (int)min((int64_t)8, o.cols - col);
+        // whole 16-byte pieces are read where the matrix has all of them
+        const uintptr_t from = reinterpret_cast<uintptr_t>(g) & ~(uintptr_t)15;
+        if (o.vec && n == 8) {
+            c[q].load_aligned(g);
+        } else if (from >= reinterpret_cast<uintptr_t>(o.p) &&
+                   from + 8 * sizeof(T) + 16 <= reinterpret_cast<uintptr_t>(o.end)) {
+            c[q].load_around(g);
+            if (n < 8) c[q].keep(n);
         } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-                if (col + e < o.cols) c[q].set(e, __ldg(g + e));
+            c[q].load_each(g, n);
         }
     }
 }
@@ -179,10 +225,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (warp >= kLoadWarp) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kLoadRegs));
         const int t = threadIdx.x - kLoadWarp * 32;
-        const Operand<T> oa{static_cast<const T*>(p.A), p.lda, p.a_mn ? p.R : p.M, p.a_mn ? p.M : p.R, p.a_mn, vec_a,
-                            nullptr};
-        const Operand<T> ob{static_cast<const T*>(p.B), p.ldb, p.b_mn ? p.R : p.N, p.b_mn ? p.N : p.R, p.b_mn, vec_b,
-                            p.label_reduces ? &p : nullptr};
+        const Operand<T> oa = operand<T>(p.A, p.lda, p.M, p.R, p.a_mn, vec_a);
+        const Operand<T> ob = operand<T>(p.B, p.ldb, p.N, p.R, p.b_mn, vec_b);
         for (int q = 0; q < tl.resident; ++q) {
             Chunk<T> b[BN / 32];
             load_tile<T, BN>(ob, (int64_t)(blockIdx.x % tl.tiles_n) * BN, (int64_t)q * kBR, t, b);
