@@ -2,6 +2,7 @@
 // the description of one matrix product with its epilogue, and the launchers.
 #pragma once
 #include <algorithm>
+#include <atomic>
 #include <cstdint>
 #include <stdexcept>
 #include <string>
@@ -114,6 +115,18 @@ __device__ __forceinline__ float act_slope(float z) {
     return 1.f;
 }
 
+// Lets a kernel use `bytes` of dynamic shared memory, once per kernel and device.
+template <auto KERNEL>
+void allow_shared(int bytes) {
+    static std::atomic<uint64_t> done{0};
+    int dev = 0;
+    OPS_CK(cudaGetDevice(&dev));
+    const uint64_t bit = 1ull << (dev & 63);
+    if (done.load(std::memory_order_acquire) & bit) return;
+    OPS_CK(cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    done.fetch_or(bit, std::memory_order_release);
+}
+
 // What a matrix product does with its result.
 enum EpiKind {
     kEpiLinear = 0,  // bias, activation, residual; element type T or float
@@ -176,6 +189,9 @@ int64_t stats_blocks_tc16(const Product& p);
 void launch_product_tc16(const Product& p, cudaStream_t s);
 bool gave_up_tc16(cudaStream_t s);
 void launch_product_tcv(const Product& p, cudaStream_t s);
+// layers with few outputs and many rows (ops_few.cu)
+bool can_product_few(const Product& p);
+void launch_product_few(const Product& p, cudaStream_t s);
 int64_t stats_blocks_tcv(const Product& p);
 bool gave_up_tcv(cudaStream_t s);
 

@@ -514,19 +514,6 @@ __device__ __forceinline__ void row_end(const Product& p, const RowState& r, int
     if (EPI == kEpiStats && r.in) p.stats[(p.stats_block0 + block) * p.stats_ld + r.i] = make_float2(r.top, r.sum);
 }
 
-// Lets a kernel use all of a block's shared memory, once per kernel (KEY) and
-// device.
-template <typename KEY, typename K>
-void allow_shared(K kernel) {
-    static std::atomic<uint64_t> done{0};
-    int dev = 0;
-    OPS_CK(cudaGetDevice(&dev));
-    const uint64_t bit = 1ull << (dev & 63);
-    if (done.load(std::memory_order_acquire) & bit) return;
-    OPS_CK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kBlockBytes + 1024));
-    done.fetch_or(bit, std::memory_order_release);
-}
-
 // Columns of a tile: the widest that still gives three SMs of four one, and for the
 // label statistics a function of the columns alone (stats_block).
 inline int tile_columns(const Product& p, int widest) {

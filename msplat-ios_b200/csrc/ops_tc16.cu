@@ -232,9 +232,6 @@ EncodeFn encoder() {
     return fn;
 }
 
-template <typename T, int EPI>
-struct Here;  // one kernel
-
 struct Maps {
     CUtensorMap a, b;
     OutMaps out;
@@ -242,7 +239,7 @@ struct Maps {
 
 template <typename T, int EPI>
 void run(const Product& p, const Tiles& tl, const Maps& m, int bytes, cudaStream_t s) {
-    allow_shared<Here<T, EPI>>(k_product_tc16<T, EPI>);
+    allow_shared<k_product_tc16<T, EPI>>(kBlockBytes + 1024);
     note_launches(1);
     k_product_tc16<T, EPI><<<std::min(tl.total, kSMs), kThreads, bytes, s>>>(p, tl, m.a, m.b, m.out);
     OPS_CK(cudaGetLastError());

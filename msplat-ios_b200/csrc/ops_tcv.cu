@@ -401,9 +401,6 @@ bool vectors(const void* q, int64_t ld, int64_t rows) {
 }
 
 template <typename T, int EPI, int BN>
-struct Here;  // one kernel
-
-template <typename T, int EPI, int BN>
 void run(const Product& p, Tiles tl, cudaStream_t s) {
     OutMaps maps{};
     set_outputs(p, tl, maps);
@@ -424,7 +421,7 @@ void run(const Product& p, Tiles tl, cudaStream_t s) {
         tl.stage_bytes = a_bytes + b_bytes;
         bytes = share_memory(p, tl, kEpiWarps, 0, 2, kMaxStages);
     }
-    allow_shared<Here<T, EPI, BN>>(k_product_tcv<T, EPI, BN>);
+    allow_shared<k_product_tcv<T, EPI, BN>>(kBlockBytes + 1024);
     note_launches(1);
     k_product_tcv<T, EPI, BN><<<grid, kThreads, bytes, s>>>(
         p, tl, maps, vectors<T>(p.A, p.lda, p.a_mn ? p.R : p.M), vectors<T>(p.B, p.ldb, p.b_mn ? p.R : p.N));

@@ -423,3 +423,37 @@ def test_refusals_on_the_device():
             f()
             pytest.fail(f"call {k} was not refused")
     R.check(o.linear_forward(x, w), *R.linear(x, w, None, "none", None, torch.float32)[:2], "y after refusals")
+
+
+# ---- few outputs, many rows ------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("m,n,k", [(4096, 1, 1), (5000, 3, 61), (4100, 4, 64), (4099, 7, 33), (4097, 16, 200), (4096, 9, 1030),
+                                   (4100, 3, 2600)])
+@pytest.mark.parametrize("pad,lead", [(0, 0), (3, 1), (8, 8)])
+def test_linear_few_outputs(m, n, k, pad, lead, t):
+    act = ACTS[(m + n + k) % 5]
+    x, w, b = normal(100, m, k, t, pad=pad, lead=lead), normal(101, n, k, t, std=k ** -0.5), normal(102, 1, n, t)[0]
+    res = normal(103, m, n, t)
+    z, z_untouched = guarded(m, n, R.TYPES[t])
+    out, untouched = guarded(m, n, R.TYPES[t])
+    ops().linear_forward(x, w, b, activation=act, residual=res, preact=z, out=out)
+    want, bound, wz, bz = R.linear(x, w, b, act, res, R.TYPES[t])
+    R.check(out, want, bound, "y")
+    R.check(z, wz, bz, "preact")
+    assert untouched() and z_untouched()
+
+
+@pytest.mark.parametrize("t", TYPES)
+def test_linear_neighbours_in_the_record(t):
+    """What lies beside the columns of a wider record, NaN here, does not reach the result at any alignment."""
+    for m, n in ((300, 40), (4200, 3)):
+        for lead in range(0, 9):
+            full = torch.full((m, 61 + 9), float("nan"), dtype=R.TYPES[t], device="cuda")
+            x = full[:, lead:lead + 61]
+            x.copy_(normal(104, m, 61, t))
+            w = normal(105, n, 61, t, std=0.1)
+            R.check(ops().linear_forward(x, w), *R.linear(x, w, None, "none", None, R.TYPES[t])[:2], f"lead {lead}")
+            dx, dw, _ = ops().linear_backward(x, w, normal(106, m, n, t))
+            R.check(dw, *R.linear_grads(x, w, normal(106, m, n, t), None, "none", R.TYPES[t])[1], f"dw, lead {lead}")
