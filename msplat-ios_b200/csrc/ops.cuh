@@ -29,8 +29,8 @@ struct Error : std::runtime_error {
             throw ::msplat::ops::Error(MSPLAT_ERR_CUDA, std::string(#call) + ": " + cudaGetErrorString(e_)); \
     } while (0)
 
-inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
-inline int64_t round_up(int64_t a, int64_t b) { return ceil_div(a, b) * b; }
+__host__ __device__ inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+__host__ __device__ inline int64_t round_up(int64_t a, int64_t b) { return ceil_div(a, b) * b; }
 inline int dtype_size(int dtype) { return dtype == MSPLAT_DTYPE_F32 ? 4 : 2; }
 constexpr int kSMs = 148;
 
@@ -135,7 +135,7 @@ enum EpiKind {
     kEpiGrad = 3,    // (softmax - one-hot), times g_scale, in T
 };
 
-inline int64_t slab_ld(int64_t n) { return round_up(n, 4); }
+__host__ __device__ inline int64_t slab_ld(int64_t n) { return round_up(n, 4); }
 
 // C[i, j] = sum_r A(i, r) B(j, r), i < M, j < N, r < R.
 // A(i, r) = a_mn ? A[r * lda + i] : A[i * lda + r], B(j, r) likewise.
@@ -194,6 +194,22 @@ bool can_product_few(const Product& p);
 void launch_product_few(const Product& p, cudaStream_t s);
 int64_t stats_blocks_tcv(const Product& p);
 bool gave_up_tcv(cudaStream_t s);
+
+// Many rows against a small matrix in one pass (ops_rows.cu): v x d w, at most
+// 128 x 64. slab: [rows_blocks(m)][v][slab_ld(d)] partial sums of dw, sums:
+// [rows_blocks(m)][v] of g; each may be null, and dx.
+bool fits_rows(int64_t m, int64_t v, int64_t d);
+int rows_blocks(int64_t m);
+bool gave_up_rows(cudaStream_t s);
+void launch_rows_labels(int64_t m, int64_t v, int64_t d, const void* x, int64_t ldx, const void* w, int64_t ldw,
+                        const int32_t* targets, float logit_scale, float g_scale, const float* alpha, float* row_loss,
+                        double* partial, void* dx, int64_t lddx, float* slab, int dtype, cudaStream_t s);
+void launch_rows_layer(int64_t m, int64_t n, int64_t k, const void* x, int64_t ldx, const void* w, int64_t ldw,
+                       const void* z, int64_t ldz, int act, const void* dy, int64_t lddy, void* dx, int64_t lddx,
+                       float* slab, float* sums, int dtype, cudaStream_t s);
+// partial[block] = (0, labelled rows of the block's share)
+void launch_count_labels(int64_t m, const int32_t* targets, int64_t labels, double* partial, int blocks,
+                         cudaStream_t s);
 
 // dz = dy act'(z) (dz may be null) and the column sums of dz in pieces of
 // rows: partial[piece][n]. Returns the number of pieces.

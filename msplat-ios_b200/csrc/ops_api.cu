@@ -109,7 +109,15 @@ struct BackwardPlan {
     float* slab = nullptr;
     float* sums = nullptr;
     int pieces = 0;
+    bool rows = false;  // in one pass over the rows
     BackwardPlan(Arena& a, int64_t m, int64_t n, int64_t k, int act, int dtype) {
+        rows = fits_rows(m, n, k);
+        if (rows) {
+            pieces = rows_blocks(m);
+            slab = a.take<float>((int64_t)pieces * n * slab_ld(k));
+            sums = a.take<float>((int64_t)pieces * n);
+            return;
+        }
         split = plan_split(n, k, m, dtype);
         pieces = dz_pieces(m, n);
         lddz = round_up(n, 16 / dtype_size(dtype));
@@ -143,7 +151,15 @@ struct LossPlan {
     char *x = nullptr, *g = nullptr;  // x's labelled rows; a piece of the softmax gradient
     int64_t ldx;
     float *slab_x = nullptr, *slab_w = nullptr;
+    bool rows;                         // in one pass over the rows
     LossPlan(Arena& a, int64_t m, int64_t v, int64_t d, bool grad, int dtype) {
+        rows = fits_rows(m, v, d);
+        if (rows) {
+            alpha = a.take<float>(1);
+            partial = a.take<double>(2 * rows_blocks(m));
+            slab_w = a.take<float>((int64_t)rows_blocks(m) * v * slab_ld(d));
+            return;
+        }
         blocks = stats_blocks_most(v);
         stats_rows = round_up(std::max<int64_t>(kStatsBytes / (8 * blocks), 1), 256);
         if (stats_rows > m) stats_rows = m;
@@ -217,7 +233,8 @@ extern "C" {
 int msplat_ops_status(void* stream) {
     return guarded([&] {
         const bool tc16 = gave_up_tc16(static_cast<cudaStream_t>(stream));
-        if (gave_up_tcv(static_cast<cudaStream_t>(stream)) || tc16)
+        const bool rows = gave_up_rows(static_cast<cudaStream_t>(stream));
+        if (gave_up_tcv(static_cast<cudaStream_t>(stream)) || tc16 || rows)
             throw Error(MSPLAT_ERR_CUDA, "a kernel gave up waiting: the results since the last call are not valid");
     });
 }
@@ -294,6 +311,14 @@ int msplat_linear_backward(int64_t m, int64_t n, int64_t k, const void* x, int64
         Arena a(workspace);
         const BackwardPlan plan(a, m, n, k, activation, dtype);
         check_workspace(a, workspace, workspace_bytes);
+        if (plan.rows) {
+            if (!dx && !dw && !dbias) return;
+            launch_rows_layer(m, n, k, x, ldx, w, ldw, preact, ldz, activation, dy, lddy, dx, lddx,
+                              dw ? plan.slab : nullptr, dbias ? plan.sums : nullptr, dtype, s);
+            if (dw) launch_slab_sum(n, k, plan.slab, slab_ld(k), plan.pieces, dw, lddw, 1.f, nullptr, nullptr, 0, dtype, s);
+            if (dbias) launch_slab_sum(1, n, plan.sums, n, plan.pieces, dbias, n, 1.f, nullptr, nullptr, 0, dtype, s);
+            return;
+        }
         const void* dz = dy;
         int64_t lddz = lddy;
         if (activation != MSPLAT_ACT_NONE || dbias) {
@@ -390,6 +415,18 @@ int msplat_loss_cross_entropy(int64_t m, int64_t v, int64_t d, const void* x, in
         const LossPlan plan(a, m, v, d, grad, dtype);
         check_workspace(a, workspace, workspace_bytes);
 
+        const float g_scale = dtype == MSPLAT_DTYPE_F16 ? 16384.f : 1.f;
+        if (plan.rows) {
+            const int blocks = rows_blocks(m);
+            launch_count_labels(m, targets, v, plan.partial, blocks, s);
+            launch_loss_total(plan.partial, blocks, 0.f, weight * logit_scale / g_scale, nullptr, plan.alpha, s);
+            launch_rows_labels(m, v, d, x, ldx, w, ldw, targets, logit_scale, g_scale, plan.alpha, row_loss,
+                               plan.partial, dx, lddx, dw ? plan.slab_w : nullptr, dtype, s);
+            if (loss) launch_loss_total(plan.partial, blocks, weight, 0.f, loss, nullptr, s);
+            if (dw)
+                launch_slab_sum(v, d, plan.slab_w, slab_ld(d), blocks, dw, lddw, 1.f, plan.alpha, nullptr, 0, dtype, s);
+            return;
+        }
         Product logits{};
         logits.M = m; logits.N = v; logits.R = d;
         logits.A = x; logits.lda = ldx;
@@ -398,7 +435,7 @@ int msplat_loss_cross_entropy(int64_t m, int64_t v, int64_t d, const void* x, in
         logits.targets = targets;
         logits.labels = v;
         logits.logit_scale = logit_scale;
-        logits.g_scale = dtype == MSPLAT_DTYPE_F16 ? 16384.f : 1.f;
+        logits.g_scale = g_scale;
 
         if (grad) {
             launch_labelled_rows(m, d, x, ldx, targets, v, plan.x, plan.ldx, dtype, s);
@@ -427,7 +464,7 @@ int msplat_loss_cross_entropy(int64_t m, int64_t v, int64_t d, const void* x, in
             launch_join(j, s);
             joined += join_blocks(rows);
         }
-        launch_loss_total(plan.partial, joined, weight, weight * logit_scale / logits.g_scale, loss, plan.alpha, s);
+        launch_loss_total(plan.partial, joined, weight, weight * logit_scale / g_scale, loss, plan.alpha, s);
         if (!grad) return;
 
         const int64_t all = plan.by_rows ? m : v;

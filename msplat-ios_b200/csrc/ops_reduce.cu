@@ -195,6 +195,25 @@ __global__ void __launch_bounds__(1024) k_join(JoinArgs a, int shares) {
     }
 }
 
+__global__ void __launch_bounds__(256) k_count_labels(int64_t m, const int32_t* targets, int64_t labels,
+                                                      double* partial) {
+    int n = 0;
+    for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < m; i += gridDim.x * 256ll) {
+        const int32_t t = targets[i];
+        n += t >= 0 && t < labels;
+    }
+    __shared__ int warps[8];
+    n = __reduce_add_sync(~0u, n);
+    if (threadIdx.x % 32 == 0) warps[threadIdx.x / 32] = n;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        double t = 0;
+        for (int q = 0; q < 8; ++q) t += warps[q];
+        partial[2 * blockIdx.x] = 0;
+        partial[2 * blockIdx.x + 1] = t;
+    }
+}
+
 __global__ void __launch_bounds__(256) k_loss_total(const double* partial, int blocks, float weight, float factor,
                                                     float* loss, float* alpha) {
     __shared__ double ssum[256], scount[256];
@@ -215,7 +234,7 @@ __global__ void __launch_bounds__(256) k_loss_total(const double* partial, int b
     if (threadIdx.x == 0) {
         const bool any = scount[0] > 0;
         if (loss) *loss = any ? (float)(weight * ssum[0] / scount[0]) : 0.f;
-        *alpha = any ? (float)(factor / scount[0]) : 0.f;
+        if (alpha) *alpha = any ? (float)(factor / scount[0]) : 0.f;
     }
 }
 
@@ -349,6 +368,13 @@ void launch_join(const JoinArgs& a, cudaStream_t s) {
     int shares = 1;
     while (shares < 32 && shares < a.blocks) shares *= 2;
     k_join<<<join_blocks(a.m), dim3(32, 32), 0, s>>>(a, shares);
+    OPS_CK(cudaGetLastError());
+}
+
+void launch_count_labels(int64_t m, const int32_t* targets, int64_t labels, double* partial, int blocks,
+                         cudaStream_t s) {
+    note_launches(1);
+    k_count_labels<<<blocks, 256, 0, s>>>(m, targets, labels, partial);
     OPS_CK(cudaGetLastError());
 }
 

@@ -1,0 +1,606 @@
+// ops_rows.cu — everything that many rows need against a small matrix, in one
+// pass over the rows: the gradients of a narrow layer, and the label loss with
+// its gradients against a small table.
+//
+// With at most 128 columns of w (labels, or a layer's outputs) and 64 of x, all
+// that belongs to 128 rows fits into one SM, so x is read once and dx written
+// once, and nothing of size rows x columns leaves the chip:
+//   labels: s = x w^T; row statistics; g = softmax - one-hot; dx = g w; dw += g^T x
+//   layer:  g = dy act'(z);                                dx = g w; dw += g^T x
+// x, g and w lie in shared memory once each, in the 128-byte swizzle; the tensor
+// cores read the same bytes as rows or transposed (x as A of s and B of dw, g as A
+// of dx and of dw, w as B of s and of dx). 32-bit factors are split into three
+// bf16 parts as in ops_tcv.cu. dw stays in TMEM for four tiles (512 elements of
+// its reduction, because the tensor cores truncate) and is then added to the
+// block's own partial sums; the blocks' are summed by launch_slab_sum.
+//
+// Warp 0 issues the products, warps 4-7 load and split x, warps 8-15 make g (two
+// warps per 32 rows share a row's columns), warps 16-19 write dx and drain dw.
+// With three parts there is room for one tile at a time only, so its steps follow
+// one another; what bounds the kernel is that chain, 1.5 us to 2.5 us a tile.
+#include <cstddef>
+
+#include "ops_load.cuh"
+
+namespace msplat {
+namespace ops {
+
+struct RowsArgs {
+    int64_t m;
+    int v, d;             // columns of g (rows of w), columns of x and w
+    const void* x;
+    int64_t ldx;
+    const void* w;
+    int64_t ldw;
+    // labels
+    const int32_t* targets;
+    float to2, g_scale;   // logits in log2 units; factor of g in 16 bits
+    const float* alpha;   // factor of dx
+    float* row_loss;
+    double* partial;      // [blocks][2]
+    // layer
+    const void* z;
+    int64_t ldz;
+    int act;
+    const void* dy;
+    int64_t lddy;
+    float* sums;          // [blocks][v] column sums of g, or null
+    // outputs
+    void* dx;
+    int64_t lddx;
+    float* slab;          // [blocks][v][slab_ld(d)], or null
+    int dx_tma;
+    int vec_x, vec_w, vec_z, vec_dy;
+};
+
+namespace {
+
+constexpr int kThreads = 640;
+constexpr int kIssueRegs = 32, kLoadRegs = 104, kGRegs = 112, kEpiRegs = 112;
+static_assert(128 * (kIssueRegs + kLoadRegs + kEpiRegs) + 256 * kGRegs <= kThreads * 96, "setmaxnreg would wait forever");
+constexpr int kDrain = 4;  // tiles that dw stays in TMEM
+constexpr int kSmall = 64 * 128;  // bytes of 64 lines
+
+struct Smem {
+    uint64_t x_full, s_full, g_full, done, out_empty, drain, pair[4];
+    alignas(16) float2 half[2][2][kBM];  // by tile parity and half: a row's largest logit and sum
+    float sums[8][128];
+    double loss[8][2];
+    uint32_t tmem;
+    int gave_up;
+};
+
+__device__ __forceinline__ uint32_t float_bits(float v) { return __float_as_uint(v); }
+
+// Eight values into the parts' swizzled places.
+template <typename T>
+__device__ __forceinline__ void put8(uint8_t* at, uint32_t plane, const float* v) {
+    Chunk<T> c;
+#pragma unroll
+    for (int q = 0; q < Chunk<T>::kWords; ++q) {
+        if constexpr (sizeof(T) == 4)
+            c.w[q] = float_bits(v[q]);
+        else
+            c.w[q] = pack2<T>(v[2 * q], v[2 * q + 1]);
+    }
+    c.store(at, plane);
+}
+template <typename T>
+__device__ __forceinline__ float chunk_at(const Chunk<T>& c, int q) {
+    if constexpr (sizeof(T) == 4) {
+        return __uint_as_float(c.w[q]);
+    } else {
+        const float2 f = unpack2<T>(c.w[q / 2]);
+        return q & 1 ? f.y : f.x;
+    }
+}
+
+__device__ __forceinline__ uint4 load16(const uint4* g, bool ok) {
+    // volatile: not moved down to its use, behind the wait that it overlaps
+    uint4 v;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %5, 0;\n\t"
+        "mov.b32 %0, 0;\n\tmov.b32 %1, 0;\n\tmov.b32 %2, 0;\n\tmov.b32 %3, 0;\n\t"
+        "@p ld.global.nc.v4.b32 {%0, %1, %2, %3}, [%4];\n\t}"
+        : "=&r"(v.x), "=&r"(v.y), "=&r"(v.z), "=&r"(v.w)
+        : "l"(g), "r"((uint32_t)ok));
+    return v;
+}
+
+// 128 rows from i0, columns c0 .. c0 + 63, by THREADS threads as load_tile; all
+// loads of an aligned matrix are issued before any is used. With targets, rows
+// without a label are zeros.
+template <typename T, int THREADS>
+__device__ __forceinline__ void load_rows(const Operand<T>& o, int64_t i0, int c0, int t, Chunk<T> (&c)[kBM * 8 / THREADS],
+                                          const int32_t* targets = nullptr, int labels = 0) {
+    constexpr int kN = kBM * 8 / THREADS;
+    bool has[kN];
+#pragma unroll
+    for (int q = 0; q < kN; ++q) {
+        const int64_t row = i0 + t / 8 + THREADS / 8 * q;
+        has[q] = row < o.rows;
+        if (targets && has[q]) {
+            const int32_t l = __ldg(targets + row);
+            has[q] = l >= 0 && l < labels;
+        }
+    }
+    if (!o.vec) {
+        load_tile<T, kBM, THREADS>(o, i0, c0, t, c);
+#pragma unroll
+        for (int q = 0; q < kN; ++q)
+            if (!has[q]) c[q].zero();
+        return;
+    }
+    const int col = c0 + t % 8 * 8, n = (int)min((int64_t)8, o.cols - col);
+    const T* g = o.p + (i0 + t / 8) * o.ld + col;
+#pragma unroll
+    for (int q = 0; q < kN; ++q)
+#pragma unroll
+        for (int k = 0; k < Chunk<T>::kPieces; ++k) {
+            const uint4 v = load16(reinterpret_cast<const uint4*>(g + (int64_t)(THREADS / 8 * q) * o.ld) + k, n == 8 && has[q]);
+            c[q].w[4 * k] = v.x; c[q].w[4 * k + 1] = v.y; c[q].w[4 * k + 2] = v.z; c[q].w[4 * k + 3] = v.w;
+        }
+    if (n > 0 && n < 8) {
+#pragma unroll
+        for (int q = 0; q < kN; ++q)
+            if (has[q]) c[q].load_each(g + (int64_t)(THREADS / 8 * q) * o.ld, n);
+    }
+}
+
+// The products of the parts, the corrections into `corr`.
+template <int P>
+__device__ __forceinline__ void products(uint32_t d, uint32_t corr, const uint64_t (&a)[P], const uint64_t (&b)[P],
+                                         uint32_t idesc, bool fresh) {
+    if constexpr (P > 1) {
+        const int pa[5] = {0, 2, 1, 0, 1}, pb[5] = {2, 0, 1, 1, 0};
+#pragma unroll
+        for (int q = 0; q < 5; ++q) tc_mma(corr, a[pa[q]], b[pb[q]], idesc, !fresh || q > 0);
+    }
+    tc_mma(d, a[0], b[0], idesc, !fresh);
+}
+
+template <int P>
+__device__ __forceinline__ void accumulators(uint32_t d, uint32_t corr, float (&v)[32]) {
+    uint32_t raw[32];
+    tmem_load32(d, raw);
+    tmem_wait();
+#pragma unroll
+    for (int q = 0; q < 32; ++q) v[q] = __uint_as_float(raw[q]);
+    if constexpr (P > 1) {
+        tmem_load32(corr, raw);
+        tmem_wait();
+#pragma unroll
+        for (int q = 0; q < 32; ++q) v[q] += __uint_as_float(raw[q]);
+    }
+}
+
+template <typename T, bool LABELS, int VG, int ACT>
+__global__ void __launch_bounds__(kThreads, 1)
+    k_rows(const __grid_constant__ RowsArgs p, const __grid_constant__ CUtensorMap map_dx, const uint32_t idesc_s,
+           const uint32_t idesc_x, const uint32_t idesc_w) {
+    constexpr int P = planes<T>();
+    constexpr int kXPlane = kBM * 128, kWPlane = VG * kSmall, kGPlane = VG * kBM * 128, kGGroup = kBM * 128;
+    constexpr uint32_t kS = 0, kSCorr = 128, kX = 256, kXCorr = 320, kW = 384, kWCorr = 448;
+    extern __shared__ __align__(1024) uint8_t dyn[];
+    __shared__ Smem sm;
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    uint8_t* xs = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(dyn) + 1023) & ~(uintptr_t)1023);
+    uint8_t* ws = xs + P * kXPlane;
+    uint8_t* gs = ws + P * kWPlane;
+    uint8_t* boxes = gs + P * kGPlane;
+    const int64_t tiles = (p.m + kBM - 1) / kBM;
+
+    if (threadIdx.x == 0) {
+        mbar_init(smem_u32(&sm.x_full), 4);
+        mbar_init(smem_u32(&sm.s_full), 1);
+        mbar_init(smem_u32(&sm.g_full), 8);
+        mbar_init(smem_u32(&sm.done), 1);
+        mbar_init(smem_u32(&sm.out_empty), 4);
+        mbar_init(smem_u32(&sm.drain), 1);
+        for (int q = 0; q < 4; ++q) mbar_init(smem_u32(&sm.pair[q]), 2);
+        sm.gave_up = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) tmem_alloc(smem_u32(&sm.tmem), 512);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = sm.tmem;
+    volatile int* gave_up = &sm.gave_up;
+    uint32_t phase = 0;  // of this block's current tile, for every barrier
+
+    if (warp < 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssueRegs));
+        bool ok = true;
+        int count = 0;
+        for (int64_t tile = blockIdx.x; warp == 0 && tile < tiles; tile += gridDim.x, ++count, phase ^= 1) {
+            if (!(ok = mbar_wait(smem_u32(&sm.x_full), phase, gave_up))) break;
+            tc_fence_after();
+            const uint32_t x = smem_u32(xs), w = smem_u32(ws), g = smem_u32(gs);
+            if (LABELS) {
+                if (elect_one()) {
+                    for (int k = 0; k * 16 < p.d; ++k) {
+                        uint64_t a[P], b[P];
+#pragma unroll
+                        for (int q = 0; q < P; ++q) {
+                            a[q] = smem_desc(x + q * kXPlane + k * 32, 16);
+                            b[q] = smem_desc(w + q * kWPlane + k * 32, 16);
+                        }
+                        products<P>(tmem + kS, tmem + kSCorr, a, b, idesc_s, k == 0);
+                    }
+                    tc_commit(smem_u32(&sm.s_full));
+                }
+                __syncwarp();
+            }
+            if (!(ok = mbar_wait(smem_u32(&sm.g_full), phase, gave_up))) break;
+            if (!(ok = mbar_wait(smem_u32(&sm.out_empty), phase ^ 1, gave_up))) break;
+            tc_fence_after();
+            if (elect_one()) {
+                if (p.dx)
+                    for (int k = 0; k * 16 < p.v; ++k) {
+                        uint64_t a[P], b[P];
+#pragma unroll
+                        for (int q = 0; q < P; ++q) {
+                            a[q] = smem_desc(g + q * kGPlane + k / 4 * kGGroup + k % 4 * 32, 16);
+                            b[q] = smem_desc(w + q * kWPlane + k * 2048, 16);
+                        }
+                        products<P>(tmem + kX, tmem + kXCorr, a, b, idesc_x, k == 0);
+                    }
+                if (p.slab)
+                    for (int k = 0; k < kBM / 16; ++k) {
+                        uint64_t a[P], b[P];
+#pragma unroll
+                        for (int q = 0; q < P; ++q) {
+                            // of a single group the second 64 rows of the result are not read
+                            a[q] = smem_desc(g + q * kGPlane + k * 2048, kGGroup);
+                            b[q] = smem_desc(x + q * kXPlane + k * 2048, 16);
+                        }
+                        products<P>(tmem + kW, tmem + kWCorr, a, b, idesc_w, k == 0 && count % kDrain == 0);
+                    }
+                tc_commit(smem_u32(&sm.done));
+            }
+            __syncwarp();
+        }
+        if (!ok && warp == 0) {
+            if (elect_one()) {
+                tc_commit(smem_u32(&sm.drain));
+                mbar_wait_bounded(smem_u32(&sm.drain), 0, nullptr);
+            }
+            __syncwarp();
+        }
+    } else if (warp < 8) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kLoadRegs));
+        const int t = threadIdx.x - 128;
+        const Operand<T> ox = operand<T>(p.x, p.ldx, p.m, p.d, false, p.vec_x);
+        const Operand<T> ow = operand<T>(p.w, p.ldw, p.v, p.d, false, p.vec_w);
+        for (int q = 0; q < VG; ++q) {
+            Chunk<T> c[4];
+            load_tile<T, 64, 128>(ow, 64 * q, 0, t, c);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int line = t / 8 + 16 * e;
+                c[e].store(ws + q * kSmall + line * 128 + ((t % 8) ^ (line & 7)) * 16, kWPlane);
+            }
+        }
+        for (int64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x, phase ^= 1) {
+            Chunk<T> c[8];
+            load_rows<T, 128>(ox, tile * kBM, 0, t, c, LABELS ? p.targets : nullptr, p.v);
+            if (!mbar_wait(smem_u32(&sm.done), phase ^ 1, gave_up)) break;
+            store_tile<T, kBM, 128>(xs, t, c);
+            fence_async();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&sm.x_full));
+        }
+    } else if (warp < 16) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kGRegs));
+        if constexpr (LABELS) {
+            const int quarter = warp % 4, half = (warp - 8) / 4, line = quarter * 32 + lane;
+            const uint32_t s = tmem + ((uint32_t)quarter << 21) + half * 32 * VG;
+            uint8_t* out = gs + line * 128;
+            double sum = 0, count = 0;
+            for (int64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x, phase ^= 1) {
+                const int64_t i = tile * kBM + line;
+                const int32_t target = i < p.m ? __ldg(p.targets + i) : -1;
+                const bool has = target >= 0 && target < p.v;
+                if (!mbar_wait(smem_u32(&sm.s_full), phase, gave_up)) break;
+                tc_fence_after();
+                float v[VG][32], top = -INFINITY, mine = 0.f;
+                const int at = target - half * 32 * VG;
+#pragma unroll
+                for (int c = 0; c < VG; ++c) {
+                    accumulators<P>(s + kS + 32 * c, s + kSCorr + 32 * c, v[c]);
+                    const int left = p.v - half * 32 * VG - 32 * c;
+#pragma unroll
+                    for (int q = 0; q < 32; ++q) {
+                        v[c][q] = q < left ? __fmul_rn(v[c][q], p.to2) : -INFINITY;
+                        top = fmaxf(top, v[c][q]);
+                    }
+                    if (__any_sync(~0u, at >= 32 * c && at < 32 * c + 32)) {
+#pragma unroll
+                        for (int q = 0; q < 32; ++q)
+                            if (32 * c + q == at) mine = v[c][q];
+                    }
+                }
+                const float ref = top == -INFINITY ? 0.f : top;
+                float total = 0.f;
+#pragma unroll
+                for (int c = 0; c < VG; ++c)
+#pragma unroll
+                    for (int q = 0; q < 32; ++q) {
+                        v[c][q] = exp2_fast(v[c][q] - ref);
+                        total += v[c][q];
+                    }
+                // the two halves of a row
+                const int parity = phase;
+                sm.half[parity][half][line] = make_float2(ref, total);
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&sm.pair[quarter]));
+                if (!mbar_wait(smem_u32(&sm.pair[quarter]), phase, gave_up)) break;
+                const float2 o = sm.half[parity][half ^ 1][line];
+                // (a half without columns has the sum 0 and no say)
+                const float all = o.y == 0.f ? ref : total == 0.f ? o.x : fmaxf(ref, o.x);
+                const float up = total == 0.f ? 0.f : exp2_fast(ref - all);
+                const float sums = total * up + (o.y == 0.f ? 0.f : o.y * exp2_fast(o.x - all));
+                const bool holds = has && at >= 0 && at < 32 * VG;
+                const float row = ((all - mine) + log2f(sums)) * kLn2;
+                if (holds) {
+                    sum += row;
+                    count += 1;
+                }
+                if (p.row_loss && i < p.m && (holds || (!has && half == 0))) p.row_loss[i] = has ? row : 0.f;
+                const float factor = up / sums;
+#pragma unroll
+                for (int c = 0; c < VG; ++c) {
+#pragma unroll
+                    for (int q = 0; q < 32; ++q) v[c][q] *= factor;
+                    if (__any_sync(~0u, at >= 32 * c && at < 32 * c + 32)) {
+#pragma unroll
+                        for (int q = 0; q < 32; ++q)
+                            if (32 * c + q == at) v[c][q] -= 1.f;
+                    }
+#pragma unroll
+                    for (int q = 0; q < 32; ++q) v[c][q] = has ? (sizeof(T) == 2 ? v[c][q] * p.g_scale : v[c][q]) : 0.f;
+                }
+                if (!mbar_wait(smem_u32(&sm.done), phase ^ 1, gave_up)) break;
+#pragma unroll
+                for (int c = 0; c < VG; ++c)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int piece = half * 4 * VG + 4 * c + e;
+                        put8<T>(out + piece / 8 * kGGroup + ((piece % 8) ^ (line & 7)) * 16, kGPlane, &v[c][8 * e]);
+                    }
+                fence_async();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&sm.g_full));
+            }
+            for (int q = 16; q; q >>= 1) {
+                sum += __shfl_xor_sync(~0u, sum, q);
+                count += __shfl_xor_sync(~0u, count, q);
+            }
+            if (lane == 0) {
+                sm.loss[warp - 8][0] = sum;
+                sm.loss[warp - 8][1] = count;
+            }
+        } else {
+            const int t = threadIdx.x - 256;
+            const Operand<T> oy = operand<T>(p.dy, p.lddy, p.m, p.v, false, p.vec_dy);
+            const Operand<T> oz = operand<T>(p.z, p.ldz, p.m, p.v, false, p.vec_z);
+            float sums[VG][8];
+#pragma unroll
+            for (int c = 0; c < VG; ++c)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) sums[c][e] = 0.f;
+            bool ok = true;
+            for (int64_t tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x, phase ^= 1) {
+#pragma unroll
+                for (int c = 0; c < VG; ++c) {
+                    Chunk<T> a[4], b[4];
+                    load_rows<T, 256>(oy, tile * kBM, 64 * c, t, a);
+                    if (ACT != MSPLAT_ACT_NONE) load_rows<T, 256>(oz, tile * kBM, 64 * c, t, b);
+                    if (c == 0 && !(ok = mbar_wait(smem_u32(&sm.done), phase ^ 1, gave_up))) break;
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        const int line = t / 8 + 32 * q;
+                        float g[8];
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            g[e] = chunk_at(a[q], e);
+                            if (ACT != MSPLAT_ACT_NONE) g[e] *= act_slope<ACT>(chunk_at(b[q], e));
+                            sums[c][e] += g[e];
+                        }
+                        put8<T>(gs + c * kGGroup + line * 128 + ((t % 8) ^ (line & 7)) * 16, kGPlane, g);
+                    }
+                }
+                if (!ok) break;
+                fence_async();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&sm.g_full));
+            }
+#pragma unroll
+            for (int c = 0; c < VG; ++c)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    float s = sums[c][e];
+                    s += __shfl_xor_sync(~0u, s, 8);
+                    s += __shfl_xor_sync(~0u, s, 16);
+                    if (lane < 8) sm.sums[warp - 8][64 * c + 8 * lane + e] = s;
+                }
+        }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kEpiRegs));
+        const int quarter = warp % 4;
+        const uint32_t d = tmem + ((uint32_t)quarter << 21);
+        uint8_t* box = boxes + quarter * kBoxBytes;
+        const float alpha = LABELS ? __ldg(p.alpha) : 1.f;
+        float* mine = p.slab ? p.slab + ((int64_t)blockIdx.x * p.v + quarter * 32 + lane) * slab_ld(p.d) : nullptr;
+        const bool keeps = p.slab && quarter * 32 + lane < p.v;
+        int count = 0;
+        for (int64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x, phase ^= 1, ++count) {
+            const int64_t i0 = tile * kBM + quarter * 32;
+            if (!mbar_wait(smem_u32(&sm.done), phase, gave_up)) break;
+            tc_fence_after();
+            if (p.dx && i0 < p.m) {
+                bool zero = false;
+                if (LABELS && i0 + lane < p.m) {
+                    const int32_t l = __ldg(p.targets + i0 + lane);
+                    zero = l < 0 || l >= p.v;
+                }
+                for (int c = 0; c < p.d; c += 32) {
+                    float v[32];
+                    accumulators<P>(d + kX + c, d + kXCorr + c, v);
+                    if (LABELS) {
+#pragma unroll
+                        for (int q = 0; q < 32; ++q) v[q] = zero ? 0.f : v[q] * alpha;
+                    }
+                    const int first = sizeof(T) == 2 && c ? 4 : 0;
+                    const bool send = sizeof(T) == 4 || c + 32 >= p.d;
+                    if (p.dx_tma && first == 0) {
+                        if (lane == 0) bulk_wait_read(0);
+                        __syncwarp();
+                    }
+                    box_write<T>(box, lane, first, v);
+                    if (p.dx_tma) {
+                        if (!send) continue;
+                        fence_async();
+                        __syncwarp();
+                        if (lane == 0) {
+                            tma_store(&map_dx, smem_u32(box), first ? 0 : c, (int)i0, 0, false);
+                            bulk_commit();
+                        }
+                    } else {
+                        __syncwarp();
+                        box_copy<T, false>(box, first, static_cast<T*>(p.dx), p.lddx, i0, c, p.m, p.d, lane);
+                        __syncwarp();
+                    }
+                }
+            }
+            if (p.slab && (count % kDrain == kDrain - 1 || tile + gridDim.x >= tiles)) {
+                for (int c = 0; c < p.d; c += 32) {
+                    float v[32];
+                    accumulators<P>(d + kW + c, d + kWCorr + c, v);
+                    if (!keeps) continue;
+                    float4* o = reinterpret_cast<float4*>(mine + c);
+                    const int n = ((int)slab_ld(p.d) - c) / 4;
+#pragma unroll
+                    for (int q = 0; q < 8; ++q) {
+                        if (q >= n) break;
+                        float4 f = count < kDrain ? make_float4(0.f, 0.f, 0.f, 0.f) : o[q];
+                        f.x += v[4 * q];
+                        f.y += v[4 * q + 1];
+                        f.z += v[4 * q + 2];
+                        f.w += v[4 * q + 3];
+                        o[q] = f;
+                    }
+                }
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&sm.out_empty));
+        }
+        if (lane == 0) bulk_wait_all();
+    }
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 1) tmem_free(tmem, 512);
+    if (LABELS) {
+        if (threadIdx.x == 0) {
+            double sum = 0, count = 0;
+            for (int q = 0; q < 8; ++q) {
+                sum += sm.loss[q][0];
+                count += sm.loss[q][1];
+            }
+            p.partial[2 * blockIdx.x] = sum;
+            p.partial[2 * blockIdx.x + 1] = count;
+        }
+    } else if (p.sums && threadIdx.x < p.v) {
+        float s = 0.f;
+        for (int q = 0; q < 8; ++q) s += sm.sums[q][threadIdx.x];
+        p.sums[(int64_t)blockIdx.x * p.v + threadIdx.x] = s;
+    }
+}
+
+template <typename T, bool LABELS, int VG, int ACT>
+void run(const RowsArgs& a, const CUtensorMap& dx, cudaStream_t s) {
+    constexpr int P = planes<T>();
+    constexpr int bytes = P * (kBM * 128 + VG * kSmall + VG * kBM * 128) + 4 * kBoxBytes + 1024;
+    static_assert(bytes + sizeof(Smem) + 1024 <= 227 * 1024, "shared memory of a block");
+    const bool bf16 = !std::is_same<T, __half>::value;
+    const int nv = (int)round_up(a.v, 16), nd = (int)round_up(a.d, 16);
+    allow_shared<k_rows<T, LABELS, VG, ACT>>(bytes);
+    note_launches(1);
+    k_rows<T, LABELS, VG, ACT><<<rows_blocks(a.m), kThreads, bytes, s>>>(
+        a, dx, instr_desc(bf16, false, false, nv), instr_desc(bf16, false, true, nd), instr_desc(bf16, true, true, nd));
+    OPS_CK(cudaGetLastError());
+}
+
+template <typename T, bool LABELS, int ACT>
+void sized(const RowsArgs& a, const CUtensorMap& dx, cudaStream_t s) {
+    if (a.v <= 64)
+        run<T, LABELS, 1, ACT>(a, dx, s);
+    else
+        run<T, LABELS, 2, ACT>(a, dx, s);
+}
+
+template <typename T>
+void typed(RowsArgs a, int dtype, cudaStream_t s) {
+    a.vec_x = vectors<T>(a.x, a.ldx, a.m);
+    a.vec_w = vectors<T>(a.w, a.ldw, a.v);
+    a.vec_z = a.z && vectors<T>(a.z, a.ldz, a.m);
+    a.vec_dy = a.dy && vectors<T>(a.dy, a.lddy, a.m);
+    CUtensorMap dx{};
+    a.dx_tma = a.dx && tma_ready(a.dx, a.lddx, a.m, sizeof(T));
+    if (a.dx_tma) dx = map_output(a.dx, a.m, a.d, a.lddx, 1, dtype);
+    if (a.targets) return sized<T, true, MSPLAT_ACT_NONE>(a, dx, s);
+    switch (a.act) {
+        case MSPLAT_ACT_RELU: return sized<T, false, MSPLAT_ACT_RELU>(a, dx, s);
+        case MSPLAT_ACT_GELU: return sized<T, false, MSPLAT_ACT_GELU>(a, dx, s);
+        case MSPLAT_ACT_SILU: return sized<T, false, MSPLAT_ACT_SILU>(a, dx, s);
+        case MSPLAT_ACT_SIGMOID: return sized<T, false, MSPLAT_ACT_SIGMOID>(a, dx, s);
+        default: return sized<T, false, MSPLAT_ACT_NONE>(a, dx, s);
+    }
+}
+
+void launch(const RowsArgs& a, int dtype, cudaStream_t s) {
+    if (dtype == MSPLAT_DTYPE_F32)
+        typed<float>(a, dtype, s);
+    else if (dtype == MSPLAT_DTYPE_F16)
+        typed<__half>(a, dtype, s);
+    else
+        typed<__nv_bfloat16>(a, dtype, s);
+}
+
+}  // namespace
+
+bool gave_up_rows(cudaStream_t s) { return take_gave_up(s); }
+
+bool fits_rows(int64_t m, int64_t v, int64_t d) { return v <= 128 && d <= 64 && m >= 8192; }
+int rows_blocks(int64_t m) { return (int)std::min<int64_t>(ceil_div(m, kBM), kSMs); }
+
+void launch_rows_labels(int64_t m, int64_t v, int64_t d, const void* x, int64_t ldx, const void* w, int64_t ldw,
+                        const int32_t* targets, float logit_scale, float g_scale, const float* alpha, float* row_loss,
+                        double* partial, void* dx, int64_t lddx, float* slab, int dtype, cudaStream_t s) {
+    RowsArgs a{};
+    a.m = m; a.v = (int)v; a.d = (int)d;
+    a.x = x; a.ldx = ldx; a.w = w; a.ldw = ldw;
+    a.targets = targets; a.to2 = logit_scale * kLog2e; a.g_scale = g_scale; a.alpha = alpha;
+    a.row_loss = row_loss; a.partial = partial;
+    a.dx = dx; a.lddx = lddx; a.slab = slab;
+    launch(a, dtype, s);
+}
+
+void launch_rows_layer(int64_t m, int64_t n, int64_t k, const void* x, int64_t ldx, const void* w, int64_t ldw,
+                       const void* z, int64_t ldz, int act, const void* dy, int64_t lddy, void* dx, int64_t lddx,
+                       float* slab, float* sums, int dtype, cudaStream_t s) {
+    RowsArgs a{};
+    a.m = m; a.v = (int)n; a.d = (int)k;
+    a.x = x; a.ldx = ldx; a.w = w; a.ldw = ldw;
+    a.z = z; a.ldz = ldz; a.act = act; a.dy = dy; a.lddy = lddy;
+    a.dx = dx; a.lddx = lddx; a.slab = slab; a.sums = sums;
+    launch(a, dtype, s);
+}
+
+}  // namespace ops
+}  // namespace msplat

@@ -20,7 +20,7 @@
 // block keeps to one column of tiles and loads them once (resident).
 #include <cstddef>
 
-#include "ops_tc.cuh"
+#include "ops_load.cuh"
 
 namespace msplat {
 namespace ops {
@@ -45,144 +45,6 @@ struct Smem {
     int gave_up;
 };
 static_assert(offsetof(Smem, bias) % 16 == 0 && sizeof(Smem) <= 2048, "read as float4; share_memory counts 2048");
-
-template <typename T>
-constexpr int planes() { return sizeof(T) == 4 ? 3 : 1; }
-
-// Eight consecutive elements on their way to shared memory, as 32-bit words.
-template <typename T>
-struct Chunk {
-    static constexpr int kWords = 8 * sizeof(T) / 4;
-    uint32_t w[kWords];
-
-    __device__ __forceinline__ void zero() {
-#pragma unroll
-        for (int q = 0; q < kWords; ++q) w[q] = 0;
-    }
-    // Element by element: the first n.
-    __device__ __forceinline__ void load_each(const T* g, int n) {
-        zero();
-#pragma unroll
-        for (int q = 0; q < 8; ++q)
-            if (q < n) {
-                if constexpr (sizeof(T) == 4)
-                    w[q] = __ldg(reinterpret_cast<const uint32_t*>(g) + q);
-                else
-                    w[q / 2] |= (uint32_t)__ldg(reinterpret_cast<const uint16_t*>(g) + q) << 16 * (q & 1);
-            }
-    }
-    // From a 16-byte boundary.
-    __device__ __forceinline__ void load_aligned(const T* g) {
-#pragma unroll
-        for (int q = 0; q < kWords / 4; ++q) {
-            const uint4 v = __ldg(reinterpret_cast<const uint4*>(g) + q);
-            w[4 * q] = v.x; w[4 * q + 1] = v.y; w[4 * q + 2] = v.z; w[4 * q + 3] = v.w;
-        }
-    }
-    // From any element: the 16-byte pieces around it, shifted into place.
-    __device__ __forceinline__ void load_around(const T* g) {
-        const uintptr_t a = reinterpret_cast<uintptr_t>(g);
-        const uint32_t off = (uint32_t)(a & 15);
-        const uint4* at = reinterpret_cast<const uint4*>(a & ~(uintptr_t)15);
-        uint32_t r[kWords + 4];
-#pragma unroll
-        for (int q = 0; q < kWords / 4 + 1; ++q) {
-            const uint4 v = q < kWords / 4 || off ? __ldg(at + q) : make_uint4(0, 0, 0, 0);
-            r[4 * q] = v.x; r[4 * q + 1] = v.y; r[4 * q + 2] = v.z; r[4 * q + 3] = v.w;
-        }
-#pragma unroll
-        for (int q = 0; q < kWords + 2; ++q) r[q] = off & 8 ? r[q + 2] : r[q];
-#pragma unroll
-        for (int q = 0; q < kWords + 1; ++q) r[q] = off & 4 ? r[q + 1] : r[q];
-#pragma unroll
-        for (int q = 0; q < kWords; ++q) w[q] = sizeof(T) == 4 ? r[q] : __funnelshift_r(r[q], r[q + 1], (off & 2) * 8);
-    }
-    // Zeros behind the first n elements.
-    __device__ __forceinline__ void keep(int n) {
-#pragma unroll
-        for (int q = 0; q < kWords; ++q) {
-            if constexpr (sizeof(T) == 4)
-                w[q] = q < n ? w[q] : 0;
-            else
-                w[q] = 2 * q + 1 < n ? w[q] : 2 * q < n ? w[q] & 0xFFFF : 0;
-        }
-    }
-    // The parts, `plane` bytes apart.
-    __device__ __forceinline__ void store(uint8_t* s, uint32_t plane) const {
-        if constexpr (sizeof(T) == 4) {
-            uint32_t o[3][4];
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                float a = __uint_as_float(w[2 * q]), b = __uint_as_float(w[2 * q + 1]);
-#pragma unroll
-                for (int k = 0; k < 3; ++k) {
-                    o[k][q] = pack2<__nv_bfloat16>(a, b);
-                    a -= __uint_as_float(o[k][q] << 16);
-                    b -= __uint_as_float(o[k][q] & 0xFFFF0000u);
-                }
-            }
-#pragma unroll
-            for (int k = 0; k < 3; ++k)
-                *reinterpret_cast<uint4*>(s + k * plane) = make_uint4(o[k][0], o[k][1], o[k][2], o[k][3]);
-        } else {
-            *reinterpret_cast<uint4*>(s) = make_uint4(w[0], w[1], w[2], w[3]);
-        }
-    }
-};
-
-// One operand as rows of consecutive elements: [i][r], or [r][i] when mn.
-template <typename T>
-struct Operand {
-    const T* p;
-    int64_t ld, rows, cols;
-    bool mn, vec;
-    const T* end;  // behind the last element
-};
-template <typename T>
-__device__ __forceinline__ Operand<T> operand(const void* p, int64_t ld, int64_t I, int64_t R, bool mn, bool vec) {
-    Operand<T> o{static_cast<const T*>(p), ld, mn ? R : I, mn ? I : R, mn, vec, nullptr};
-    o.end = o.p + (o.rows - 1) * ld + o.cols;
-    return o;
-}
-
-// The stage's tile of an operand: WIDE / 32 chunks of eight per thread, thread
-// t taking chunk t % 8 of row t / 8 + 32 q (eight lanes read one row's 64
-// elements and fill one 128-byte row of shared memory).
-template <typename T, int WIDE>
-__device__ __forceinline__ void load_tile(const Operand<T>& o, int64_t i0, int64_t r0, int t, Chunk<T> (&c)[WIDE / 32]) {
-#pragma unroll
-    for (int q = 0; q < WIDE / 32; ++q) {
-        const int line = t / 8 + 32 * q;
-        // mn: 64 rows of r per group of 64 i
-        const int64_t row = o.mn ? r0 + line % 64 : i0 + line;
-        const int64_t col = (o.mn ? i0 + line / 64 * 64 : r0) + t % 8 * 8;
-        if (row >= o.rows || col >= o.cols) {
-            c[q].zero();
-            continue;
-        }
-        const T* g = o.p + row * o.ld + col;
-        const int n = (int)min((int64_t)8, o.cols - col);
-        // whole 16-byte pieces are read where the matrix has all of them
-        const uintptr_t from = reinterpret_cast<uintptr_t>(g) & ~(uintptr_t)15;
-        if (o.vec && n == 8) {
-            c[q].load_aligned(g);
-        } else if (from >= reinterpret_cast<uintptr_t>(o.p) &&
-                   from + 8 * sizeof(T) + 16 <= reinterpret_cast<uintptr_t>(o.end)) {
-            c[q].load_around(g);
-            if (n < 8) c[q].keep(n);
-        } else {
-            c[q].load_each(g, n);
-        }
-    }
-}
-template <typename T, int WIDE>
-__device__ __forceinline__ void store_tile(uint8_t* s, int t, const Chunk<T> (&c)[WIDE / 32]) {
-#pragma unroll
-    for (int q = 0; q < WIDE / 32; ++q) {
-        const int line = t / 8 + 32 * q;
-        c[q].store(s + line * 128 + ((t % 8) ^ (line & 7)) * 16, WIDE * 128);
-    }
-}
 
 template <typename T, int EPI, int BN>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -229,8 +91,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         const Operand<T> ob = operand<T>(p.B, p.ldb, p.N, p.R, p.b_mn, vec_b);
         for (int q = 0; q < tl.resident; ++q) {
             Chunk<T> b[BN / 32];
-            load_tile<T, BN>(ob, (int64_t)(blockIdx.x % tl.tiles_n) * BN, (int64_t)q * kBR, t, b);
-            store_tile<T, BN>(resident + (size_t)q * kB, t, b);
+            load_tile<T, BN, kLoaders>(ob, (int64_t)(blockIdx.x % tl.tiles_n) * BN, (int64_t)q * kBR, t, b);
+            store_tile<T, BN, kLoaders>(resident + (size_t)q * kB, t, b);
         }
         int stage = 0;
         uint32_t phase = 0;
@@ -241,12 +103,12 @@ __global__ void __launch_bounds__(kThreads, 1)
             tile_of(p, tl, w, tm, tn, split, r0, r1);
             for (int64_t r = r0; r < r1; r += kBR) {
                 Chunk<T> a[kBM / 32], b[BN / 32];
-                load_tile<T, kBM>(oa, (int64_t)tm * kBM, r, t, a);
-                if (!tl.resident) load_tile<T, BN>(ob, (int64_t)tn * BN, r, t, b);
+                load_tile<T, kBM, kLoaders>(oa, (int64_t)tm * kBM, r, t, a);
+                if (!tl.resident) load_tile<T, BN, kLoaders>(ob, (int64_t)tn * BN, r, t, b);
                 if (!(ok = mbar_wait(smem_u32(&sm.empty[stage]), phase ^ 1, gave_up))) break;
                 uint8_t* s = tiles + (size_t)stage * stage_bytes;
-                store_tile<T, kBM>(s, t, a);
-                if (!tl.resident) store_tile<T, BN>(s + kA, t, b);
+                store_tile<T, kBM, kLoaders>(s, t, a);
+                if (!tl.resident) store_tile<T, BN, kLoaders>(s + kA, t, b);
                 fence_async();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(smem_u32(&sm.full[stage]));
@@ -393,11 +255,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncthreads();
     tc_fence_after();
     if (warp == 1) tmem_free(tmem, 2 * kTileCols);
-}
-
-template <typename T>
-bool vectors(const void* q, int64_t ld, int64_t rows) {
-    return reinterpret_cast<uintptr_t>(q) % 16 == 0 && (rows <= 1 || ld % (16 / (int64_t)sizeof(T)) == 0);
 }
 
 template <typename T, int EPI, int BN>

@@ -457,3 +457,60 @@ def test_linear_neighbours_in_the_record(t):
             R.check(ops().linear_forward(x, w), *R.linear(x, w, None, "none", None, R.TYPES[t])[:2], f"lead {lead}")
             dx, dw, _ = ops().linear_backward(x, w, normal(106, m, n, t))
             R.check(dw, *R.linear_grads(x, w, normal(106, m, n, t), None, "none", R.TYPES[t])[1], f"dw, lead {lead}")
+
+
+# ---- many rows against a small matrix ----------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("m,v,d", [(8192, 1, 1), (8193, 2, 7), (9000, 64, 32), (8320, 65, 33), (20_001, 101, 32),
+                                   (8200, 128, 64), (150_000, 17, 48), (100_000, 40, 16)])
+def test_loss_small_table(m, v, d, t):
+    x, w = normal(110, m, d, t, std=2.0), normal(111, v, d, t, std=d ** -0.5)
+    check_loss(x, w, labels(112, m, v), 1.5 if m % 2 else 1.0, 4096.0 if t == "f16" else 1.0)
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("pad,lead", [(8, 0), (8, 8), (5, 1)])
+def test_loss_small_table_strides_and_masked_rows(pad, lead, t):
+    m, v, d = 8300, 70, 40
+    x, w = normal(113, m, d, t, pad=pad, lead=lead), normal(114, v, d, t, pad=pad, lead=lead)
+    targets = labels(115, m, v, off=0.4)
+    off = ~((targets >= 0) & (targets < v))
+    x[off] = torch.where(torch.arange(d, device="cuda") % 2 == 0, float("nan"), float("inf")).to(x.dtype)
+    check_loss(x, w, targets, 1.0, 100.0)
+    loss, row, dx, dw = ops().loss_cross_entropy(x, w, torch.full_like(targets, -5))
+    assert float(loss) == 0 and not row.any() and not dx.any() and not dw.any()
+
+
+@pytest.mark.parametrize("t", TYPES)
+def test_loss_small_table_extreme_logits(t):
+    big = {"f32": 1e30, "bf16": 1e30, "f16": 6e4}[t]
+    x = torch.zeros(8192, 16, dtype=R.TYPES[t], device="cuda")
+    x[:, 0] = big
+    for v in (50, 100):
+        w = torch.zeros(v, 16, dtype=R.TYPES[t], device="cuda")
+        w[v - 1, 0], w[:v - 2, 0] = 1, -1
+        targets = torch.full((8192,), v - 1, dtype=torch.int32, device="cuda")
+        loss, row, dx, dw = ops().loss_cross_entropy(x, w, targets)
+        assert float(loss) == 0 and not row.any() and not dx.any() and not dw.any()
+        targets[:] = v - 2
+        loss, row, dx, dw = ops().loss_cross_entropy(x, w, targets, weight=64.0)
+        assert torch.allclose(row, x[:, 0].float(), rtol=4 * 2.0 ** -24, atol=0) and bool(torch.isfinite(dx).all())
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("m,n,k", [(8192, 1, 1), (8193, 3, 20), (9000, 64, 32), (8320, 65, 33), (20_001, 100, 64),
+                                   (8200, 128, 64), (150_000, 16, 48), (77_777, 33, 7)])
+@pytest.mark.parametrize("pad,lead", [(0, 0), (13, 10)])
+def test_linear_backward_narrow(m, n, k, pad, lead, t):
+    act = ACTS[(m + n + k) % 5]
+    x, w = normal(116, m, k, t, pad=pad, lead=lead), normal(117, n, k, t, std=k ** -0.5)
+    z, dy = normal(118, m, n, t), normal(119, m, n, t, pad=pad, lead=lead)
+    full = ops().linear_backward(x, w, dy, preact=z, activation=act)
+    for got, (want, bound), name in zip(full, R.linear_grads(x, w, dy, z, act, R.TYPES[t]), ("dx", "dw", "dbias")):
+        R.check(got, want, bound, name)
+    for need in ((1, 0, 0), (0, 1, 0), (0, 0, 1)):
+        part = ops().linear_backward(x, w, dy, preact=z, activation=act, need_dx=need[0], need_dw=need[1], need_dbias=need[2])
+        for a, b in zip(full, part):
+            assert b is None or torch.equal(a, b)
