@@ -14,10 +14,11 @@
 // its reduction, because the tensor cores truncate) and is then added to the
 // block's own partial sums; the blocks' are summed by launch_slab_sum.
 //
-// Warp 0 issues the products, warps 4-7 load and split x, warps 8-15 make g (two
-// warps per 32 rows share a row's columns), warps 16-19 write dx and drain dw.
+// Warp 0 issues the products, warps 8-15 make g (two warps per 32 rows share a
+// row's columns), warps 4-7 load and split x for the next tile and then write dx
+// of this one; dw has two accumulators so that one can be drained meanwhile.
 // With three parts there is room for one tile at a time only, so its steps follow
-// one another; what bounds the kernel is that chain, 1.5 us to 2.5 us a tile.
+// one another; what bounds the kernel is that chain.
 #include <cstddef>
 
 #include "ops_load.cuh"
@@ -55,9 +56,7 @@ struct RowsArgs {
 
 namespace {
 
-constexpr int kThreads = 640;
-constexpr int kIssueRegs = 32, kLoadRegs = 104, kGRegs = 112, kEpiRegs = 112;
-static_assert(128 * (kIssueRegs + kLoadRegs + kEpiRegs) + 256 * kGRegs <= kThreads * 96, "setmaxnreg would wait forever");
+constexpr int kThreads = 512;
 constexpr int kDrain = 4;  // tiles that dw stays in TMEM
 constexpr int kSmall = 64 * 128;  // bytes of 64 lines
 
@@ -147,19 +146,18 @@ __device__ __forceinline__ void load_rows(const Operand<T>& o, int64_t i0, int c
     }
 }
 
-// The products of the parts, the corrections into `corr`.
+// The corrections of the parts' products (in front of them, or apart).
 template <int P>
-__device__ __forceinline__ void products(uint32_t d, uint32_t corr, const uint64_t (&a)[P], const uint64_t (&b)[P],
-                                         uint32_t idesc, bool fresh) {
+__device__ __forceinline__ void corrections(uint32_t d, const uint64_t (&a)[P], const uint64_t (&b)[P], uint32_t idesc,
+                                            bool fresh) {
     if constexpr (P > 1) {
         const int pa[5] = {0, 2, 1, 0, 1}, pb[5] = {2, 0, 1, 1, 0};
 #pragma unroll
-        for (int q = 0; q < 5; ++q) tc_mma(corr, a[pa[q]], b[pb[q]], idesc, !fresh || q > 0);
+        for (int q = 0; q < 5; ++q) tc_mma(d, a[pa[q]], b[pb[q]], idesc, !fresh || q > 0);
     }
-    tc_mma(d, a[0], b[0], idesc, !fresh);
 }
 
-template <int P>
+template <int P>  // P > 1: with the corrections
 __device__ __forceinline__ void accumulators(uint32_t d, uint32_t corr, float (&v)[32]) {
     uint32_t raw[32];
     tmem_load32(d, raw);
@@ -180,7 +178,9 @@ __global__ void __launch_bounds__(kThreads, 1)
            const uint32_t idesc_x, const uint32_t idesc_w) {
     constexpr int P = planes<T>();
     constexpr int kXPlane = kBM * 128, kWPlane = VG * kSmall, kGPlane = VG * kBM * 128, kGGroup = kBM * 128;
-    constexpr uint32_t kS = 0, kSCorr = 128, kX = 256, kXCorr = 320, kW = 384, kWCorr = 448;
+    // TMEM: s (its corrections are added first, while the sums are small), dx and
+    // two times dw with their corrections apart
+    constexpr uint32_t kS = 0, kX = 128, kXCorr = 192, kW = 256, kWCorr = 64, kWNext = 128;
     extern __shared__ __align__(1024) uint8_t dyn[];
     __shared__ Smem sm;
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
@@ -210,7 +210,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint32_t phase = 0;  // of this block's current tile, for every barrier
 
     if (warp < 4) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssueRegs));
         bool ok = true;
         int count = 0;
         for (int64_t tile = blockIdx.x; warp == 0 && tile < tiles; tile += gridDim.x, ++count, phase ^= 1) {
@@ -219,14 +218,19 @@ __global__ void __launch_bounds__(kThreads, 1)
             const uint32_t x = smem_u32(xs), w = smem_u32(ws), g = smem_u32(gs);
             if (LABELS) {
                 if (elect_one()) {
-                    for (int k = 0; k * 16 < p.d; ++k) {
+                    const int steps = (p.d + 15) / 16;
+                    for (int k = 0; k < (P > 1 ? 2 : 1) * steps; ++k) {
+                        const int at = (k % steps) * 32;
                         uint64_t a[P], b[P];
 #pragma unroll
                         for (int q = 0; q < P; ++q) {
-                            a[q] = smem_desc(x + q * kXPlane + k * 32, 16);
-                            b[q] = smem_desc(w + q * kWPlane + k * 32, 16);
+                            a[q] = smem_desc(x + q * kXPlane + at, 16);
+                            b[q] = smem_desc(w + q * kWPlane + at, 16);
                         }
-                        products<P>(tmem + kS, tmem + kSCorr, a, b, idesc_s, k == 0);
+                        if (P > 1 && k < steps)
+                            corrections<P>(tmem + kS, a, b, idesc_s, k == 0);
+                        else
+                            tc_mma(tmem + kS, a[0], b[0], idesc_s, k > 0);
                     }
                     tc_commit(smem_u32(&sm.s_full));
                 }
@@ -244,7 +248,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                             a[q] = smem_desc(g + q * kGPlane + k / 4 * kGGroup + k % 4 * 32, 16);
                             b[q] = smem_desc(w + q * kWPlane + k * 2048, 16);
                         }
-                        products<P>(tmem + kX, tmem + kXCorr, a, b, idesc_x, k == 0);
+                        corrections<P>(tmem + kXCorr, a, b, idesc_x, k == 0);
+                        tc_mma(tmem + kX, a[0], b[0], idesc_x, k > 0);
                     }
                 if (p.slab)
                     for (int k = 0; k < kBM / 16; ++k) {
@@ -255,7 +260,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                             a[q] = smem_desc(g + q * kGPlane + k * 2048, kGGroup);
                             b[q] = smem_desc(x + q * kXPlane + k * 2048, 16);
                         }
-                        products<P>(tmem + kW, tmem + kWCorr, a, b, idesc_w, k == 0 && count % kDrain == 0);
+                        const uint32_t dw = tmem + kW + (count / kDrain & 1) * kWNext;
+                        const bool fresh = k == 0 && count % kDrain == 0;
+                        corrections<P>(dw + kWCorr, a, b, idesc_w, fresh);
+                        tc_mma(dw, a[0], b[0], idesc_w, !fresh);
                     }
                 tc_commit(smem_u32(&sm.done));
             }
@@ -269,7 +277,6 @@ __global__ void __launch_bounds__(kThreads, 1)
             __syncwarp();
         }
     } else if (warp < 8) {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kLoadRegs));
         const int t = threadIdx.x - 128;
         const Operand<T> ox = operand<T>(p.x, p.ldx, p.m, p.d, false, p.vec_x);
         const Operand<T> ow = operand<T>(p.w, p.ldw, p.v, p.d, false, p.vec_w);
@@ -282,17 +289,95 @@ __global__ void __launch_bounds__(kThreads, 1)
                 c[e].store(ws + q * kSmall + line * 128 + ((t % 8) ^ (line & 7)) * 16, kWPlane);
             }
         }
-        for (int64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x, phase ^= 1) {
-            Chunk<T> c[8];
-            load_rows<T, 128>(ox, tile * kBM, 0, t, c, LABELS ? p.targets : nullptr, p.v);
-            if (!mbar_wait(smem_u32(&sm.done), phase ^ 1, gave_up)) break;
-            store_tile<T, kBM, 128>(xs, t, c);
-            fence_async();
+        const int quarter = warp % 4;
+        const uint32_t d = tmem + ((uint32_t)quarter << 21);
+        uint8_t* box = boxes + quarter * kBoxBytes;
+        const float alpha = LABELS ? __ldg(p.alpha) : 1.f;
+        float* mine = p.slab ? p.slab + ((int64_t)blockIdx.x * p.v + quarter * 32 + lane) * slab_ld(p.d) : nullptr;
+        const bool keeps = p.slab && quarter * 32 + lane < p.v;
+        const int count_all = (int)((tiles - blockIdx.x + gridDim.x - 1) / gridDim.x);
+        // step `count`: x of tile `count` goes in and dx of the one before comes out
+        for (int count = 0; count <= count_all; ++count, phase ^= 1) {
+            const int64_t tile = blockIdx.x + (int64_t)count * gridDim.x;
+            if (count < count_all) {
+                Chunk<T> c[8];
+                load_rows<T, 128>(ox, tile * kBM, 0, t, c, LABELS ? p.targets : nullptr, p.v);
+                if (!mbar_wait(smem_u32(&sm.done), phase ^ 1, gave_up)) break;
+                store_tile<T, kBM, 128>(xs, t, c);
+                fence_async();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&sm.x_full));
+            } else if (!mbar_wait(smem_u32(&sm.done), phase ^ 1, gave_up)) {
+                break;
+            }
+            if (count == 0) continue;
+            const int64_t i0 = (tile - gridDim.x) * kBM + quarter * 32;
+            tc_fence_after();
+            if (p.dx && i0 < p.m) {
+                bool zero = false;
+                if (LABELS && i0 + lane < p.m) {
+                    const int32_t l = __ldg(p.targets + i0 + lane);
+                    zero = l < 0 || l >= p.v;
+                }
+                for (int c = 0; c < p.d; c += 32) {
+                    float v[32];
+                    accumulators<P>(d + kX + c, d + kXCorr + c, v);
+                    if (LABELS) {
+#pragma unroll
+                        for (int q = 0; q < 32; ++q) v[q] = zero ? 0.f : v[q] * alpha;
+                    }
+                    const int first = sizeof(T) == 2 && c ? 4 : 0;
+                    const bool send = sizeof(T) == 4 || c + 32 >= p.d;
+                    if (p.dx_tma && first == 0) {
+                        if (lane == 0) bulk_wait_read(0);
+                        __syncwarp();
+                    }
+                    box_write<T>(box, lane, first, v);
+                    if (p.dx_tma) {
+                        if (!send) continue;
+                        fence_async();
+                        __syncwarp();
+                        if (lane == 0) {
+                            tma_store(&map_dx, smem_u32(box), first ? 0 : c, (int)i0, 0, false);
+                            bulk_commit();
+                        }
+                    } else {
+                        __syncwarp();
+                        box_copy<T, false>(box, first, static_cast<T*>(p.dx), p.lddx, i0, c, p.m, p.d, lane);
+                        __syncwarp();
+                    }
+                }
+            }
+            // dx's accumulators are free; dw's other ones too: they were drained
+            // before this step, in program order
+            const bool drains = p.slab && (count % kDrain == 0 || count == count_all);
+            tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(smem_u32(&sm.x_full));
+            if (lane == 0) mbar_arrive(smem_u32(&sm.out_empty));
+            if (drains) {
+                const uint32_t dw = d + kW + ((count - 1) / kDrain & 1) * kWNext;
+                for (int c = 0; c < p.d; c += 32) {
+                    float v[32];
+                    accumulators<P>(dw + c, dw + kWCorr + c, v);
+                    if (!keeps) continue;
+                    float4* o = reinterpret_cast<float4*>(mine + c);
+                    const int n = ((int)slab_ld(p.d) - c) / 4;
+#pragma unroll
+                    for (int q = 0; q < 8; ++q) {
+                        if (q >= n) break;
+                        float4 f = count <= kDrain ? make_float4(0.f, 0.f, 0.f, 0.f) : o[q];
+                        f.x += v[4 * q];
+                        f.y += v[4 * q + 1];
+                        f.z += v[4 * q + 2];
+                        f.w += v[4 * q + 3];
+                        o[q] = f;
+                    }
+                }
+                tc_fence_before();
+            }
         }
-    } else if (warp < 16) {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kGRegs));
+        if (lane == 0) bulk_wait_all();
+    } else {
         if constexpr (LABELS) {
             const int quarter = warp % 4, half = (warp - 8) / 4, line = quarter * 32 + lane;
             const uint32_t s = tmem + ((uint32_t)quarter << 21) + half * 32 * VG;
@@ -308,7 +393,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const int at = target - half * 32 * VG;
 #pragma unroll
                 for (int c = 0; c < VG; ++c) {
-                    accumulators<P>(s + kS + 32 * c, s + kSCorr + 32 * c, v[c]);
+                    accumulators<1>(s + kS + 32 * c, 0, v[c]);
                     const int left = p.v - half * 32 * VG - 32 * c;
 #pragma unroll
                     for (int q = 0; q < 32; ++q) {
@@ -427,78 +512,6 @@ __global__ void __launch_bounds__(kThreads, 1)
                     if (lane < 8) sm.sums[warp - 8][64 * c + 8 * lane + e] = s;
                 }
         }
-    } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kEpiRegs));
-        const int quarter = warp % 4;
-        const uint32_t d = tmem + ((uint32_t)quarter << 21);
-        uint8_t* box = boxes + quarter * kBoxBytes;
-        const float alpha = LABELS ? __ldg(p.alpha) : 1.f;
-        float* mine = p.slab ? p.slab + ((int64_t)blockIdx.x * p.v + quarter * 32 + lane) * slab_ld(p.d) : nullptr;
-        const bool keeps = p.slab && quarter * 32 + lane < p.v;
-        int count = 0;
-        for (int64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x, phase ^= 1, ++count) {
-            const int64_t i0 = tile * kBM + quarter * 32;
-            if (!mbar_wait(smem_u32(&sm.done), phase, gave_up)) break;
-            tc_fence_after();
-            if (p.dx && i0 < p.m) {
-                bool zero = false;
-                if (LABELS && i0 + lane < p.m) {
-                    const int32_t l = __ldg(p.targets + i0 + lane);
-                    zero = l < 0 || l >= p.v;
-                }
-                for (int c = 0; c < p.d; c += 32) {
-                    float v[32];
-                    accumulators<P>(d + kX + c, d + kXCorr + c, v);
-                    if (LABELS) {
-#pragma unroll
-                        for (int q = 0; q < 32; ++q) v[q] = zero ? 0.f : v[q] * alpha;
-                    }
-                    const int first = sizeof(T) == 2 && c ? 4 : 0;
-                    const bool send = sizeof(T) == 4 || c + 32 >= p.d;
-                    if (p.dx_tma && first == 0) {
-                        if (lane == 0) bulk_wait_read(0);
-                        __syncwarp();
-                    }
-                    box_write<T>(box, lane, first, v);
-                    if (p.dx_tma) {
-                        if (!send) continue;
-                        fence_async();
-                        __syncwarp();
-                        if (lane == 0) {
-                            tma_store(&map_dx, smem_u32(box), first ? 0 : c, (int)i0, 0, false);
-                            bulk_commit();
-                        }
-                    } else {
-                        __syncwarp();
-                        box_copy<T, false>(box, first, static_cast<T*>(p.dx), p.lddx, i0, c, p.m, p.d, lane);
-                        __syncwarp();
-                    }
-                }
-            }
-            if (p.slab && (count % kDrain == kDrain - 1 || tile + gridDim.x >= tiles)) {
-                for (int c = 0; c < p.d; c += 32) {
-                    float v[32];
-                    accumulators<P>(d + kW + c, d + kWCorr + c, v);
-                    if (!keeps) continue;
-                    float4* o = reinterpret_cast<float4*>(mine + c);
-                    const int n = ((int)slab_ld(p.d) - c) / 4;
-#pragma unroll
-                    for (int q = 0; q < 8; ++q) {
-                        if (q >= n) break;
-                        float4 f = count < kDrain ? make_float4(0.f, 0.f, 0.f, 0.f) : o[q];
-                        f.x += v[4 * q];
-                        f.y += v[4 * q + 1];
-                        f.z += v[4 * q + 2];
-                        f.w += v[4 * q + 3];
-                        o[q] = f;
-                    }
-                }
-            }
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(smem_u32(&sm.out_empty));
-        }
-        if (lane == 0) bulk_wait_all();
     }
     __syncwarp();
     tc_fence_before();
