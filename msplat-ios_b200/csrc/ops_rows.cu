@@ -61,7 +61,7 @@ constexpr int kDrain = 4;  // tiles that dw stays in TMEM
 constexpr int kSmall = 64 * 128;  // bytes of 64 lines
 
 struct Smem {
-    uint64_t x_full, s_full, g_full, done, out_empty, drain, pair[4];
+    uint64_t x_full, x_free, s_full, g_full[2], g_free[2], done, out_empty, drain, pair[4];
     alignas(16) float2 half[2][2][kBM];  // by tile parity and half: a row's largest logit and sum
     float sums[8][128];
     double loss[8][2];
@@ -172,12 +172,38 @@ __device__ __forceinline__ void accumulators(uint32_t d, uint32_t corr, float (&
     }
 }
 
+// Shared memory: the parts of x, w and g, g twice where that fits, and dx's boxes.
+template <typename T, int VG>
+struct Layout {
+    static constexpr int P = planes<T>(), kXPlane = kBM * 128, kWPlane = VG * kSmall, kGPlane = VG * kBM * 128;
+    static constexpr int fixed = P * (kXPlane + kWPlane) + 4 * kBoxBytes + 1024, most = 227 * 1024 - sizeof(Smem) - 1024;
+    static constexpr int buffers = fixed + 2 * P * kGPlane <= most ? 2 : 1;
+    static constexpr int bytes = fixed + buffers * P * kGPlane;
+    static_assert(bytes <= most, "shared memory of a block");
+};
+
+// v[at] for at in 0 .. 31, by halving
+__device__ __forceinline__ float pick32(const float (&v)[32], int at) {
+    float a[16];
+#pragma unroll
+    for (int q = 0; q < 16; ++q) a[q] = at & 1 ? v[2 * q + 1] : v[2 * q];
+#pragma unroll
+    for (int q = 0; q < 8; ++q) a[q] = at & 2 ? a[2 * q + 1] : a[2 * q];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) a[q] = at & 4 ? a[2 * q + 1] : a[2 * q];
+#pragma unroll
+    for (int q = 0; q < 2; ++q) a[q] = at & 8 ? a[2 * q + 1] : a[2 * q];
+    return at & 16 ? a[1] : a[0];
+}
+
 template <typename T, bool LABELS, int VG, int ACT>
 __global__ void __launch_bounds__(kThreads, 1)
     k_rows(const __grid_constant__ RowsArgs p, const __grid_constant__ CUtensorMap map_dx, const uint32_t idesc_s,
            const uint32_t idesc_x, const uint32_t idesc_w) {
     constexpr int P = planes<T>();
-    constexpr int kXPlane = kBM * 128, kWPlane = VG * kSmall, kGPlane = VG * kBM * 128, kGGroup = kBM * 128;
+    using L = Layout<T, VG>;
+    constexpr int kXPlane = L::kXPlane, kWPlane = L::kWPlane, kGPlane = L::kGPlane, kGGroup = kBM * 128;
+    constexpr int kBuffers = L::buffers;
     // TMEM: s (its corrections are added first, while the sums are small), dx and
     // two times dw with their corrections apart
     constexpr uint32_t kS = 0, kX = 128, kXCorr = 192, kW = 256, kWCorr = 64, kWNext = 128;
@@ -186,14 +212,18 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     uint8_t* xs = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(dyn) + 1023) & ~(uintptr_t)1023);
     uint8_t* ws = xs + P * kXPlane;
-    uint8_t* gs = ws + P * kWPlane;
-    uint8_t* boxes = gs + P * kGPlane;
+    uint8_t* g0 = ws + P * kWPlane;
+    uint8_t* boxes = g0 + kBuffers * P * kGPlane;
     const int64_t tiles = (p.m + kBM - 1) / kBM;
 
     if (threadIdx.x == 0) {
         mbar_init(smem_u32(&sm.x_full), 4);
         mbar_init(smem_u32(&sm.s_full), 1);
-        mbar_init(smem_u32(&sm.g_full), 8);
+        mbar_init(smem_u32(&sm.x_free), 1);
+        for (int q = 0; q < 2; ++q) {
+            mbar_init(smem_u32(&sm.g_full[q]), 8);
+            mbar_init(smem_u32(&sm.g_free[q]), 1);
+        }
         mbar_init(smem_u32(&sm.done), 1);
         mbar_init(smem_u32(&sm.out_empty), 4);
         mbar_init(smem_u32(&sm.drain), 1);
@@ -215,7 +245,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int64_t tile = blockIdx.x; warp == 0 && tile < tiles; tile += gridDim.x, ++count, phase ^= 1) {
             if (!(ok = mbar_wait(smem_u32(&sm.x_full), phase, gave_up))) break;
             tc_fence_after();
-            const uint32_t x = smem_u32(xs), w = smem_u32(ws), g = smem_u32(gs);
+            const int buffer = count % kBuffers;
+            const uint32_t x = smem_u32(xs), w = smem_u32(ws), g = smem_u32(g0 + buffer * P * kGPlane);
             if (LABELS) {
                 if (elect_one()) {
                     const int steps = (p.d + 15) / 16;
@@ -236,21 +267,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 __syncwarp();
             }
-            if (!(ok = mbar_wait(smem_u32(&sm.g_full), phase, gave_up))) break;
+            if (!(ok = mbar_wait(smem_u32(&sm.g_full[buffer]), count / kBuffers & 1, gave_up))) break;
             if (!(ok = mbar_wait(smem_u32(&sm.out_empty), phase ^ 1, gave_up))) break;
             tc_fence_after();
             if (elect_one()) {
-                if (p.dx)
-                    for (int k = 0; k * 16 < p.v; ++k) {
-                        uint64_t a[P], b[P];
-#pragma unroll
-                        for (int q = 0; q < P; ++q) {
-                            a[q] = smem_desc(g + q * kGPlane + k / 4 * kGGroup + k % 4 * 32, 16);
-                            b[q] = smem_desc(w + q * kWPlane + k * 2048, 16);
-                        }
-                        corrections<P>(tmem + kXCorr, a, b, idesc_x, k == 0);
-                        tc_mma(tmem + kX, a[0], b[0], idesc_x, k > 0);
-                    }
+                // dw first: x is free for the next tile while dx runs
                 if (p.slab)
                     for (int k = 0; k < kBM / 16; ++k) {
                         uint64_t a[P], b[P];
@@ -265,6 +286,19 @@ __global__ void __launch_bounds__(kThreads, 1)
                         corrections<P>(dw + kWCorr, a, b, idesc_w, fresh);
                         tc_mma(dw, a[0], b[0], idesc_w, !fresh);
                     }
+                tc_commit(smem_u32(&sm.x_free));
+                if (p.dx)
+                    for (int k = 0; k * 16 < p.v; ++k) {
+                        uint64_t a[P], b[P];
+#pragma unroll
+                        for (int q = 0; q < P; ++q) {
+                            a[q] = smem_desc(g + q * kGPlane + k / 4 * kGGroup + k % 4 * 32, 16);
+                            b[q] = smem_desc(w + q * kWPlane + k * 2048, 16);
+                        }
+                        corrections<P>(tmem + kXCorr, a, b, idesc_x, k == 0);
+                        tc_mma(tmem + kX, a[0], b[0], idesc_x, k > 0);
+                    }
+                tc_commit(smem_u32(&sm.g_free[buffer]));
                 tc_commit(smem_u32(&sm.done));
             }
             __syncwarp();
@@ -302,15 +336,14 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (count < count_all) {
                 Chunk<T> c[8];
                 load_rows<T, 128>(ox, tile * kBM, 0, t, c, LABELS ? p.targets : nullptr, p.v);
-                if (!mbar_wait(smem_u32(&sm.done), phase ^ 1, gave_up)) break;
+                if (!mbar_wait(smem_u32(&sm.x_free), phase ^ 1, gave_up)) break;
                 store_tile<T, kBM, 128>(xs, t, c);
                 fence_async();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(smem_u32(&sm.x_full));
-            } else if (!mbar_wait(smem_u32(&sm.done), phase ^ 1, gave_up)) {
-                break;
             }
             if (count == 0) continue;
+            if (!mbar_wait(smem_u32(&sm.done), phase ^ 1, gave_up)) break;
             const int64_t i0 = (tile - gridDim.x) * kBM + quarter * 32;
             tc_fence_after();
             if (p.dx && i0 < p.m) {
@@ -381,9 +414,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         if constexpr (LABELS) {
             const int quarter = warp % 4, half = (warp - 8) / 4, line = quarter * 32 + lane;
             const uint32_t s = tmem + ((uint32_t)quarter << 21) + half * 32 * VG;
-            uint8_t* out = gs + line * 128;
             double sum = 0, count = 0;
-            for (int64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x, phase ^= 1) {
+            int turn = 0;
+            for (int64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x, phase ^= 1, ++turn) {
                 const int64_t i = tile * kBM + line;
                 const int32_t target = i < p.m ? __ldg(p.targets + i) : -1;
                 const bool has = target >= 0 && target < p.v;
@@ -391,30 +424,34 @@ __global__ void __launch_bounds__(kThreads, 1)
                 tc_fence_after();
                 float v[VG][32], top = -INFINITY, mine = 0.f;
                 const int at = target - half * 32 * VG;
+                const bool holds = has && at >= 0 && at < 32 * VG;
 #pragma unroll
                 for (int c = 0; c < VG; ++c) {
                     accumulators<1>(s + kS + 32 * c, 0, v[c]);
+#pragma unroll
+                    for (int q = 0; q < 32; ++q) v[c][q] = __fmul_rn(v[c][q], p.to2);
                     const int left = p.v - half * 32 * VG - 32 * c;
+                    if (left < 32) {
 #pragma unroll
-                    for (int q = 0; q < 32; ++q) {
-                        v[c][q] = q < left ? __fmul_rn(v[c][q], p.to2) : -INFINITY;
-                        top = fmaxf(top, v[c][q]);
+                        for (int q = 0; q < 32; ++q) v[c][q] = q < left ? v[c][q] : -INFINITY;
                     }
-                    if (__any_sync(~0u, at >= 32 * c && at < 32 * c + 32)) {
+                    float tops[4] = {top, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                        for (int q = 0; q < 32; ++q)
-                            if (32 * c + q == at) mine = v[c][q];
-                    }
+                    for (int q = 0; q < 32; ++q) tops[q % 4] = fmaxf(tops[q % 4], v[c][q]);
+                    top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+                    const float picked = pick32(v[c], at);
+                    mine = at >> 5 == c ? picked : mine;
                 }
                 const float ref = top == -INFINITY ? 0.f : top;
-                float total = 0.f;
+                float more[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int c = 0; c < VG; ++c)
 #pragma unroll
                     for (int q = 0; q < 32; ++q) {
                         v[c][q] = exp2_fast(v[c][q] - ref);
-                        total += v[c][q];
+                        more[q % 4] += v[c][q];
                     }
+                const float total = (more[0] + more[1]) + (more[2] + more[3]);
                 // the two halves of a row
                 const int parity = phase;
                 sm.half[parity][half][line] = make_float2(ref, total);
@@ -426,38 +463,46 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const float all = o.y == 0.f ? ref : total == 0.f ? o.x : fmaxf(ref, o.x);
                 const float up = total == 0.f ? 0.f : exp2_fast(ref - all);
                 const float sums = total * up + (o.y == 0.f ? 0.f : o.y * exp2_fast(o.x - all));
-                const bool holds = has && at >= 0 && at < 32 * VG;
                 const float row = ((all - mine) + log2f(sums)) * kLn2;
                 if (holds) {
                     sum += row;
                     count += 1;
                 }
                 if (p.row_loss && i < p.m && (holds || (!has && half == 0))) p.row_loss[i] = has ? row : 0.f;
-                const float factor = up / sums;
-#pragma unroll
-                for (int c = 0; c < VG; ++c) {
-#pragma unroll
-                    for (int q = 0; q < 32; ++q) v[c][q] *= factor;
-                    if (__any_sync(~0u, at >= 32 * c && at < 32 * c + 32)) {
-#pragma unroll
-                        for (int q = 0; q < 32; ++q)
-                            if (32 * c + q == at) v[c][q] -= 1.f;
-                    }
-#pragma unroll
-                    for (int q = 0; q < 32; ++q) v[c][q] = has ? (sizeof(T) == 2 ? v[c][q] * p.g_scale : v[c][q]) : 0.f;
-                }
-                if (!mbar_wait(smem_u32(&sm.done), phase ^ 1, gave_up)) break;
+                // rows without a label have x = 0 here, finite values, and the factor 0
+                const float factor = has ? up / sums : 0.f, scaled = sizeof(T) == 2 ? factor * p.g_scale : factor;
+                const int buffer = turn % kBuffers;
+                if (!mbar_wait(smem_u32(&sm.g_free[buffer]), (turn / kBuffers & 1) ^ 1, gave_up)) break;
+                uint8_t* out = g0 + buffer * P * kGPlane + line * 128;
 #pragma unroll
                 for (int c = 0; c < VG; ++c)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         const int piece = half * 4 * VG + 4 * c + e;
-                        put8<T>(out + piece / 8 * kGGroup + ((piece % 8) ^ (line & 7)) * 16, kGPlane, &v[c][8 * e]);
+                        float g[8];
+#pragma unroll
+                        for (int q = 0; q < 8; ++q) g[q] = v[c][8 * e + q] * scaled;
+                        put8<T>(out + piece / 8 * kGGroup + ((piece % 8) ^ (line & 7)) * 16, kGPlane, g);
                     }
+                if (holds) {  // the one-hot, over what was just written
+                    float g = exp2_fast(mine - ref) * factor - 1.f;
+                    if (sizeof(T) == 2) g *= p.g_scale;
+                    uint8_t* one = out + target / 64 * kGGroup + ((target / 8 % 8) ^ (line & 7)) * 16 + target % 8 * 2;
+                    if constexpr (sizeof(T) == 2) {
+                        *reinterpret_cast<T*>(one) = from_f32<T>(g);
+                    } else {
+#pragma unroll
+                        for (int q = 0; q < P; ++q) {
+                            const __nv_bfloat16 h = __float2bfloat16_rn(g);
+                            *reinterpret_cast<__nv_bfloat16*>(one + q * kGPlane) = h;
+                            g -= __bfloat162float(h);
+                        }
+                    }
+                }
                 fence_async();
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(smem_u32(&sm.g_full));
+                if (lane == 0) mbar_arrive(smem_u32(&sm.g_full[buffer]));
             }
             for (int q = 16; q; q >>= 1) {
                 sum += __shfl_xor_sync(~0u, sum, q);
@@ -477,13 +522,16 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                 for (int e = 0; e < 8; ++e) sums[c][e] = 0.f;
             bool ok = true;
-            for (int64_t tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x, phase ^= 1) {
+            int turn = 0;
+            for (int64_t tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x, ++turn) {
+                const int buffer = turn % kBuffers;
+                uint8_t* gs = g0 + buffer * P * kGPlane;
 #pragma unroll
                 for (int c = 0; c < VG; ++c) {
                     Chunk<T> a[4], b[4];
                     load_rows<T, 256>(oy, tile * kBM, 64 * c, t, a);
                     if (ACT != MSPLAT_ACT_NONE) load_rows<T, 256>(oz, tile * kBM, 64 * c, t, b);
-                    if (c == 0 && !(ok = mbar_wait(smem_u32(&sm.done), phase ^ 1, gave_up))) break;
+                    if (c == 0 && !(ok = mbar_wait(smem_u32(&sm.g_free[buffer]), (turn / kBuffers & 1) ^ 1, gave_up))) break;
 #pragma unroll
                     for (int q = 0; q < 4; ++q) {
                         const int line = t / 8 + 32 * q;
@@ -500,7 +548,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (!ok) break;
                 fence_async();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(smem_u32(&sm.g_full));
+                if (lane == 0) mbar_arrive(smem_u32(&sm.g_full[buffer]));
             }
 #pragma unroll
             for (int c = 0; c < VG; ++c)
@@ -537,9 +585,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
 template <typename T, bool LABELS, int VG, int ACT>
 void run(const RowsArgs& a, const CUtensorMap& dx, cudaStream_t s) {
-    constexpr int P = planes<T>();
-    constexpr int bytes = P * (kBM * 128 + VG * kSmall + VG * kBM * 128) + 4 * kBoxBytes + 1024;
-    static_assert(bytes + sizeof(Smem) + 1024 <= 227 * 1024, "shared memory of a block");
+    constexpr int bytes = Layout<T, VG>::bytes;
     const bool bf16 = !std::is_same<T, __half>::value;
     const int nv = (int)round_up(a.v, 16), nd = (int)round_up(a.d, 16);
     allow_shared<k_rows<T, LABELS, VG, ACT>>(bytes);
