@@ -341,6 +341,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                 fence_async();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(smem_u32(&sm.x_full));
+                // the next tile's rows start towards L2 while dx of the last is written
+                const int64_t ahead = (tile + gridDim.x) * kBM + t;
+                if (ahead < p.m)
+                    for (int c = 0; c < p.d; c += 128 / (int)sizeof(T))
+                        asm volatile("prefetch.global.L2 [%0];" ::"l"(ox.p + ahead * p.ldx + c));
             }
             if (count == 0) continue;
             if (!mbar_wait(smem_u32(&sm.done), phase ^ 1, gave_up)) break;
