@@ -70,6 +70,11 @@ struct Chunk {
     }
     // The parts, `plane` bytes apart.
     __device__ __forceinline__ void store(uint8_t* s, uint32_t plane) const {
+        store_to([&](int k) { return s + k * plane; });
+    }
+    // Part k to place(k).
+    template <typename F>
+    __device__ __forceinline__ void store_to(F place) const {
         if constexpr (sizeof(T) == 4) {
             uint32_t o[3][4];
 #pragma unroll
@@ -84,9 +89,9 @@ struct Chunk {
             }
 #pragma unroll
             for (int k = 0; k < 3; ++k)
-                *reinterpret_cast<uint4*>(s + k * plane) = make_uint4(o[k][0], o[k][1], o[k][2], o[k][3]);
+                *reinterpret_cast<uint4*>(place(k)) = make_uint4(o[k][0], o[k][1], o[k][2], o[k][3]);
         } else {
-            *reinterpret_cast<uint4*>(s) = make_uint4(w[0], w[1], w[2], w[3]);
+            *reinterpret_cast<uint4*>(place(0)) = make_uint4(w[0], w[1], w[2], w[3]);
         }
     }
 };

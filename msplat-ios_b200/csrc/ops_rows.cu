@@ -14,6 +14,12 @@
 // its reduction, because the tensor cores truncate) and is then added to the
 // block's own partial sums; the blocks' are summed by launch_slab_sum.
 //
+// PACK (32-bit x of at most 32 columns): the parts of x and of w lie side by side,
+// [h m] in one block of 128-byte rows and [l] in the next, so that one
+// instruction multiplies a part of g with all three (or two) of them: three
+// reads of g per 16 elements in place of six, which is what the products spend
+// their time on (128 x 16 of g are 4 KB of shared memory, as many of x 1 KB).
+//
 // Warp 0 issues the products, warps 8-15 make g (two warps per 32 rows share a
 // row's columns), warps 4-7 load and split x for the next tile and then write dx
 // of this one; dw has two accumulators so that one can be drained meanwhile.
@@ -157,7 +163,7 @@ __device__ __forceinline__ void corrections(uint32_t d, const uint64_t (&a)[P], 
     }
 }
 
-template <int P>  // P > 1: with the corrections
+template <int P>  // P > 1: with the corrections; 4: with two blocks of them
 __device__ __forceinline__ void accumulators(uint32_t d, uint32_t corr, float (&v)[32]) {
     uint32_t raw[32];
     tmem_load32(d, raw);
@@ -170,17 +176,36 @@ __device__ __forceinline__ void accumulators(uint32_t d, uint32_t corr, float (&
 #pragma unroll
         for (int q = 0; q < 32; ++q) v[q] += __uint_as_float(raw[q]);
     }
+    if constexpr (P == 4) {
+        tmem_load32(corr + 32, raw);
+        tmem_wait();
+#pragma unroll
+        for (int q = 0; q < 32; ++q) v[q] += __uint_as_float(raw[q]);
+    }
 }
 
 // Shared memory: the parts of x, w and g, g twice where that fits, and dx's boxes.
-template <typename T, int VG>
+template <typename T, int VG, bool PACK>
 struct Layout {
-    static constexpr int P = planes<T>(), kXPlane = kBM * 128, kWPlane = VG * kSmall, kGPlane = VG * kBM * 128;
-    static constexpr int fixed = P * (kXPlane + kWPlane) + 4 * kBoxBytes + 1024, most = 227 * 1024 - sizeof(Smem) - 1024;
+    static constexpr int P = planes<T>(), kXBlock = kBM * 128, kWBlock = VG * kSmall, kGPlane = VG * kBM * 128;
+    static constexpr int blocks = PACK ? 2 : P;  // of x and of w
+    static constexpr int fixed = blocks * (kXBlock + kWBlock) + 4 * kBoxBytes + 1024,
+                         most = 227 * 1024 - sizeof(Smem) - 1024;
     static constexpr int buffers = fixed + 2 * P * kGPlane <= most ? 2 : 1;
     static constexpr int bytes = fixed + buffers * P * kGPlane;
     static_assert(bytes <= most, "shared memory of a block");
+    // where part q begins in blocks of `block` bytes
+    __device__ static constexpr int part(int q, int block) { return PACK ? (q >> 1) * block + (q & 1) * 64 : q * block; }
 };
+// The parts of eight elements of a line, `piece` the first of them / 8.
+template <typename T, bool PACK>
+__device__ __forceinline__ void store_parts(const Chunk<T>& c, uint8_t* s, int line, int piece, int block) {
+    if (PACK && piece >= 4) return;
+    c.store_to([&](int k) {
+        const int at = PACK ? piece + 4 * (k & 1) : piece;
+        return s + (PACK ? k >> 1 : k) * block + line * 128 + ((at ^ (line & 7)) << 4);
+    });
+}
 
 // v[at] for at in 0 .. 31, by halving
 __device__ __forceinline__ float pick32(const float (&v)[32], int at) {
@@ -196,23 +221,26 @@ __device__ __forceinline__ float pick32(const float (&v)[32], int at) {
     return at & 16 ? a[1] : a[0];
 }
 
-template <typename T, bool LABELS, int VG, int ACT>
+template <typename T, bool LABELS, int VG, int ACT, bool PACK>
 __global__ void __launch_bounds__(kThreads, 1)
     k_rows(const __grid_constant__ RowsArgs p, const __grid_constant__ CUtensorMap map_dx, const uint32_t idesc_s,
            const uint32_t idesc_x, const uint32_t idesc_w) {
+    static_assert(!PACK || sizeof(T) == 4, "parts");
     constexpr int P = planes<T>();
-    using L = Layout<T, VG>;
-    constexpr int kXPlane = L::kXPlane, kWPlane = L::kWPlane, kGPlane = L::kGPlane, kGGroup = kBM * 128;
+    using L = Layout<T, VG, PACK>;
+    constexpr int kXBlock = L::kXBlock, kWBlock = L::kWBlock, kGPlane = L::kGPlane, kGGroup = kBM * 128;
     constexpr int kBuffers = L::buffers;
     // TMEM: s (its corrections are added first, while the sums are small), dx and
-    // two times dw with their corrections apart
-    constexpr uint32_t kS = 0, kX = 128, kXCorr = 192, kW = 256, kWCorr = 64, kWNext = 128;
+    // two times dw with their corrections apart (PACK: in the 64 columns after
+    // the 32 of the sum)
+    constexpr uint32_t kS = 0, kX = 128, kW = 256, kCorr = PACK ? 32 : 64, kWNext = 128;
+    const uint32_t narrower = 4u << 17;  // 32 columns less in an instruction descriptor
     extern __shared__ __align__(1024) uint8_t dyn[];
     __shared__ Smem sm;
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     uint8_t* xs = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(dyn) + 1023) & ~(uintptr_t)1023);
-    uint8_t* ws = xs + P * kXPlane;
-    uint8_t* g0 = ws + P * kWPlane;
+    uint8_t* ws = xs + L::blocks * kXBlock;
+    uint8_t* g0 = ws + L::blocks * kWBlock;
     uint8_t* boxes = g0 + kBuffers * P * kGPlane;
     const int64_t tiles = (p.m + kBM - 1) / kBM;
 
@@ -255,8 +283,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                         uint64_t a[P], b[P];
 #pragma unroll
                         for (int q = 0; q < P; ++q) {
-                            a[q] = smem_desc(x + q * kXPlane + at, 16);
-                            b[q] = smem_desc(w + q * kWPlane + at, 16);
+                            a[q] = smem_desc(x + L::part(q, kXBlock) + at, 16);
+                            b[q] = smem_desc(w + L::part(q, kWBlock) + at, 16);
                         }
                         if (P > 1 && k < steps)
                             corrections<P>(tmem + kS, a, b, idesc_s, k == 0);
@@ -279,12 +307,18 @@ __global__ void __launch_bounds__(kThreads, 1)
                         for (int q = 0; q < P; ++q) {
                             // of a single group the second 64 rows of the result are not read
                             a[q] = smem_desc(g + q * kGPlane + k * 2048, kGGroup);
-                            b[q] = smem_desc(x + q * kXPlane + k * 2048, 16);
+                            b[q] = smem_desc(x + (PACK ? 0 : q * kXBlock) + k * 2048, PACK ? kXBlock : 16);
                         }
                         const uint32_t dw = tmem + kW + (count / kDrain & 1) * kWNext;
                         const bool fresh = k == 0 && count % kDrain == 0;
-                        corrections<P>(dw + kWCorr, a, b, idesc_w, fresh);
-                        tc_mma(dw, a[0], b[0], idesc_w, !fresh);
+                        if constexpr (PACK) {
+                            tc_mma(dw, a[0], b[0], idesc_w, !fresh);
+                            tc_mma(dw + 32, a[1], b[0], idesc_w - narrower, true);
+                            tc_mma(dw + 64, a[2], b[0], idesc_w - 2 * narrower, true);
+                        } else {
+                            corrections<P>(dw + kCorr, a, b, idesc_w, fresh);
+                            tc_mma(dw, a[0], b[0], idesc_w, !fresh);
+                        }
                     }
                 tc_commit(smem_u32(&sm.x_free));
                 if (p.dx)
@@ -293,10 +327,16 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                         for (int q = 0; q < P; ++q) {
                             a[q] = smem_desc(g + q * kGPlane + k / 4 * kGGroup + k % 4 * 32, 16);
-                            b[q] = smem_desc(w + q * kWPlane + k * 2048, 16);
+                            b[q] = smem_desc(w + (PACK ? 0 : q * kWBlock) + k * 2048, PACK ? kWBlock : 16);
                         }
-                        corrections<P>(tmem + kXCorr, a, b, idesc_x, k == 0);
-                        tc_mma(tmem + kX, a[0], b[0], idesc_x, k > 0);
+                        if constexpr (PACK) {
+                            tc_mma(tmem + kX, a[0], b[0], idesc_x, k > 0);
+                            tc_mma(tmem + kX + 32, a[1], b[0], idesc_x - narrower, true);
+                            tc_mma(tmem + kX + 64, a[2], b[0], idesc_x - 2 * narrower, true);
+                        } else {
+                            corrections<P>(tmem + kX + kCorr, a, b, idesc_x, k == 0);
+                            tc_mma(tmem + kX, a[0], b[0], idesc_x, k > 0);
+                        }
                     }
                 tc_commit(smem_u32(&sm.g_free[buffer]));
                 tc_commit(smem_u32(&sm.done));
@@ -320,7 +360,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const int line = t / 8 + 16 * e;
-                c[e].store(ws + q * kSmall + line * 128 + ((t % 8) ^ (line & 7)) * 16, kWPlane);
+                store_parts<T, PACK>(c[e], ws + q * kSmall, line, t % 8, kWBlock);
             }
         }
         const int quarter = warp % 4;
@@ -337,7 +377,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                 Chunk<T> c[8];
                 load_rows<T, 128>(ox, tile * kBM, 0, t, c, LABELS ? p.targets : nullptr, p.v);
                 if (!mbar_wait(smem_u32(&sm.x_free), phase ^ 1, gave_up)) break;
-                store_tile<T, kBM, 128>(xs, t, c);
+#pragma unroll
+                for (int q = 0; q < 8; ++q) store_parts<T, PACK>(c[q], xs, t / 8 + 16 * q, t % 8, kXBlock);
                 fence_async();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(smem_u32(&sm.x_full));
@@ -359,7 +400,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 for (int c = 0; c < p.d; c += 32) {
                     float v[32];
-                    accumulators<P>(d + kX + c, d + kXCorr + c, v);
+                    accumulators<PACK ? 4 : P>(d + kX + c, d + kX + kCorr + c, v);
                     if (LABELS) {
 #pragma unroll
                         for (int q = 0; q < 32; ++q) v[q] = zero ? 0.f : v[q] * alpha;
@@ -396,7 +437,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const uint32_t dw = d + kW + ((count - 1) / kDrain & 1) * kWNext;
                 for (int c = 0; c < p.d; c += 32) {
                     float v[32];
-                    accumulators<P>(dw + c, dw + kWCorr + c, v);
+                    accumulators<PACK ? 4 : P>(dw + c, dw + kCorr + c, v);
                     if (!keeps) continue;
                     float4* o = reinterpret_cast<float4*>(mine + c);
                     const int n = ((int)slab_ld(p.d) - c) / 4;
@@ -588,24 +629,31 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
 }
 
-template <typename T, bool LABELS, int VG, int ACT>
+template <typename T, bool LABELS, int VG, int ACT, bool PACK>
 void run(const RowsArgs& a, const CUtensorMap& dx, cudaStream_t s) {
-    constexpr int bytes = Layout<T, VG>::bytes;
+    constexpr int bytes = Layout<T, VG, PACK>::bytes;
     const bool bf16 = !std::is_same<T, __half>::value;
-    const int nv = (int)round_up(a.v, 16), nd = (int)round_up(a.d, 16);
-    allow_shared<k_rows<T, LABELS, VG, ACT>>(bytes);
+    const int nv = (int)round_up(a.v, 16), nd = PACK ? 96 : (int)round_up(a.d, 16);
+    allow_shared<k_rows<T, LABELS, VG, ACT, PACK>>(bytes);
     note_launches(1);
-    k_rows<T, LABELS, VG, ACT><<<rows_blocks(a.m), kThreads, bytes, s>>>(
+    k_rows<T, LABELS, VG, ACT, PACK><<<rows_blocks(a.m), kThreads, bytes, s>>>(
         a, dx, instr_desc(bf16, false, false, nv), instr_desc(bf16, false, true, nd), instr_desc(bf16, true, true, nd));
     OPS_CK(cudaGetLastError());
 }
 
+template <typename T, bool LABELS, int ACT, bool PACK>
+void wide(const RowsArgs& a, const CUtensorMap& dx, cudaStream_t s) {
+    if (a.v <= 64)
+        run<T, LABELS, 1, ACT, PACK>(a, dx, s);
+    else
+        run<T, LABELS, 2, ACT, PACK>(a, dx, s);
+}
 template <typename T, bool LABELS, int ACT>
 void sized(const RowsArgs& a, const CUtensorMap& dx, cudaStream_t s) {
-    if (a.v <= 64)
-        run<T, LABELS, 1, ACT>(a, dx, s);
-    else
-        run<T, LABELS, 2, ACT>(a, dx, s);
+    if constexpr (sizeof(T) == 4) {
+        if (a.d <= 32) return wide<T, LABELS, ACT, true>(a, dx, s);
+    }
+    wide<T, LABELS, ACT, false>(a, dx, s);
 }
 
 template <typename T>
