@@ -23,8 +23,8 @@
 // Warp 0 issues the products, warps 8-15 make g (two warps per 32 rows share a
 // row's columns), warps 4-7 load and split x for the next tile and then write dx
 // of this one; dw has two accumulators so that one can be drained meanwhile.
-// With three parts there is room for one tile at a time only, so its steps follow
-// one another; what bounds the kernel is that chain.
+// What bounds the kernel is the chain of a tile's steps: x into place, s, g, dw and
+// dx, of which those that shared memory has two buffers for overlap.
 #include <cstddef>
 
 #include "ops_load.cuh"
@@ -67,7 +67,7 @@ constexpr int kDrain = 4;  // tiles that dw stays in TMEM
 constexpr int kSmall = 64 * 128;  // bytes of 64 lines
 
 struct Smem {
-    uint64_t x_full, x_free, s_full, g_full[2], g_free[2], done, out_empty, drain, pair[4];
+    uint64_t x_full[2], x_free[2], s_full, g_full[2], g_free[2], done, out_empty, drain, pair[4];
     alignas(16) float2 half[2][2][kBM];  // by tile parity and half: a row's largest logit and sum
     float sums[8][128];
     double loss[8][2];
@@ -184,15 +184,17 @@ __device__ __forceinline__ void accumulators(uint32_t d, uint32_t corr, float (&
     }
 }
 
-// Shared memory: the parts of x, w and g, g twice where that fits, and dx's boxes.
+// Shared memory: the parts of x, w and g, x and then g twice where that fits, and
+// dx's boxes.
 template <typename T, int VG, bool PACK>
 struct Layout {
     static constexpr int P = planes<T>(), kXBlock = kBM * 128, kWBlock = VG * kSmall, kGPlane = VG * kBM * 128;
     static constexpr int blocks = PACK ? 2 : P;  // of x and of w
-    static constexpr int fixed = blocks * (kXBlock + kWBlock) + 4 * kBoxBytes + 1024,
-                         most = 227 * 1024 - sizeof(Smem) - 1024;
-    static constexpr int buffers = fixed + 2 * P * kGPlane <= most ? 2 : 1;
-    static constexpr int bytes = fixed + buffers * P * kGPlane;
+    static constexpr int most = 227 * 1024 - sizeof(Smem) - 1024, w = blocks * kWBlock, rest = 4 * kBoxBytes + 1024,
+                         x = blocks * kXBlock, g = P * kGPlane;
+    static constexpr int x_buffers = 2 * x + w + g + rest <= most ? 2 : 1;
+    static constexpr int g_buffers = x_buffers * x + w + 2 * g + rest <= most ? 2 : 1;
+    static constexpr int bytes = x_buffers * x + w + g_buffers * g + rest;
     static_assert(bytes <= most, "shared memory of a block");
     // where part q begins in blocks of `block` bytes
     __device__ static constexpr int part(int q, int block) { return PACK ? (q >> 1) * block + (q & 1) * 64 : q * block; }
@@ -229,7 +231,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     constexpr int P = planes<T>();
     using L = Layout<T, VG, PACK>;
     constexpr int kXBlock = L::kXBlock, kWBlock = L::kWBlock, kGPlane = L::kGPlane, kGGroup = kBM * 128;
-    constexpr int kBuffers = L::buffers;
+    constexpr int kXBuffers = L::x_buffers, kBuffers = L::g_buffers;
+    // with two buffers of x a tile's s comes before the last tile's dw and dx, so
+    // that its g is made while they run
+    constexpr bool kAhead = LABELS && kXBuffers == 2;
     // TMEM: s (its corrections are added first, while the sums are small), dx and
     // two times dw with their corrections apart (PACK: in the 64 columns after
     // the 32 of the sum)
@@ -239,16 +244,16 @@ __global__ void __launch_bounds__(kThreads, 1)
     __shared__ Smem sm;
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     uint8_t* xs = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(dyn) + 1023) & ~(uintptr_t)1023);
-    uint8_t* ws = xs + L::blocks * kXBlock;
+    uint8_t* ws = xs + kXBuffers * L::x;
     uint8_t* g0 = ws + L::blocks * kWBlock;
     uint8_t* boxes = g0 + kBuffers * P * kGPlane;
     const int64_t tiles = (p.m + kBM - 1) / kBM;
 
     if (threadIdx.x == 0) {
-        mbar_init(smem_u32(&sm.x_full), 4);
         mbar_init(smem_u32(&sm.s_full), 1);
-        mbar_init(smem_u32(&sm.x_free), 1);
         for (int q = 0; q < 2; ++q) {
+            mbar_init(smem_u32(&sm.x_full[q]), 4);
+            mbar_init(smem_u32(&sm.x_free[q]), 1);
             mbar_init(smem_u32(&sm.g_full[q]), 8);
             mbar_init(smem_u32(&sm.g_free[q]), 1);
         }
@@ -265,69 +270,154 @@ __global__ void __launch_bounds__(kThreads, 1)
     tc_fence_after();
     const uint32_t tmem = sm.tmem;
     volatile int* gave_up = &sm.gave_up;
-    uint32_t phase = 0;  // of this block's current tile, for every barrier
+    uint32_t phase = 0;  // of this block's current tile, for the barriers with one buffer
+    const int count_all = (int)((tiles - blockIdx.x + gridDim.x - 1) / gridDim.x);
+
+    // dx of tile count - 1 out of TMEM, whose products are done, and dw after
+    // every kDrain tiles: by the loaders between two tiles, or for a layer, whose
+    // g takes less time, by the first four of the warps that make it.
+    const int quarter = warp % 4;
+    const uint32_t d = tmem + ((uint32_t)quarter << 21);
+    uint8_t* box = boxes + quarter * kBoxBytes;
+    const float alpha = LABELS ? __ldg(p.alpha) : 1.f;
+    float* mine = p.slab ? p.slab + ((int64_t)blockIdx.x * p.v + quarter * 32 + lane) * slab_ld(p.d) : nullptr;
+    const bool keeps = p.slab && quarter * 32 + lane < p.v;
+    auto write_out = [&](int count) {
+        const int64_t i0 = (blockIdx.x + (int64_t)(count - 1) * gridDim.x) * kBM + quarter * 32;
+        tc_fence_after();
+        if (p.dx && i0 < p.m) {
+            bool zero = false;
+            if (LABELS && i0 + lane < p.m) {
+                const int32_t l = __ldg(p.targets + i0 + lane);
+                zero = l < 0 || l >= p.v;
+            }
+            for (int c = 0; c < p.d; c += 32) {
+                float v[32];
+                accumulators<PACK ? 4 : P>(d + kX + c, d + kX + kCorr + c, v);
+                if (LABELS) {
+#pragma unroll
+                    for (int q = 0; q < 32; ++q) v[q] = zero ? 0.f : v[q] * alpha;
+                }
+                const int first = sizeof(T) == 2 && c ? 4 : 0;
+                const bool send = sizeof(T) == 4 || c + 32 >= p.d;
+                if (p.dx_tma && first == 0) {
+                    if (lane == 0) bulk_wait_read(0);
+                    __syncwarp();
+                }
+                box_write<T>(box, lane, first, v);
+                if (p.dx_tma) {
+                    if (!send) continue;
+                    fence_async();
+                    __syncwarp();
+                    if (lane == 0) {
+                        tma_store(&map_dx, smem_u32(box), first ? 0 : c, (int)i0, 0, false);
+                        bulk_commit();
+                    }
+                } else {
+                    __syncwarp();
+                    box_copy<T, false>(box, first, static_cast<T*>(p.dx), p.lddx, i0, c, p.m, p.d, lane);
+                    __syncwarp();
+                }
+            }
+        }
+        // dx's accumulators are free; dw's other ones too: they were drained
+        // before this step, in program order
+        const bool drains = p.slab && (count % kDrain == 0 || count == count_all);
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&sm.out_empty));
+        if (drains) {
+            const uint32_t dw = d + kW + ((count - 1) / kDrain & 1) * kWNext;
+            for (int c = 0; c < p.d; c += 32) {
+                float v[32];
+                accumulators<PACK ? 4 : P>(dw + c, dw + kCorr + c, v);
+                if (!keeps) continue;
+                // only this thread adds to its row, in this order
+                float* o = mine + c;
+                const int n = ((int)slab_ld(p.d) - c) / 4;
+#pragma unroll
+                for (int q = 0; q < 8; ++q) {
+                    if (q >= n) break;
+                    if (count <= kDrain)
+                        *reinterpret_cast<float4*>(o + 4 * q) =
+                            make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+                    else
+                        asm volatile("red.relaxed.gpu.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(o + 4 * q),
+                                     "f"(v[4 * q]), "f"(v[4 * q + 1]), "f"(v[4 * q + 2]), "f"(v[4 * q + 3])
+                                     : "memory");
+                }
+            }
+            tc_fence_before();
+        }
+    };
 
     if (warp < 4) {
-        bool ok = true;
-        int count = 0;
-        for (int64_t tile = blockIdx.x; warp == 0 && tile < tiles; tile += gridDim.x, ++count, phase ^= 1) {
-            if (!(ok = mbar_wait(smem_u32(&sm.x_full), phase, gave_up))) break;
-            tc_fence_after();
-            const int buffer = count % kBuffers;
-            const uint32_t x = smem_u32(xs), w = smem_u32(ws), g = smem_u32(g0 + buffer * P * kGPlane);
-            if (LABELS) {
-                if (elect_one()) {
-                    const int steps = (p.d + 15) / 16;
-                    for (int k = 0; k < (P > 1 ? 2 : 1) * steps; ++k) {
-                        const int at = (k % steps) * 32;
-                        uint64_t a[P], b[P];
+        const uint32_t w = smem_u32(ws);
+        auto issue_s = [&](int count) {
+            const uint32_t x = smem_u32(xs + count % kXBuffers * L::x);
+            if (elect_one()) {
+                const int steps = (p.d + 15) / 16;
+                const uint64_t da = smem_desc(x, 16), db = smem_desc(w, 16);
+                uint64_t a[P], b[P];
+                for (int turn = P > 1 ? 0 : 1; turn < 2; ++turn) {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        if (k >= steps) break;
 #pragma unroll
                         for (int q = 0; q < P; ++q) {
-                            a[q] = smem_desc(x + L::part(q, kXBlock) + at, 16);
-                            b[q] = smem_desc(w + L::part(q, kWBlock) + at, 16);
+                            a[q] = da + ((L::part(q, kXBlock) + k * 32) >> 4);
+                            b[q] = db + ((L::part(q, kWBlock) + k * 32) >> 4);
                         }
-                        if (P > 1 && k < steps)
+                        if (turn == 0)
                             corrections<P>(tmem + kS, a, b, idesc_s, k == 0);
                         else
-                            tc_mma(tmem + kS, a[0], b[0], idesc_s, k > 0);
+                            tc_mma(tmem + kS, a[0], b[0], idesc_s, P > 1 || k > 0);
                     }
-                    tc_commit(smem_u32(&sm.s_full));
                 }
-                __syncwarp();
+                tc_commit(smem_u32(&sm.s_full));
             }
-            if (!(ok = mbar_wait(smem_u32(&sm.g_full[buffer]), count / kBuffers & 1, gave_up))) break;
-            if (!(ok = mbar_wait(smem_u32(&sm.out_empty), phase ^ 1, gave_up))) break;
-            tc_fence_after();
+            __syncwarp();
+        };
+        auto issue_gradients = [&](int count) {
+            const int buffer = count % kBuffers;
+            const uint32_t x = smem_u32(xs + count % kXBuffers * L::x), g = smem_u32(g0 + buffer * L::g);
             if (elect_one()) {
                 // dw first: x is free for the next tile while dx runs
-                if (p.slab)
+                // (descriptors advance by constants: this one thread's instructions
+                // are what the products wait for when the other warps are busy)
+                uint64_t a[P], b[P];
+                if (p.slab) {
+                    // of a single group the second 64 rows of the result are not read
+                    const uint64_t da = smem_desc(g, kGGroup), db = smem_desc(x, PACK ? kXBlock : 16);
+                    const uint32_t dw = tmem + kW + (count / kDrain & 1) * kWNext;
+                    const bool add = count % kDrain != 0;
+#pragma unroll
                     for (int k = 0; k < kBM / 16; ++k) {
-                        uint64_t a[P], b[P];
 #pragma unroll
                         for (int q = 0; q < P; ++q) {
-                            // of a single group the second 64 rows of the result are not read
-                            a[q] = smem_desc(g + q * kGPlane + k * 2048, kGGroup);
-                            b[q] = smem_desc(x + (PACK ? 0 : q * kXBlock) + k * 2048, PACK ? kXBlock : 16);
+                            a[q] = da + ((q * kGPlane + k * 2048) >> 4);
+                            b[q] = db + (((PACK ? 0 : q * kXBlock) + k * 2048) >> 4);
                         }
-                        const uint32_t dw = tmem + kW + (count / kDrain & 1) * kWNext;
-                        const bool fresh = k == 0 && count % kDrain == 0;
                         if constexpr (PACK) {
-                            tc_mma(dw, a[0], b[0], idesc_w, !fresh);
+                            tc_mma(dw, a[0], b[0], idesc_w, add || k > 0);
                             tc_mma(dw + 32, a[1], b[0], idesc_w - narrower, true);
                             tc_mma(dw + 64, a[2], b[0], idesc_w - 2 * narrower, true);
                         } else {
-                            corrections<P>(dw + kCorr, a, b, idesc_w, fresh);
-                            tc_mma(dw, a[0], b[0], idesc_w, !fresh);
+                            corrections<P>(dw + kCorr, a, b, idesc_w, !add && k == 0);
+                            tc_mma(dw, a[0], b[0], idesc_w, add || k > 0);
                         }
                     }
-                tc_commit(smem_u32(&sm.x_free));
-                if (p.dx)
-                    for (int k = 0; k * 16 < p.v; ++k) {
-                        uint64_t a[P], b[P];
+                }
+                tc_commit(smem_u32(&sm.x_free[count % kXBuffers]));
+                if (p.dx) {
+                    const uint64_t da = smem_desc(g, 16), db = smem_desc(w, PACK ? kWBlock : 16);
+#pragma unroll
+                    for (int k = 0; k < 4 * VG; ++k) {
+                        if (k * 16 >= p.v) break;
 #pragma unroll
                         for (int q = 0; q < P; ++q) {
-                            a[q] = smem_desc(g + q * kGPlane + k / 4 * kGGroup + k % 4 * 32, 16);
-                            b[q] = smem_desc(w + (PACK ? 0 : q * kWBlock) + k * 2048, PACK ? kWBlock : 16);
+                            a[q] = da + ((q * kGPlane + k / 4 * kGGroup + k % 4 * 32) >> 4);
+                            b[q] = db + (((PACK ? 0 : q * kWBlock) + k * 2048) >> 4);
                         }
                         if constexpr (PACK) {
                             tc_mma(tmem + kX, a[0], b[0], idesc_x, k > 0);
@@ -338,10 +428,35 @@ __global__ void __launch_bounds__(kThreads, 1)
                             tc_mma(tmem + kX, a[0], b[0], idesc_x, k > 0);
                         }
                     }
+                }
                 tc_commit(smem_u32(&sm.g_free[buffer]));
                 tc_commit(smem_u32(&sm.done));
             }
             __syncwarp();
+        };
+        bool ok = true;
+        for (int count = 0; warp == 0 && count < count_all; ++count, phase ^= 1) {
+            if (!(ok = mbar_wait(smem_u32(&sm.x_full[count % kXBuffers]), count / kXBuffers & 1, gave_up))) break;
+            tc_fence_after();
+            if (LABELS) issue_s(count);
+            if (kAhead && count > 0) {
+                if (!(ok = mbar_wait(smem_u32(&sm.out_empty), phase, gave_up))) break;
+                tc_fence_after();
+                issue_gradients(count - 1);
+            }
+            if (!(ok = mbar_wait(smem_u32(&sm.g_full[count % kBuffers]), count / kBuffers & 1, gave_up))) break;
+            tc_fence_after();
+            if (!kAhead) {
+                if (!(ok = mbar_wait(smem_u32(&sm.out_empty), phase ^ 1, gave_up))) break;
+                tc_fence_after();
+                issue_gradients(count);
+            }
+        }
+        if (kAhead && ok && warp == 0) {
+            if ((ok = mbar_wait(smem_u32(&sm.out_empty), phase, gave_up))) {
+                tc_fence_after();
+                issue_gradients(count_all - 1);
+            }
         }
         if (!ok && warp == 0) {
             if (elect_one()) {
@@ -363,102 +478,39 @@ __global__ void __launch_bounds__(kThreads, 1)
                 store_parts<T, PACK>(c[e], ws + q * kSmall, line, t % 8, kWBlock);
             }
         }
-        const int quarter = warp % 4;
-        const uint32_t d = tmem + ((uint32_t)quarter << 21);
-        uint8_t* box = boxes + quarter * kBoxBytes;
-        const float alpha = LABELS ? __ldg(p.alpha) : 1.f;
-        float* mine = p.slab ? p.slab + ((int64_t)blockIdx.x * p.v + quarter * 32 + lane) * slab_ld(p.d) : nullptr;
-        const bool keeps = p.slab && quarter * 32 + lane < p.v;
-        const int count_all = (int)((tiles - blockIdx.x + gridDim.x - 1) / gridDim.x);
-        // step `count`: x of tile `count` goes in and dx of the one before comes out
-        for (int count = 0; count <= count_all; ++count, phase ^= 1) {
+        // x of a tile into its buffer
+        auto bring = [&](int count) {
             const int64_t tile = blockIdx.x + (int64_t)count * gridDim.x;
-            if (count < count_all) {
-                Chunk<T> c[8];
-                load_rows<T, 128>(ox, tile * kBM, 0, t, c, LABELS ? p.targets : nullptr, p.v);
-                if (!mbar_wait(smem_u32(&sm.x_free), phase ^ 1, gave_up)) break;
+            Chunk<T> c[8];
+            load_rows<T, 128>(ox, tile * kBM, 0, t, c, LABELS ? p.targets : nullptr, p.v);
+            const int buffer = count % kXBuffers;
+            if (!mbar_wait(smem_u32(&sm.x_free[buffer]), (count / kXBuffers & 1) ^ 1, gave_up)) return false;
 #pragma unroll
-                for (int q = 0; q < 8; ++q) store_parts<T, PACK>(c[q], xs, t / 8 + 16 * q, t % 8, kXBlock);
-                fence_async();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(smem_u32(&sm.x_full));
-                // the next tile's rows start towards L2 while dx of the last is written
-                const int64_t ahead = (tile + gridDim.x) * kBM + t;
-                if (ahead < p.m)
-                    for (int c = 0; c < p.d; c += 128 / (int)sizeof(T))
-                        asm volatile("prefetch.global.L2 [%0];" ::"l"(ox.p + ahead * p.ldx + c));
-            }
-            if (count == 0) continue;
-            if (!mbar_wait(smem_u32(&sm.done), phase ^ 1, gave_up)) break;
-            const int64_t i0 = (tile - gridDim.x) * kBM + quarter * 32;
-            tc_fence_after();
-            if (p.dx && i0 < p.m) {
-                bool zero = false;
-                if (LABELS && i0 + lane < p.m) {
-                    const int32_t l = __ldg(p.targets + i0 + lane);
-                    zero = l < 0 || l >= p.v;
-                }
-                for (int c = 0; c < p.d; c += 32) {
-                    float v[32];
-                    accumulators<PACK ? 4 : P>(d + kX + c, d + kX + kCorr + c, v);
-                    if (LABELS) {
-#pragma unroll
-                        for (int q = 0; q < 32; ++q) v[q] = zero ? 0.f : v[q] * alpha;
-                    }
-                    const int first = sizeof(T) == 2 && c ? 4 : 0;
-                    const bool send = sizeof(T) == 4 || c + 32 >= p.d;
-                    if (p.dx_tma && first == 0) {
-                        if (lane == 0) bulk_wait_read(0);
-                        __syncwarp();
-                    }
-                    box_write<T>(box, lane, first, v);
-                    if (p.dx_tma) {
-                        if (!send) continue;
-                        fence_async();
-                        __syncwarp();
-                        if (lane == 0) {
-                            tma_store(&map_dx, smem_u32(box), first ? 0 : c, (int)i0, 0, false);
-                            bulk_commit();
-                        }
-                    } else {
-                        __syncwarp();
-                        box_copy<T, false>(box, first, static_cast<T*>(p.dx), p.lddx, i0, c, p.m, p.d, lane);
-                        __syncwarp();
-                    }
-                }
-            }
-            // dx's accumulators are free; dw's other ones too: they were drained
-            // before this step, in program order
-            const bool drains = p.slab && (count % kDrain == 0 || count == count_all);
-            tc_fence_before();
+            for (int q = 0; q < 8; ++q) store_parts<T, PACK>(c[q], xs + buffer * L::x, t / 8 + 16 * q, t % 8, kXBlock);
+            fence_async();
             __syncwarp();
-            if (lane == 0) mbar_arrive(smem_u32(&sm.out_empty));
-            if (drains) {
-                const uint32_t dw = d + kW + ((count - 1) / kDrain & 1) * kWNext;
-                for (int c = 0; c < p.d; c += 32) {
-                    float v[32];
-                    accumulators<PACK ? 4 : P>(dw + c, dw + kCorr + c, v);
-                    if (!keeps) continue;
-                    float4* o = reinterpret_cast<float4*>(mine + c);
-                    const int n = ((int)slab_ld(p.d) - c) / 4;
-#pragma unroll
-                    for (int q = 0; q < 8; ++q) {
-                        if (q >= n) break;
-                        float4 f = count <= kDrain ? make_float4(0.f, 0.f, 0.f, 0.f) : o[q];
-                        f.x += v[4 * q];
-                        f.y += v[4 * q + 1];
-                        f.z += v[4 * q + 2];
-                        f.w += v[4 * q + 3];
-                        o[q] = f;
-                    }
-                }
-                tc_fence_before();
-            }
+            if (lane == 0) mbar_arrive(smem_u32(&sm.x_full[buffer]));
+            // the next tile's rows start towards L2
+            const int64_t ahead = (tile + gridDim.x) * kBM + t;
+            if (ahead < p.m)
+                for (int e = 0; e < p.d; e += 128 / (int)sizeof(T))
+                    asm volatile("prefetch.global.L2 [%0];" ::"l"(ox.p + ahead * p.ldx + e));
+            return true;
+        };
+        // step `count`: x goes in as far ahead as there are buffers, dx of the
+        // tile before comes out
+        bool ok = kXBuffers == 1 || bring(0);
+        for (int count = 0; ok && count <= count_all; ++count, phase ^= 1) {
+            const int64_t tile = blockIdx.x + (int64_t)count * gridDim.x;
+            if (count + kXBuffers - 1 < count_all && !bring(count + kXBuffers - 1)) break;
+            if (!LABELS || count == 0) continue;
+            if (!mbar_wait(smem_u32(&sm.done), phase ^ 1, gave_up)) break;
+            write_out(count);
         }
         if (lane == 0) bulk_wait_all();
     } else {
         if constexpr (LABELS) {
-            const int quarter = warp % 4, half = (warp - 8) / 4, line = quarter * 32 + lane;
+            const int half = (warp - 8) / 4, line = quarter * 32 + lane;
             const uint32_t s = tmem + ((uint32_t)quarter << 21) + half * 32 * VG;
             double sum = 0, count = 0;
             int turn = 0;
@@ -595,7 +647,21 @@ __global__ void __launch_bounds__(kThreads, 1)
                 fence_async();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(smem_u32(&sm.g_full[buffer]));
+                // the next tile's rows start towards L2, two threads a row
+                const int64_t ahead = (tile + gridDim.x) * kBM + t / 2;
+                if (ahead < p.m)
+                    for (int e = t % 2 * (128 / (int)sizeof(T)); e < p.v; e += 256 / (int)sizeof(T)) {
+                        asm volatile("prefetch.global.L2 [%0];" ::"l"(oy.p + ahead * p.lddy + e));
+                        if (ACT != MSPLAT_ACT_NONE)
+                            asm volatile("prefetch.global.L2 [%0];" ::"l"(oz.p + ahead * p.ldz + e));
+                    }
+                if (warp < 12 && turn > 0) {
+                    if (!(ok = mbar_wait(smem_u32(&sm.done), (turn & 1) ^ 1, gave_up))) break;
+                    write_out(turn);
+                }
             }
+            if (warp < 12 && ok && mbar_wait(smem_u32(&sm.done), (count_all & 1) ^ 1, gave_up)) write_out(count_all);
+            if (lane == 0) bulk_wait_all();
 #pragma unroll
             for (int c = 0; c < VG; ++c)
 #pragma unroll
