@@ -189,6 +189,9 @@ int64_t stats_blocks_tc16(const Product& p);
 void launch_product_tc16(const Product& p, cudaStream_t s);
 bool gave_up_tc16(cudaStream_t s);
 void launch_product_tcv(const Product& p, cudaStream_t s);
+// layers of a few rows (ops_gemv.cu)
+bool can_product_gemv(const Product& p);
+void launch_product_gemv(const Product& p, cudaStream_t s);
 // layers with few outputs and many rows (ops_few.cu)
 bool can_product_few(const Product& p);
 void launch_product_few(const Product& p, cudaStream_t s);

@@ -9,8 +9,7 @@
 // take neighbouring pieces. (Each thread reading its own row touches 32 lines
 // per instruction.) 1M x 61 -> 3 f16 of an unaligned record takes 53 us, 2.5 TB/s;
 // what bounds it is issuing the conversions and the masks of a row's two ends.
-// The weights are
-// in shared memory as float, read as broadcasts.
+// The weights are in shared memory as float, read as broadcasts.
 #include "ops.cuh"
 
 namespace msplat {

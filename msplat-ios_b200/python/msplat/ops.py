@@ -179,7 +179,7 @@ def linear_forward(x, w, bias=None, activation="none", residual=None, preact=Non
     act = _act(activation)
     with _On(device, stream) as on:
         if out is None:
-            out = torch.empty((m, n), dtype=out_dtype, device=device)
+            out = x.new_empty((m, n)) if out_dtype == x.dtype else x.new_empty((m, n), dtype=out_dtype)
         py, ldy = _matrix(out, "out", device, out_dtype, m, n)
         _check(L.msplat_linear_forward(m, n, k, px, ldx, pw, ldw, pb, act, pr, ldr, pz, ldz, py, ldy, dt,
                                        _DTYPES[out_dtype], on.handle))
@@ -203,7 +203,7 @@ def linear_backward(x, w, dy, preact=None, activation="none", need_dx=True, need
         _refuse("preact is needed for this activation")
     pz, ldz = _matrix(preact, "preact", device, x.dtype, m, n) if act else (None, 0)
     with _On(device, stream) as on:
-        new = lambda *shape: torch.empty(shape, dtype=x.dtype, device=device)  # noqa: E731
+        new = lambda *shape: x.new_empty(shape)  # noqa: E731
         dx = new(m, k) if need_dx else None
         dw = new(n, k) if need_dw else None
         dbias = new(n) if need_dbias else None
@@ -232,7 +232,7 @@ def dropout(x, p, seed, offset=0, residual=None, out=None, offset_dev=None, stre
     po = _vector(offset_dev, "offset_dev", device, torch.int64, 1)
     with _On(device, stream) as on:
         if out is None:
-            out = torch.empty((m, n), dtype=x.dtype, device=device)
+            out = x.new_empty((m, n))
         py, ldy = _matrix(out, "out", device, x.dtype, m, n)
         _check(L.msplat_dropout(m, n, px, ldx, pr, ldr, py, ldy, p, seed, offset, po, dt, on.handle))
     return out
