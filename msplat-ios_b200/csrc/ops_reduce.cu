@@ -143,11 +143,20 @@ __global__ void __launch_bounds__(1024) k_join(JoinArgs a, int shares) {
         // only) has no reference; a sum of NaN counts
         float top = -INFINITY, total = 0.f;
         if (i < a.m)
-            for (int64_t b = share; b < a.blocks; b += shares) {
-                const float2 v = __ldcs(a.stats + b * a.stats_ld + i);
-                if (v.y == 0.f) continue;
-                const float t = fmaxf(top, v.x);
-                total = (total == 0.f ? 0.f : total * exp2f(top - t)) + v.y * exp2f(v.x - t);
+            for (int64_t b = share; b < a.blocks; b += 8 * shares) {
+                float2 v[8];  // eight reads in flight
+#pragma unroll
+                for (int q = 0; q < 8; ++q)
+                    v[q] = b + q * shares < a.blocks ? __ldcs(a.stats + (b + q * shares) * a.stats_ld + i)
+                                                     : make_float2(0.f, 0.f);
+                float t = top;
+#pragma unroll
+                for (int q = 0; q < 8; ++q)
+                    if (v[q].y != 0.f) t = fmaxf(t, v[q].x);
+                total = total == 0.f ? 0.f : total * exp2f(top - t);
+#pragma unroll
+                for (int q = 0; q < 8; ++q)
+                    if (v[q].y != 0.f) total += v[q].y * exp2f(v[q].x - t);
                 top = t;
             }
         tops[warp][lane] = top;

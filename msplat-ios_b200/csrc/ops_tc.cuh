@@ -468,8 +468,10 @@ __device__ __forceinline__ bool columns32(const Product& p, const Tiles& tl, con
 #pragma unroll
             for (int q = 0; q < 32; ++q) v[q] = q < n ? v[q] : -INFINITY;
         }
+        float tops[4] = {top, v[1], v[2], v[3]};
 #pragma unroll
-        for (int q = 0; q < 32; ++q) top = fmaxf(top, v[q]);
+        for (int q = 0; q < 32; ++q) tops[q % 4] = fmaxf(tops[q % 4], v[q]);
+        top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
         const int64_t at = r.target - p.col0 - j0;
         if (__any_sync(~0u, r.in && at >= 0 && at < 32)) {
 #pragma unroll
