@@ -19,9 +19,14 @@
  * call unless its comment says otherwise. Sums, softmax statistics and
  * activations are evaluated in 32 bits (matrix products of MSPLAT_DTYPE_F32
  * keep all 24 bits of both factors) and rounded once into the output's type.
+ * A factor of MSPLAT_DTYPE_F32 above 3.38e38 in size counts as infinite, and an
+ * infinite one may give NaN where the formula gives an infinity; factors below
+ * 1e-30 may lose their lowest bits. Whatever lies in the other columns of a
+ * wider record is neither used nor written, but 16-byte pieces of it between the
+ * first and the last element of a matrix may be read.
  *
  * Calls are asynchronous on `stream`, allocate nothing, keep nothing between
- * calls and may be captured into a CUDA graph. Working memory comes from the
+ * calls and may be captured into a CUDA graph. Sizes are at most 2^30. Working memory comes from the
  * caller: *_workspace gives its size in bytes, the pointer must be 256-byte
  * aligned, and two calls that may run at the same time (on two streams, or in
  * two graphs) need two of them. Results do not depend on the order in which
@@ -56,7 +61,7 @@ enum {
  * preact [m,n] when that is not NULL (msplat_linear_backward reads it).
  * residual, preact and y have the type y_dtype: dtype, or MSPLAT_DTYPE_F32.
  * residual may be the same memory as y (then ldr == ldy). m may be 0; n and k
- * are at least 1, and m, n, k at most 2^31 - 1. Needs no workspace. */
+ * are at least 1, and m, n, k at most 2^30. Needs no workspace. */
 int msplat_linear_forward(int64_t m, int64_t n, int64_t k, const void* x, int64_t ldx, const void* w, int64_t ldw,
                           const void* bias, int32_t activation, const void* residual, int64_t ldr, void* preact,
                           int64_t ldz, void* y, int64_t ldy, int32_t dtype, int32_t y_dtype, void* stream);
@@ -105,7 +110,7 @@ int msplat_dropout(int64_t rows, int64_t cols, const void* x, int64_t ldx, const
  * NULL; what is given is overwritten. The 16-bit types round the softmax
  * minus the one-hot to dtype between the products (MSPLAT_DTYPE_F16 times
  * 2^14, so that small probabilities keep their bits). m may be 0; v and d are
- * at least 1, and m, v, d at most 2^31 - 1. logit_scale and weight are
+ * at least 1, and m, v, d at most 2^30. logit_scale and weight are
  * finite. */
 int msplat_loss_cross_entropy_workspace(int64_t m, int64_t v, int64_t d, int32_t grad, int32_t dtype,
                                         uint64_t* bytes);

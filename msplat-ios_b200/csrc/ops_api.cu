@@ -29,8 +29,9 @@ void require(bool ok, const char* what) {
 }
 
 void check_size(int64_t v, int64_t least, const char* name) {
-    if (v < least || v > 0x7fffffff)
-        throw Error(MSPLAT_ERR_ARGUMENT, std::string(name) + " must be in [" + std::to_string(least) + ", 2^31 - 1]");
+    // tile and element coordinates stay below 2^31 with a tile's overhang
+    if (v < least || v > (1 << 30))
+        throw Error(MSPLAT_ERR_ARGUMENT, std::string(name) + " must be in [" + std::to_string(least) + ", 2^30]");
 }
 
 void check_dtype(int dtype) {

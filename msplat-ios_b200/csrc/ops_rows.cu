@@ -471,7 +471,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int t = threadIdx.x - 128;
         const Operand<T> ox = operand<T>(p.x, p.ldx, p.m, p.d, false, p.vec_x);
         const Operand<T> ow = operand<T>(p.w, p.ldw, p.v, p.d, false, p.vec_w);
-        for (int q = 0; q < VG; ++q) {
+        // a layer's x is read for dw only, its w for dx only (either may be null)
+        const bool reads_x = LABELS || p.slab, reads_w = LABELS || p.dx;
+        for (int q = 0; reads_w && q < VG; ++q) {
             Chunk<T> c[4];
             load_tile<T, 64, 128>(ow, 64 * q, 0, t, c);
 #pragma unroll
@@ -484,17 +486,20 @@ __global__ void __launch_bounds__(kThreads, 1)
         auto bring = [&](int count) {
             const int64_t tile = blockIdx.x + (int64_t)count * gridDim.x;
             Chunk<T> c[8];
-            load_rows<T, 128>(ox, tile * kBM, 0, t, c, LABELS ? p.targets : nullptr, p.v);
+            if (reads_x) load_rows<T, 128>(ox, tile * kBM, 0, t, c, LABELS ? p.targets : nullptr, p.v);
             const int buffer = count % kXBuffers;
             if (!mbar_wait(smem_u32(&sm.x_free[buffer]), (count / kXBuffers & 1) ^ 1, gave_up)) return false;
+            if (reads_x) {
 #pragma unroll
-            for (int q = 0; q < 8; ++q) store_parts<T, PACK>(c[q], xs + buffer * L::x, t / 8 + 16 * q, t % 8, kXBlock);
+                for (int q = 0; q < 8; ++q)
+                    store_parts<T, PACK>(c[q], xs + buffer * L::x, t / 8 + 16 * q, t % 8, kXBlock);
+            }
             fence_async();
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&sm.x_full[buffer]));
             // the next tile's rows start towards L2
             const int64_t ahead = (tile + gridDim.x) * kBM + t;
-            if (ahead < p.m)
+            if (reads_x && ahead < p.m)
                 for (int e = 0; e < p.d; e += 128 / (int)sizeof(T))
                     asm volatile("prefetch.global.L2 [%0];" ::"l"(ox.p + ahead * p.ldx + e));
             return true;

@@ -97,6 +97,12 @@ def _dtype(x):
     return code
 
 
+def _rows(w, name):
+    if not isinstance(w, torch.Tensor) or w.dim() != 2:
+        _refuse(f"{name} must be a matrix")
+    return w.shape[0]
+
+
 def _act(name):
     code = ACTIVATIONS.get(name)
     return code if code is not None else _refuse(f"unknown activation {name!r}")
@@ -166,7 +172,7 @@ def linear_forward(x, w, bias=None, activation="none", residual=None, preact=Non
     L = _lib()
     dt = _dtype(x)
     device, (m, k) = x.device, x.shape if x.dim() == 2 else _refuse("x must be a matrix")
-    n = w.shape[0]
+    n = _rows(w, "w")
     if out_dtype is None:
         out_dtype = x.dtype if out is None else out.dtype
     if out_dtype != x.dtype and out_dtype != torch.float32:
@@ -194,7 +200,7 @@ def linear_backward(x, w, dy, preact=None, activation="none", need_dx=True, need
     L = _lib()
     dt = _dtype(x)
     device, (m, k) = x.device, x.shape if x.dim() == 2 else _refuse("x must be a matrix")
-    n = w.shape[0]
+    n = _rows(w, "w")
     px, ldx = _matrix(x, "x", device, x.dtype)
     pw, ldw = _matrix(w, "w", device, x.dtype, n, k)
     pdy, lddy = _matrix(dy, "dy", device, x.dtype, m, n)
@@ -248,7 +254,7 @@ def loss_cross_entropy(x, w, targets, logit_scale=1.0, weight=1.0, grad=True, st
     L = _lib()
     dt = _dtype(x)
     device, (m, d) = x.device, x.shape if x.dim() == 2 else _refuse("x must be a matrix")
-    v = w.shape[0]
+    v = _rows(w, "w")
     px, ldx = _matrix(x, "x", device, x.dtype)
     pw, ldw = _matrix(w, "w", device, x.dtype, v, d)
     pt = _vector(targets, "targets", device, torch.int32, m)

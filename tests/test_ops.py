@@ -514,3 +514,93 @@ def test_linear_backward_narrow(m, n, k, pad, lead, t):
         part = ops().linear_backward(x, w, dy, preact=z, activation=act, need_dx=need[0], need_dw=need[1], need_dbias=need[2])
         for a, b in zip(full, part):
             assert b is None or torch.equal(a, b)
+
+
+# ---- the C entry points' own freedoms ------------------------------------------------------------------------------------
+
+
+def workspace(size_fn, *args):
+    import ctypes as C
+    size = C.c_uint64()
+    assert size_fn(*args, C.byref(size)) == 0
+    return torch.empty(size.value + 1, dtype=torch.uint8, device="cuda"), size.value
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("m,n,k", [(300, 200, 96), (9000, 40, 24), (9000, 100, 50), (8192, 3, 32)])
+def test_backward_c_entry(m, n, k, t):
+    """Gradients into views of wider records; x null without dw, w null without dx; nothing beside the views is written."""
+    L, code = ops()._lib(), {"f32": 0, "f16": 4, "bf16": 5}[t]
+    x, w = normal(120, m, k, t), normal(121, n, k, t, std=k ** -0.5)
+    z, dy = normal(122, m, n, t), normal(123, m, n, t)
+    want = R.linear_grads(x, w, dy, z, "gelu", R.TYPES[t])
+    ws, size = workspace(L.msplat_linear_backward_workspace, m, n, k, 2, code)
+    stream = torch.cuda.current_stream().cuda_stream
+    for pad in (3, 8):
+        dx, dx_clean = guarded(m, k, R.TYPES[t], pad=pad)
+        dw, dw_clean = guarded(n, k, R.TYPES[t], pad=pad)
+        db = torch.empty(n, dtype=R.TYPES[t], device="cuda")
+        for has_dx, has_dw in ((1, 1), (1, 0), (0, 1), (0, 0)):
+            dx.zero_(), dw.zero_(), db.zero_()
+            assert L.msplat_linear_backward(
+                m, n, k, x.data_ptr() if has_dw else None, k, w.data_ptr() if has_dx else None, k, z.data_ptr(), n, 2,
+                dy.data_ptr(), n, dx.data_ptr() if has_dx else None, dx.stride(0), dw.data_ptr() if has_dw else None,
+                dw.stride(0), db.data_ptr(), code, ws.data_ptr(), size, stream) == 0, L.msplat_last_error()
+            if has_dx:
+                R.check(dx, *want[0], "dx")
+            if has_dw:
+                R.check(dw, *want[1], "dw")
+            R.check(db, *want[2], "dbias")
+            assert dx_clean() and dw_clean() and bool(dx.any()) == bool(has_dx) and bool(dw.any()) == bool(has_dw)
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("m,v,d", [(300, 200, 96), (9000, 40, 24), (9000, 100, 50)])
+def test_loss_c_entry(m, v, d, t):
+    """Every output alone, in views of wider records, with a workspace for exactly what is asked."""
+    L, code = ops()._lib(), {"f32": 0, "f16": 4, "bf16": 5}[t]
+    x, w, targets = normal(124, m, d, t), normal(125, v, d, t, std=d ** -0.5), labels(126, m, v)
+    want = R.loss(x, w, targets, 1.0, 50.0, R.TYPES[t])
+    stream = torch.cuda.current_stream().cuda_stream
+    for pad in (3, 8):
+        for asked in ("loss", "row_loss", "dx", "dw"):
+            ws, size = workspace(L.msplat_loss_cross_entropy_workspace, m, v, d, asked in ("dx", "dw"), code)
+            out, clean = {"loss": (torch.empty((), device="cuda"), None), "row_loss": (torch.empty(m, device="cuda"), None),
+                          "dx": guarded(m, d, R.TYPES[t], pad=pad), "dw": guarded(v, d, R.TYPES[t], pad=pad)}[asked]
+            at = {name: out.data_ptr() if name == asked else None for name in ("loss", "row_loss", "dx", "dw")}
+            assert L.msplat_loss_cross_entropy(m, v, d, x.data_ptr(), d, w.data_ptr(), d, targets.data_ptr(), 1.0, 50.0,
+                                               at["loss"], at["row_loss"], at["dx"], d + 2 * pad, at["dw"], d + 2 * pad, code,
+                                               ws.data_ptr(), size, stream) == 0, L.msplat_last_error()
+            R.check(out, *want[asked], asked)
+            assert clean is None or clean()
+
+
+def test_status():
+    x, w = normal(127, 300, 64, "bf16"), normal(128, 64, 64, "bf16")
+    ops().linear_forward(x, w)
+    ops().status()
+
+
+def test_two_threads():
+    """The same call from two host threads at once, each on its stream."""
+    import threading
+    x, w, targets = normal(129, 9000, 48, "f32"), normal(130, 90, 48, "f32"), labels(131, 9000, 90)
+    want = ops().loss_cross_entropy(x, w, targets)
+    torch.cuda.synchronize()
+    got, fail = {}, []
+
+    def work(k):
+        try:
+            s = torch.cuda.Stream()
+            for _ in range(5):
+                got[k] = ops().loss_cross_entropy(x, w, targets, stream=s)
+            s.synchronize()
+        except Exception as e:  # noqa: BLE001
+            fail.append(e)
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(2)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    assert not fail
+    for r in got.values():
+        for a, b in zip(want, r):
+            assert torch.equal(a, b)
