@@ -238,7 +238,8 @@ struct JoinArgs {
 int join_blocks(int64_t m);
 // The rows of x with a label, zeros in place of the others: what the products
 // read, so that an unlabelled row's NaN or infinity reaches nothing (in dw even
-// a zero gradient times it would).
+// a zero gradient times it would). Without targets, all of x (into rows that
+// TMA can address).
 void launch_labelled_rows(int64_t m, int64_t d, const void* x, int64_t ldx, const int32_t* targets, int64_t labels,
                           void* out, int64_t ldo, int dtype, cudaStream_t s);
 void launch_join(const JoinArgs& a, cudaStream_t s);

@@ -149,7 +149,9 @@ struct LossPlan {
     float *lse, *label_logit, *alpha;
     double* partial;
     float2* stats;
-    char *x = nullptr, *g = nullptr;  // x's labelled rows; a piece of the softmax gradient
+    // x's labelled rows and, when rows of d 16-bit elements are no multiple of 16
+    // bytes, w, with rows of ldx elements; a piece of the softmax gradient
+    char *x = nullptr, *w = nullptr, *g = nullptr;
     int64_t ldx;
     float *slab_x = nullptr, *slab_w = nullptr;
     bool rows;                         // in one pass over the rows
@@ -169,10 +171,12 @@ struct LossPlan {
         label_logit = a.take<float>(m);
         partial = a.take<double>(2 * ceil_div(m, stats_rows) * join_blocks(stats_rows));
         stats = a.take<float2>(blocks * stats_rows);
-        if (!grad) return;
         const int es = dtype_size(dtype);
         ldx = round_up(d, 16 / es);
-        x = a.take<char>(m * ldx * es);
+        const bool odd = es == 2 && ldx != d;
+        if (grad || odd) x = a.take<char>(m * ldx * es);
+        if (odd) w = a.take<char>(v * ldx * es);
+        if (!grad) return;
         by_rows = m >= v;
         const int64_t other = round_up(by_rows ? v : m, 16 / es), all = by_rows ? m : v;
         chunk = std::min(all, round_up(std::max<int64_t>(kPieceBytes / (other * es), 1), 128));
@@ -438,10 +442,15 @@ int msplat_loss_cross_entropy(int64_t m, int64_t v, int64_t d, const void* x, in
         logits.logit_scale = logit_scale;
         logits.g_scale = g_scale;
 
-        if (grad) {
+        if (plan.x) {
             launch_labelled_rows(m, d, x, ldx, targets, v, plan.x, plan.ldx, dtype, s);
             logits.A = x = plan.x;
             logits.lda = ldx = plan.ldx;
+        }
+        if (plan.w && !can_product_tc16(logits)) {
+            launch_labelled_rows(v, d, w, ldw, nullptr, 0, plan.w, plan.ldx, dtype, s);
+            logits.B = w = plan.w;
+            logits.ldb = ldw = plan.ldx;
         }
         int joined = 0;
         for (int64_t r0 = 0; r0 < m; r0 += plan.stats_rows) {

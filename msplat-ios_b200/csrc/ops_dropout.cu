@@ -40,7 +40,8 @@ struct DropArgs {
 
 // One thread per block of eight elements of the row-major order. FLAT: the
 // matrices are contiguous and 16-byte aligned, so a block is one or two
-// 16-byte accesses; otherwise each element finds its row and column.
+// 16-byte accesses; otherwise each element finds its row and column (with a
+// 32-bit division per block where the elements are fewer than 2^32).
 template <typename T, bool FLAT>
 __global__ void __launch_bounds__(256) k_dropout(DropArgs<T> a) {
     const int64_t n = a.rows * a.cols, blocks = (n + 7) / 8;
@@ -71,19 +72,36 @@ __global__ void __launch_bounds__(256) k_dropout(DropArgs<T> a) {
 #pragma unroll
             for (int q = 0; q < (int)sizeof(T) / 2; ++q) reinterpret_cast<uint4*>(a.y + e0)[q] = vx.q[q];
         } else {
-            int64_t row = e0 / a.cols, col = e0 - row * a.cols;
+            int64_t row = n >> 32 ? e0 / a.cols : (int64_t)((uint32_t)e0 / (uint32_t)a.cols), col = e0 - row * a.cols;
+            const T* x = a.x + row * a.ldx + col;
+            const T* res = a.residual + (a.residual ? row * a.ldr + col : 0);
+            T* y = a.y + row * a.ldy + col;
+            T vx[8], vr[8], *to[8];
+            // every load before the first store, so that they overlap
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
+                to[i] = y;
                 if (e0 + i < n) {
-                    const uint32_t draw = (i & 1) ? w[i / 2] >> 16 : w[i / 2] & 0xFFFFu;
-                    float v = draw >= a.below ? to_f32(a.x[row * a.ldx + col]) * a.scale : 0.f;
-                    if (a.residual) v += to_f32(a.residual[row * a.ldr + col]);
-                    a.y[row * a.ldy + col] = from_f32<T>(v);
+                    vx[i] = *x;
+                    if (a.residual) vr[i] = *res;
                 }
+                ++x;
+                ++y;
+                ++res;
                 if (++col == a.cols) {
                     col = 0;
-                    ++row;
+                    x += a.ldx - a.cols;
+                    y += a.ldy - a.cols;
+                    res += a.ldr - a.cols;
                 }
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                if (e0 + i >= n) break;
+                const uint32_t draw = (i & 1) ? w[i / 2] >> 16 : w[i / 2] & 0xFFFFu;
+                float v = draw >= a.below ? to_f32(vx[i]) * a.scale : 0.f;
+                if (a.residual) v += to_f32(vr[i]);
+                *to[i] = from_f32<T>(v);
             }
         }
     }

@@ -248,21 +248,27 @@ __global__ void __launch_bounds__(256) k_loss_total(const double* partial, int b
     }
 }
 
-// One thread per vector of V elements.
+// `lanes` threads (a power of two) share a row, in vectors of V elements.
 template <typename T, int V>
 __global__ void __launch_bounds__(256) k_labelled_rows(int64_t m, int64_t d, const T* x, int64_t ldx,
-                                                       const int32_t* targets, int64_t labels, T* out, int64_t ldo) {
-    const int64_t per = (d + V - 1) / V;
-    for (int64_t e = blockIdx.x * 256ll + threadIdx.x; e < m * per; e += gridDim.x * 256ll) {
-        const int64_t i = e / per, j = (e - i * per) * V;
-        const int32_t t = __ldg(targets + i);
-        const bool has = t >= 0 && t < labels;
-        const T* from = x + i * ldx + j;
-        T* to = out + i * ldo + j;
-        if (V > 1) {
-            *reinterpret_cast<uint4*>(to) = has ? __ldg(reinterpret_cast<const uint4*>(from)) : make_uint4(0, 0, 0, 0);
-        } else {
-            *to = has ? *from : from_f32<T>(0.f);
+                                                       const int32_t* targets, int64_t labels, T* out, int64_t ldo,
+                                                       int lanes) {
+    const int rows = 256 / lanes;
+    for (int64_t i = blockIdx.x * (int64_t)rows + threadIdx.x / lanes; i < m; i += gridDim.x * (int64_t)rows) {
+        bool has = true;
+        if (targets) {
+            const int32_t t = __ldg(targets + i);
+            has = t >= 0 && t < labels;
+        }
+        const T* from = x + i * ldx;
+        T* to = out + i * ldo;
+#pragma unroll 4
+        for (int64_t j = threadIdx.x % lanes * V; j < d; j += lanes * V) {
+            if (V > 1)
+                *reinterpret_cast<uint4*>(to + j) =
+                    has ? __ldg(reinterpret_cast<const uint4*>(from + j)) : make_uint4(0, 0, 0, 0);
+            else
+                to[j] = has ? from[j] : from_f32<T>(0.f);
         }
     }
 }
@@ -272,15 +278,16 @@ void labelled_typed(int64_t m, int64_t d, const void* x, int64_t ldx, const int3
                     int64_t ldo, cudaStream_t s) {
     constexpr int V = 16 / sizeof(T);
     const bool vec = reinterpret_cast<uintptr_t>(x) % 16 == 0 && (m <= 1 || ldx % V == 0) && d % V == 0;
-    const int64_t ctas = ceil_div(m * ceil_div(d, vec ? V : 1), 256);
-    const unsigned grid = (unsigned)std::min<int64_t>(ctas, kSMs * 16);
+    int lanes = 1;
+    while (lanes < 32 && lanes * (vec ? V : 1) < d) lanes *= 2;
+    const unsigned grid = (unsigned)std::min<int64_t>(ceil_div(m * lanes, 256), kSMs * 16);
     note_launches(1);
     if (vec)
         k_labelled_rows<T, V><<<grid, 256, 0, s>>>(m, d, static_cast<const T*>(x), ldx, targets, labels,
-                                                   static_cast<T*>(out), ldo);
+                                                   static_cast<T*>(out), ldo, lanes);
     else
         k_labelled_rows<T, 1><<<grid, 256, 0, s>>>(m, d, static_cast<const T*>(x), ldx, targets, labels,
-                                                   static_cast<T*>(out), ldo);
+                                                   static_cast<T*>(out), ldo, lanes);
     OPS_CK(cudaGetLastError());
 }
 

@@ -292,6 +292,33 @@ __device__ __forceinline__ void box_copy(uint8_t* box, int first, TO* g, int64_t
                                          int64_t N, int lane) {
     constexpr int per = 16 / sizeof(TO);
     const int n = (int)min((int64_t)32, N - j0), rows = (int)min((int64_t)32, M - i0);
+    if (n == 32) {  // a row per step, eight of them in flight
+        TO* m = g + i0 * ld + j0 + lane;
+        const int piece = first + lane / per, within = lane % per;
+#pragma unroll
+        for (int r0 = 0; r0 < 32; r0 += 8) {
+            TO v[8];
+#pragma unroll
+            for (int r = 0; r < 8; ++r) {
+                TO* b = reinterpret_cast<TO*>(box + box_piece(r0 + r, piece)) + within;
+                if (!IN)
+                    v[r] = *b;
+                else if (r0 + r < rows)
+                    v[r] = m[r * ld];
+            }
+#pragma unroll
+            for (int r = 0; r < 8; ++r) {
+                TO* b = reinterpret_cast<TO*>(box + box_piece(r0 + r, piece)) + within;
+                if (r0 + r >= rows) break;
+                if (IN)
+                    *b = v[r];
+                else
+                    m[r * ld] = v[r];
+            }
+            m += 8 * ld;
+        }
+        return;
+    }
     for (int e = lane; e < rows * n; e += 32) {
         const int r = e / n, c = e - r * n;
         TO* b = reinterpret_cast<TO*>(box + box_piece(r, first + c / per)) + c % per;
