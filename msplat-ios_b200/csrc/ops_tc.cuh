@@ -292,30 +292,25 @@ __device__ __forceinline__ void box_copy(uint8_t* box, int first, TO* g, int64_t
                                          int64_t N, int lane) {
     constexpr int per = 16 / sizeof(TO);
     const int n = (int)min((int64_t)32, N - j0), rows = (int)min((int64_t)32, M - i0);
-    if (n == 32) {  // a row per step, eight of them in flight
-        TO* m = g + i0 * ld + j0 + lane;
+    if (rows == 32) {
+        // a row per step, sixteen of them in flight (lanes behind the last column
+        // read it once more)
+        TO* m = g + i0 * ld + j0 + min(lane, n - 1);
         const int piece = first + lane / per, within = lane % per;
+        const bool mine = lane < n;
 #pragma unroll
-        for (int r0 = 0; r0 < 32; r0 += 8) {
-            TO v[8];
+        for (int r0 = 0; r0 < 32; r0 += 16) {
+            TO v[16];
 #pragma unroll
-            for (int r = 0; r < 8; ++r) {
-                TO* b = reinterpret_cast<TO*>(box + box_piece(r0 + r, piece)) + within;
-                if (!IN)
-                    v[r] = *b;
-                else if (r0 + r < rows)
-                    v[r] = m[r * ld];
-            }
+            for (int r = 0; r < 16; ++r)
+                v[r] = IN ? m[(r0 + r) * ld] : reinterpret_cast<TO*>(box + box_piece(r0 + r, piece))[within];
 #pragma unroll
-            for (int r = 0; r < 8; ++r) {
-                TO* b = reinterpret_cast<TO*>(box + box_piece(r0 + r, piece)) + within;
-                if (r0 + r >= rows) break;
+            for (int r = 0; r < 16; ++r) {
                 if (IN)
-                    *b = v[r];
-                else
-                    m[r * ld] = v[r];
+                    reinterpret_cast<TO*>(box + box_piece(r0 + r, piece))[within] = v[r];
+                else if (mine)
+                    m[(r0 + r) * ld] = v[r];
             }
-            m += 8 * ld;
         }
         return;
     }

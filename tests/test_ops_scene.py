@@ -82,7 +82,7 @@ def plain_gradients(net, dcolour, keep, targets, weight):
     known = (targets >= 0) & (targets < p["table"].shape[0])
     ce = torch.nn.functional.cross_entropy((h @ p["table"].T)[known], targets[known].long()) * weight
     ((rgb * dcolour.double()).sum() + ce).backward()
-    return rgb.detach(), {k: v.grad for k, v in p.items()}, float(ce)
+    return rgb.detach(), {k: v.grad for k, v in p.items()}, float(ce.detach())
 
 
 def test_learned_colours_and_labels_gradients():
