@@ -170,9 +170,8 @@ struct Product {
     int64_t col0;       // label of column 0 of this piece
     float logit_scale;
     float g_scale;
-    float2* stats;            // [column blocks of the whole table][stats_ld]
+    float2* stats;            // [column blocks][stats_ld]
     int64_t stats_ld;
-    int64_t stats_block0;     // first column block of this piece
     float* label_logit;       // [M]
     const float* lse;         // [M], in units of log2
 };

@@ -535,7 +535,7 @@ __device__ __forceinline__ bool columns32(const Product& p, const Tiles& tl, con
 
 template <int EPI>
 __device__ __forceinline__ void row_end(const Product& p, const RowState& r, int64_t block) {
-    if (EPI == kEpiStats && r.in) p.stats[(p.stats_block0 + block) * p.stats_ld + r.i] = make_float2(r.top, r.sum);
+    if (EPI == kEpiStats && r.in) p.stats[block * p.stats_ld + r.i] = make_float2(r.top, r.sum);
 }
 
 // Columns of a tile: the widest that still gives three SMs of four one, and for the

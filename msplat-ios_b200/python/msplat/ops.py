@@ -111,8 +111,10 @@ def _act(name):
 def _enter(device, stream):
     """Makes the call's device and stream current, where they are not, so that
     what is allocated belongs to the stream: the contexts to leave again."""
+    if stream is None and device.index == _current_device():
+        return ()
     entered = []
-    if device.index != torch.cuda.current_device():
+    if device.index != _current_device():
         entered.append(torch.cuda.device(device))
     if stream is not None:
         if stream.device != device:
@@ -123,22 +125,14 @@ def _enter(device, stream):
     return entered
 
 
-class _On:
-    """The device and stream of a call. `handle` is the stream's address."""
+def _leave(entered):
+    for c in reversed(entered):
+        c.__exit__(None, None, None)
 
-    __slots__ = ("handle", "_entered")
 
-    def __init__(self, device, stream):
-        self._entered = _enter(device, stream) if stream is not None or _current_device() != device.index else None
-        self.handle = _raw_stream(device.index)
-
-    def __enter__(self):
-        return self
-
-    def __exit__(self, *a):
-        if self._entered:
-            for c in reversed(self._entered):
-                c.__exit__(*a)
+def _handle(device):
+    """The address of the current stream."""
+    return _raw_stream(device.index)
 
 
 def _current_device():
@@ -183,12 +177,17 @@ def linear_forward(x, w, bias=None, activation="none", residual=None, preact=Non
     pr, ldr = _matrix(residual, "residual", device, out_dtype, m, n)
     pz, ldz = _matrix(preact, "preact", device, out_dtype, m, n)
     act = _act(activation)
-    with _On(device, stream) as on:
+    entered = _enter(device, stream)
+    try:
         if out is None:
             out = x.new_empty((m, n)) if out_dtype == x.dtype else x.new_empty((m, n), dtype=out_dtype)
-        py, ldy = _matrix(out, "out", device, out_dtype, m, n)
+            py, ldy = out.data_ptr(), n
+        else:
+            py, ldy = _matrix(out, "out", device, out_dtype, m, n)
         _check(L.msplat_linear_forward(m, n, k, px, ldx, pw, ldw, pb, act, pr, ldr, pz, ldz, py, ldy, dt,
-                                       _DTYPES[out_dtype], on.handle))
+                                       _DTYPES[out_dtype], _handle(device)))
+    finally:
+        _leave(entered)
     return out
 
 
@@ -208,7 +207,8 @@ def linear_backward(x, w, dy, preact=None, activation="none", need_dx=True, need
     if act and preact is None:
         _refuse("preact is needed for this activation")
     pz, ldz = _matrix(preact, "preact", device, x.dtype, m, n) if act else (None, 0)
-    with _On(device, stream) as on:
+    entered = _enter(device, stream)
+    try:
         new = lambda *shape: x.new_empty(shape)  # noqa: E731
         dx = new(m, k) if need_dx else None
         dw = new(n, k) if need_dw else None
@@ -217,7 +217,9 @@ def linear_backward(x, w, dy, preact=None, activation="none", need_dx=True, need
         _check(L.msplat_linear_backward(m, n, k, px, ldx, pw, ldw, pz, ldz, act, pdy, lddy,
                                         dx.data_ptr() if need_dx else None, k, dw.data_ptr() if need_dw else None, k,
                                         dbias.data_ptr() if need_dbias else None, dt,
-                                        ws.data_ptr() if size else None, size, on.handle))
+                                        ws.data_ptr() if size else None, size, _handle(device)))
+    finally:
+        _leave(entered)
     return dx, dw, dbias
 
 
@@ -236,11 +238,16 @@ def dropout(x, p, seed, offset=0, residual=None, out=None, offset_dev=None, stre
     px, ldx = _matrix(x, "x", device, x.dtype)
     pr, ldr = _matrix(residual, "residual", device, x.dtype, m, n)
     po = _vector(offset_dev, "offset_dev", device, torch.int64, 1)
-    with _On(device, stream) as on:
+    entered = _enter(device, stream)
+    try:
         if out is None:
             out = x.new_empty((m, n))
-        py, ldy = _matrix(out, "out", device, x.dtype, m, n)
-        _check(L.msplat_dropout(m, n, px, ldx, pr, ldr, py, ldy, p, seed, offset, po, dt, on.handle))
+            py, ldy = out.data_ptr(), n
+        else:
+            py, ldy = _matrix(out, "out", device, x.dtype, m, n)
+        _check(L.msplat_dropout(m, n, px, ldx, pr, ldr, py, ldy, p, seed, offset, po, dt, _handle(device)))
+    finally:
+        _leave(entered)
     return out
 
 
@@ -258,7 +265,8 @@ def loss_cross_entropy(x, w, targets, logit_scale=1.0, weight=1.0, grad=True, st
     px, ldx = _matrix(x, "x", device, x.dtype)
     pw, ldw = _matrix(w, "w", device, x.dtype, v, d)
     pt = _vector(targets, "targets", device, torch.int32, m)
-    with _On(device, stream) as on:
+    entered = _enter(device, stream)
+    try:
         loss = torch.empty((), dtype=torch.float32, device=device)
         row_loss = torch.empty(m, dtype=torch.float32, device=device)
         dx = torch.empty((m, d), dtype=x.dtype, device=device) if grad else None
@@ -267,7 +275,9 @@ def loss_cross_entropy(x, w, targets, logit_scale=1.0, weight=1.0, grad=True, st
         _check(L.msplat_loss_cross_entropy(m, v, d, px, ldx, pw, ldw, pt, logit_scale, weight, loss.data_ptr(),
                                            row_loss.data_ptr(), dx.data_ptr() if grad else None, d,
                                            dw.data_ptr() if grad else None, d, dt, ws.data_ptr() if size else None,
-                                           size, on.handle))
+                                           size, _handle(device)))
+    finally:
+        _leave(entered)
     return loss, row_loss, dx, dw
 
 
