@@ -71,6 +71,14 @@ __global__ void __launch_bounds__(256) k_dropout(DropArgs<T> a) {
             }
 #pragma unroll
             for (int q = 0; q < (int)sizeof(T) / 2; ++q) reinterpret_cast<uint4*>(a.y + e0)[q] = vx.q[q];
+        } else if (FLAT) {
+            for (int i = 0; i < 8 && e0 + i < n; ++i) {  // the last block
+                const uint32_t word = i < 2 ? r.x : i < 4 ? r.y : i < 6 ? r.z : r.w;
+                const uint32_t draw = (i & 1) ? word >> 16 : word & 0xFFFFu;
+                float v = draw >= a.below ? to_f32(a.x[e0 + i]) * a.scale : 0.f;
+                if (a.residual) v += to_f32(a.residual[e0 + i]);
+                a.y[e0 + i] = from_f32<T>(v);
+            }
         } else {
             int64_t row = n >> 32 ? e0 / a.cols : (int64_t)((uint32_t)e0 / (uint32_t)a.cols), col = e0 - row * a.cols;
             const T* x = a.x + row * a.ldx + col;
