@@ -604,3 +604,31 @@ def test_two_threads():
     for r in got.values():
         for a, b in zip(want, r):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("t,m,n,k", [("f16", 300_000_000, 3, 9), ("bf16", 36_000_000, 64, 64), ("f32", 36_000_000, 24, 61),
+                                     ("f16", 36_000_000, 20, 61)])
+def test_far_rows(t, m, n, k):
+    """Matrices of more than 2^31 elements: the last rows of y, dx and row_loss, and a column of dw that only they reach."""
+    x = torch.zeros(m, k, dtype=R.TYPES[t], device="cuda")
+    last = normal(140, 500, k, t)
+    x[-500:] = last
+    w, b = normal(141, n, k, t, std=k ** -0.5), normal(142, 1, n, t)[0]
+    y = ops().linear_forward(x, w, b, activation="relu")
+    R.check(y[-500:], *R.linear(last, w, b, "relu", None, R.TYPES[t])[:2], "y")
+    dy = torch.zeros(m, n, dtype=R.TYPES[t], device="cuda")
+    dy[-500:] = normal(143, 500, n, t)
+    dx, dw, db = ops().linear_backward(x, w, dy, preact=y, activation="relu")
+    for got, (want, bound), name in zip((dx[-500:], dw, db), R.linear_grads(last, w, dy[-500:], y[-500:], "relu", R.TYPES[t]),
+                                        ("dx", "dw", "dbias")):
+        R.check(got, want, bound, name)
+    del y, dx, dy
+    targets = torch.full((m,), -1, dtype=torch.int32, device="cuda")
+    targets[-500:] = labels(144, 500, n)
+    _, row, dx, dw = ops().loss_cross_entropy(x, w, targets, weight=256.0)
+    want = R.loss(last, w, targets[-500:], 1.0, 256.0, R.TYPES[t])
+    R.check(row[-500:], *want["row_loss"], "row_loss")
+    R.check(dx[-500:], *want["dx"], "dx")
+    R.check(dw, *want["dw"], "dw")
+    del x, dx, row, targets
+    torch.cuda.empty_cache()
