@@ -16,6 +16,7 @@ import os
 import shutil
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
@@ -60,7 +61,7 @@ def build(verbose: bool = False, clean: bool = False) -> str:
     headers = [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith((".cuh", ".h", ".hpp"))]
     headers += [os.path.join(REPO, "include", f) for f in os.listdir(os.path.join(REPO, "include"))]
     cu, cpp = sources()
-    objs = []
+    objs, todo = [], []
     nv = nvcc()
     for f in cu + cpp:
         src = os.path.join(CSRC, f)
@@ -72,9 +73,12 @@ def build(verbose: bool = False, clean: bool = False) -> str:
         if f.endswith(".cpp"):
             cmd = ["g++", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=off", "-fno-fast-math",
                    "-I", os.path.join(REPO, "include"), "-c", src, "-o", obj]
-        if verbose:
-            print(" ".join(cmd))
-        subprocess.run(cmd, check=True)
+        todo.append(cmd)
+    # the files are compiled side by side, one compiler per core
+    with ThreadPoolExecutor(max_workers=os.cpu_count() or 1) as pool:
+        for cmd, _ in zip(todo, pool.map(lambda c: subprocess.run(c, check=True), todo)):
+            if verbose:
+                print(" ".join(cmd))
     if _stale(LIB, objs):
         cmd = [nv] + ARCH + ["-shared", "-cudart", "static", "-o", LIB] + objs + ["-lpthread", "-ldl", "-lrt"]
         if verbose:

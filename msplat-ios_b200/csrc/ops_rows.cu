@@ -508,7 +508,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         // tile before comes out
         bool ok = kXBuffers == 1 || bring(0);
         for (int count = 0; ok && count <= count_all; ++count, phase ^= 1) {
-            const int64_t tile = blockIdx.x + (int64_t)count * gridDim.x;
             if (count + kXBuffers - 1 < count_all && !bring(count + kXBuffers - 1)) break;
             if (!LABELS || count == 0) continue;
             if (!mbar_wait(smem_u32(&sm.done), phase ^ 1, gave_up)) break;

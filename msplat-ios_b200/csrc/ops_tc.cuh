@@ -4,7 +4,7 @@
 #include <atomic>
 #include <cuda.h>
 
-#include "ops_epilogue.cuh"
+#include "ops.cuh"
 
 namespace msplat {
 namespace ops {
@@ -22,6 +22,11 @@ __device__ __forceinline__ uint64_t now_ns() {
     uint64_t t;
     asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
     return t;
+}
+
+__device__ __forceinline__ bool labelled(const Product& p, int64_t row) {
+    const int32_t t = __ldg(p.targets + row);
+    return t >= 0 && t < p.labels;
 }
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
