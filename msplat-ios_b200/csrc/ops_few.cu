@@ -75,7 +75,8 @@ __global__ void __launch_bounds__(kThreads, 6) k_few(const __grid_constant__ Pro
             const int e = c * 32 + lane, r = e / PIECES, q = e - r * PIECES;
             const uintptr_t from = ((base + r * row_bytes) & ~(uintptr_t)15) + 16 * q;
             const bool ok = r < rows && from >= lo && from + 16 <= hi;
-            copy16(to + r * kPitch + q * 16, ok ? reinterpret_cast<const void*>(from) : x, ok);
+            // (what is not copied still names an aligned address, which the instruction asks for)
+            copy16(to + r * kPitch + q * 16, reinterpret_cast<const void*>(ok ? from : lo & ~(uintptr_t)15), ok);
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
