@@ -573,8 +573,15 @@ __global__ void __launch_bounds__(kThreads, 1)
                     count += 1;
                 }
                 if (p.row_loss && i < p.m && (holds || (!has && half == 0))) p.row_loss[i] = has ? row : 0.f;
-                // rows without a label have x = 0 here, finite values, and the factor 0
+                // rows without a label have x = 0 here and the factor 0; their values are
+                // finite unless a label's w is not (0 times that is NaN, and so is the sum)
                 const float factor = has ? up / sums : 0.f, scaled = sizeof(T) == 2 ? factor * p.g_scale : factor;
+                if (!has && sums != sums) {
+#pragma unroll
+                    for (int c = 0; c < VG; ++c)
+#pragma unroll
+                        for (int q = 0; q < 32; ++q) v[c][q] = 0.f;
+                }
                 const int buffer = turn % kBuffers;
                 if (!mbar_wait(smem_u32(&sm.g_free[buffer]), (turn / kBuffers & 1) ^ 1, gave_up)) break;
                 uint8_t* out = g0 + buffer * P * kGPlane + line * 128;
