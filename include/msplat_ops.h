@@ -19,9 +19,10 @@
  * call unless its comment says otherwise. Sums, softmax statistics and
  * activations are evaluated in 32 bits (matrix products of MSPLAT_DTYPE_F32
  * keep all 24 bits of both factors) and rounded once into the output's type.
- * A factor of MSPLAT_DTYPE_F32 above 3.38e38 in size counts as infinite, and an
- * infinite one may give NaN where the formula gives an infinity; factors below
- * 1e-30 may lose their lowest bits. Whatever lies in the other columns of a
+ * Infinities and NaN act as in the formulas, except that an infinite factor of
+ * MSPLAT_DTYPE_F32 may give NaN in place of an infinity beside a factor of 256 or
+ * more, or below 2^-126, in size; MSPLAT_DTYPE_F32 factors below 1e-30 may lose
+ * their lowest bits. Whatever lies in the other columns of a
  * wider record is neither used nor written, but 16-byte pieces of it between the
  * first and the last element of a matrix may be read.
  *

@@ -52,3 +52,66 @@ def test_loss_rows_without_a_label_and_a_table_that_is_not_finite(m, v, value, t
         R.check(row, *want["row_loss"], "row_loss")
         R.check(torch.cat((dw[:7], dw[8:])), *want["dw"], "dw")
         assert not dw[7].any()
+
+
+def check_wide(got, want, bound, name):
+    """R.check where the formula's value fits 32 bits; the same infinity where it is beyond them, NaN where it is NaN."""
+    top = torch.finfo(torch.float32).max
+    nan, far = want.isnan(), want.abs() > top * 1.5
+    assert torch.equal(got.isnan(), nan), f"{name}: NaN in other places"
+    assert torch.equal(got[far], torch.where(want[far] > 0, float("inf"), float("-inf")).float()), f"{name}: infinities"
+    rest = ~(nan | far)
+    R.check(got[rest], want[rest], bound[rest], name)
+
+
+@pytest.mark.parametrize("m,n,k", [(8, 40, 20), (9, 40, 20), (300, 130, 200), (5000, 3, 33), (20_000, 64, 32)])
+def test_linear_infinities_and_largest_values(m, n, k):
+    """32-bit infinities, NaN and the type's largest values in one factor or both: the formula's values from every kernel
+    (infinities beside factors below 256). Every product has at most one term that is not ordinary."""
+    big = torch.finfo(torch.float32).max
+    x, w = normal(210, m, k, "f32"), normal(211, n, k, "f32")
+    x[:, 3] = torch.tensor([float("inf"), float("-inf"), big, -big, float("nan"), 0.5, 0.0], device="cuda")[
+        torch.arange(m, device="cuda") % 7]
+    w[:, 3] = torch.tensor([1.0, -0.25, 0.0, 200.7, float("inf"), -3.3e-5, float("-inf")], device="cuda")[
+        torch.arange(n, device="cuda") % 7]
+    want = x.double() @ w.double().T
+    # the products of the ordinary terms, and the one that is not, bound the rounding
+    size = x[:, 3:4].double().abs() @ w[:, 3:4].double().abs().T
+    rest = torch.cat((x[:, :3], x[:, 4:]), 1).double().abs() @ torch.cat((w[:, :3], w[:, 4:]), 1).double().abs().T
+    off = R.SUM * (k + 8) * (size + rest)
+    check_wide(ops().linear_forward(x, w), want, off + R.rounded(want.abs(), torch.float32), "y")
+
+
+@pytest.mark.parametrize("m,n,k", [(300, 40, 24), (9000, 40, 24), (9000, 100, 50)])
+def test_linear_gradients_of_infinities(m, n, k):
+    """One infinite weight and one infinite feature: infinities of dz's signs in their columns of dx and dw, and nowhere
+    else."""
+    x, w, dy = normal(212, m, k, "f32"), normal(213, n, k, "f32"), normal(214, m, n, "f32")
+    (dx0, bx), (dw0, bw), _ = R.linear_grads(x, w, dy, None, "none", torch.float32)
+    x[m - 3, 1], w[n - 2, 4] = float("-inf"), float("inf")
+    dx, dw, _ = ops().linear_backward(x, w, dy)
+    dx0[:, 4], dw0[:, 1] = dy[:, n - 2] * float("inf"), dy[m - 3] * float("-inf")
+    check_wide(dx, dx0, bx, "dx")
+    check_wide(dw, dw0, bw, "dw")
+
+
+@pytest.mark.parametrize("m,v", [(700, 70), (8192, 40), (9001, 101)])
+@pytest.mark.parametrize("value", (float("-inf"), torch.finfo(torch.float32).min))
+def test_loss_of_a_table_padded_with_the_lowest_value(m, v, value):
+    """A label that an embedding of the lowest value takes out: its probability is 0, the rest is the table without it."""
+    d = 24
+    x, w = normal(215, m, d, "f32"), normal(216, v, d, "f32", std=d ** -0.5)
+    x[:, 5] = x[:, 5].abs() + 0.5
+    w[7, 5] = value
+    targets = labels(217, m, v, off=0.3)
+    targets[targets == 7] = 8
+    known = (targets >= 0) & (targets < v)
+    want = R.loss(x, torch.cat((w[:7], w[8:])), torch.where(targets > 7, targets - 1, targets).masked_fill(~known, -1), 1.0,
+                  100.0, torch.float32)
+    loss, row, dx, dw = ops().loss_cross_entropy(x, w, targets, weight=100.0)
+    R.check(loss, *want["loss"], "loss")
+    R.check(row, *want["row_loss"], "row_loss")
+    R.check(torch.cat((dw[:7], dw[8:])), *want["dw"], "dw")
+    assert not dw[7].any()
+    if value != float("-inf"):  # 0 times -inf is NaN in the formula too
+        R.check(dx, *want["dx"], "dx")
