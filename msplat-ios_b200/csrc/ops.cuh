@@ -51,7 +51,7 @@ __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2hal
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLog2e = 1.4426950408889634f, kLog2eRest = 1.925963e-8f;  // log2(e) is the sum
 constexpr float kLn2 = 0.6931471805599453f;
 
 // 2^x with the special function unit alone (2 units in the last place; results
@@ -69,50 +69,138 @@ __device__ __forceinline__ float recip_fast(float x) {
     return y;
 }
 
-// The Gaussian distribution function through the error function's
-// approximation 7.1.26 of Abramowitz and Stegun, Handbook of Mathematical
-// Functions: erfc(x) = t (a1 + t (a2 + ...)) exp(-x^2), t = 1 / (1 + p x), off by
-// at most 1.5e-7; a reciprocal and an exponential in place of erff's longer
-// polynomials. *density: exp(-z^2 / 2).
-__device__ __forceinline__ float normal_cdf(float z, float* density) {
-    const float x = fabsf(z) * 0.70710678118654752f;
-    const float t = recip_fast(fmaf(0.3275911f, x, 1.f));
-    const float e = exp2_fast(-kLog2e * x * x);
-    float q = fmaf(1.061405429f, t, -1.453152027f);
-    q = fmaf(q, t, 1.421413741f);
-    q = fmaf(q, t, -0.284496736f);
-    q = fmaf(q, t, 0.254829592f);
-    q = 0.5f * q * t * e;  // half of erfc(x)
-    *density = e;
-    return z < 0.f ? q : 1.f - q;
-}
-__device__ __forceinline__ float logistic(float z) { return recip_fast(1.f + exp2_fast(-kLog2e * z)); }
+// The activations, two values at a time, for results of 32 (FULL) or 16 bits.
+//
+// e^-z and e^(-z^2/2) are powers of 2 whose exponent is rounded: 2^-24 of an
+// exponent of 100 is 4e-6 of the power, far below half a step of 16 bits (2^-11) but
+// 70 steps of 32. FULL adds the rounded-off rest: 2^(b - r) = 2^b (1 - r ln 2).
+//
+// The Gaussian distribution function: with x = |z| / sqrt(2), t = 1 / (1 + p x) maps
+// 0 .. infinity to 1 .. 0, and erfc(x) e^(x^2) / t is a smooth function of t; its
+// minimax polynomials in the relative error (Remez exchange for x up to 9.4; e^(-x^2)
+// is below 2^-126 from 9.35 on), here of half of it, keep the bits of the negative
+// tail: off by 7e-9 (p = 0.4, ten coefficients, FULL; 4e-7 with t's rounding) or
+// 1.2e-6 (p = 0.5, seven).
+//
+// FULL is written with the instructions for pairs, which halve its issue slots: one
+// value at a time took 1M x 32 -> 64 with GELU from 171 to 212 us, pairs to 179.
+constexpr float kHalfLog2e = 0.72134752f, kHalfLog2eRest = 9.62981e-9f;  // log2(e) / 2 is the sum
 
-__device__ __forceinline__ float act_relu(float z) { return z < 0.f ? 0.f : z; }
-__device__ __forceinline__ float act_gelu(float z) {
-    float e;
-    return z * normal_cdf(z, &e);
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+__device__ __forceinline__ float2 exp2_rest(float2 b, float2 r) {
+    const float2 e = make_float2(exp2_fast(b.x), exp2_fast(b.y));
+    return __ffma2_rn(__fmul2_rn(e, r), both(-kLn2), e);
 }
-__device__ __forceinline__ float act_silu(float z) { return z * logistic(z); }
-__device__ __forceinline__ float act_sigmoid(float z) { return logistic(z); }
-// act'(z)
-template <int ACT>
-__device__ __forceinline__ float act_slope(float z) {
-    if (ACT == MSPLAT_ACT_RELU) return z > 0.f ? 1.f : 0.f;
-    if (ACT == MSPLAT_ACT_GELU) {
-        float e;
-        const float c = normal_cdf(z, &e);
-        return fmaf(z * 0.3989422804014327f, e, c);
+// min(|z|, 14), NaN for NaN
+__device__ __forceinline__ float size14(float z) {
+    float x;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(x) : "f"(fabsf(z)), "f"(14.f));
+    return x;
+}
+// x = size14(z): the distribution function of -x as tail * density
+__device__ __forceinline__ float2 normal_tail(float2 x, float2* density) {
+    const float2 u = __ffma2_rn(x, both(0.4f * 0.70710678118654752f), both(1.f));
+    const float2 t = make_float2(recip_fast(u.x), recip_fast(u.y));
+    float2 q = __ffma2_rn(t, both(-0.015400324f), both(0.102300011f));
+    q = __ffma2_rn(q, t, both(-0.257197171f));
+    q = __ffma2_rn(q, t, both(0.28417924f));
+    q = __ffma2_rn(q, t, both(-0.150951371f));
+    q = __ffma2_rn(q, t, both(0.140780494f));
+    q = __ffma2_rn(q, t, both(0.0631824881f));
+    q = __ffma2_rn(q, t, both(0.107818633f));
+    q = __ffma2_rn(q, t, both(0.112432256f));
+    q = __ffma2_rn(q, t, both(0.11285574f));
+    const float2 a = __fmul2_rn(x, x), b = __fmul2_rn(a, both(-kHalfLog2e));
+    const float2 rest = __ffma2_rn(x, x, __fmul2_rn(a, both(-1.f)));  // of a
+    float2 r = __ffma2_rn(a, both(kHalfLog2e), b);
+    r = __ffma2_rn(a, both(kHalfLog2eRest), r);
+    r = __ffma2_rn(rest, both(kHalfLog2e), r);
+    *density = exp2_rest(b, r);
+    return __fmul2_rn(q, t);
+}
+// the same with what 16 bits need, one value
+__device__ __forceinline__ float normal_tail16(float x, float* density) {
+    const float t = recip_fast(fmaf(0.5f * 0.70710678118654752f, x, 1.f));
+    float q = fmaf(0.0446559116f, t, -0.180322498f);
+    q = fmaf(q, t, 0.197353497f);
+    q = fmaf(q, t, 0.0169986133f);
+    q = fmaf(q, t, 0.141485006f);
+    q = fmaf(q, t, 0.138653114f);
+    q = fmaf(q, t, 0.141175792f);
+    *density = exp2_fast(-kHalfLog2e * x * x);
+    return q * t;
+}
+
+// 1 / (1 + e^-z), 0 from z = -88 downwards. *rest: what it lacks to 1 (where it
+// is not 0), which subtracting it from 1 would round off for large z.
+template <bool FULL>
+__device__ __forceinline__ float2 logistic(float2 z, float2* rest) {
+    float2 e;
+    if (FULL) {
+        const float2 x = make_float2(fminf(fmaxf(z.x, -88.f), 88.f), fminf(fmaxf(z.y, -88.f), 88.f));
+        const float2 b = __fmul2_rn(x, both(-kLog2e));
+        e = exp2_rest(b, __ffma2_rn(x, both(kLog2eRest), __ffma2_rn(x, both(kLog2e), b)));
+    } else {
+        e = make_float2(fminf(exp2_fast(-kLog2e * z.x), 3e38f), fminf(exp2_fast(-kLog2e * z.y), 3e38f));
     }
-    if (ACT == MSPLAT_ACT_SILU) {
-        const float q = logistic(z);
-        return q * fmaf(z, 1.f - q, 1.f);
+    const float2 q = make_float2(recip_fast(1.f + e.x), recip_fast(1.f + e.y));
+    *rest = __fmul2_rn(q, e);
+    return make_float2(z.x != z.x ? z.x : q.x, z.y != z.y ? z.y : q.y);
+}
+__device__ __forceinline__ float act_relu(float z) { return z < 0.f ? 0.f : z; }
+template <bool FULL>
+__device__ __forceinline__ float2 act_gelu(float2 z) {
+    // z Phi(z) = max(z, 0) - |z| Phi(-|z|)
+    const float2 x = make_float2(size14(z.x), size14(z.y)), top = make_float2(fmaxf(z.x, 0.f), fmaxf(z.y, 0.f));
+    float2 e;
+    if (FULL) return __ffma2_rn(__fmul2_rn(__fmul2_rn(normal_tail(x, &e), x), e), both(-1.f), top);
+    const float qx = normal_tail16(x.x, &e.x) * e.x, qy = normal_tail16(x.y, &e.y) * e.y;
+    return make_float2(fmaf(-x.x, qx, top.x), fmaf(-x.y, qy, top.y));
+}
+template <bool FULL>
+__device__ __forceinline__ float2 act_silu(float2 z) {
+    float2 rest;
+    return __fmul2_rn(z, logistic<FULL>(z, &rest));
+}
+template <bool FULL>
+__device__ __forceinline__ float2 act_sigmoid(float2 z) {
+    float2 rest;
+    return logistic<FULL>(z, &rest);
+}
+// act(z) for a result of type TO
+template <typename TO>
+__device__ __forceinline__ float activate(float z, int act) {
+    constexpr bool FULL = sizeof(TO) == 4;
+    return act == MSPLAT_ACT_RELU      ? act_relu(z)
+           : act == MSPLAT_ACT_GELU    ? act_gelu<FULL>(both(z)).x
+           : act == MSPLAT_ACT_SILU    ? act_silu<FULL>(both(z)).x
+           : act == MSPLAT_ACT_SIGMOID ? act_sigmoid<FULL>(both(z)).x
+                                       : z;
+}
+// act'(z) for gradients of type T
+template <int ACT, typename T>
+__device__ __forceinline__ float2 act_slope(float2 z) {
+    constexpr bool FULL = sizeof(T) == 4;
+    if (ACT == MSPLAT_ACT_RELU) return make_float2(z.x > 0.f ? 1.f : 0.f, z.y > 0.f ? 1.f : 0.f);
+    if (ACT == MSPLAT_ACT_GELU) {  // Phi + z phi is s = Phi(-|z|) - |z| phi(z) below 0 and 1 - s above
+        constexpr float kPhi = 0.3989422804014327f;
+        const float2 x = make_float2(size14(z.x), size14(z.y));
+        float2 e, s;
+        if (FULL) {
+            s = normal_tail(x, &e);
+            s = __fmul2_rn(__ffma2_rn(x, both(-kPhi), s), e);
+        } else {
+            const float qx = normal_tail16(x.x, &e.x), qy = normal_tail16(x.y, &e.y);
+            s = make_float2(fmaf(x.x, -kPhi, qx) * e.x, fmaf(x.y, -kPhi, qy) * e.y);
+        }
+        return make_float2(z.x < 0.f ? s.x : 1.f - s.x, z.y < 0.f ? s.y : 1.f - s.y);
     }
-    if (ACT == MSPLAT_ACT_SIGMOID) {
-        const float q = logistic(z);
-        return q * (1.f - q);
+    if (ACT == MSPLAT_ACT_SILU || ACT == MSPLAT_ACT_SIGMOID) {
+        float2 rest;
+        const float2 q = logistic<FULL>(z, &rest);
+        return __fmul2_rn(q, ACT == MSPLAT_ACT_SILU ? __ffma2_rn(z, rest, both(1.f)) : rest);
     }
-    return 1.f;
+    return both(1.f);
 }
 
 // Lets a kernel use `bytes` of dynamic shared memory, once per kernel and device.

@@ -139,11 +139,7 @@ __global__ void __launch_bounds__(kThreads, 6) k_few(const __grid_constant__ Pro
             if (n >= N) break;
             const float z = acc[n] + bias[n];
             if (p.preact) static_cast<TO*>(p.preact)[i * p.ldz + n] = from_f32<TO>(z);
-            float y = p.act == MSPLAT_ACT_RELU      ? act_relu(z)
-                      : p.act == MSPLAT_ACT_GELU    ? act_gelu(z)
-                      : p.act == MSPLAT_ACT_SILU    ? act_silu(z)
-                      : p.act == MSPLAT_ACT_SIGMOID ? act_sigmoid(z)
-                                                    : z;
+            float y = activate<TO>(z, p.act);
             if (p.residual) y += to_f32(static_cast<const TO*>(p.residual)[i * p.ldr + n]);
             static_cast<TO*>(p.out)[i * p.ldo + n] = from_f32<TO>(y);
         }

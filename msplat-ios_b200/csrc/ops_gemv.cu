@@ -80,11 +80,7 @@ __global__ void __launch_bounds__(kWarps * 32) k_gemv(const __grid_constant__ Pr
     if (lane >= M) return;
     const float z = mine + (p.bias ? to_f32(static_cast<const T*>(p.bias)[n]) : 0.f);
     if (p.preact) static_cast<TO*>(p.preact)[lane * p.ldz + n] = from_f32<TO>(z);
-    float y = p.act == MSPLAT_ACT_RELU      ? act_relu(z)
-              : p.act == MSPLAT_ACT_GELU    ? act_gelu(z)
-              : p.act == MSPLAT_ACT_SILU    ? act_silu(z)
-              : p.act == MSPLAT_ACT_SIGMOID ? act_sigmoid(z)
-                                            : z;
+    float y = activate<TO>(z, p.act);
     if (p.residual) y += to_f32(static_cast<const TO*>(p.residual)[lane * p.ldr + n]);
     static_cast<TO*>(p.out)[lane * p.ldo + n] = from_f32<TO>(y);
 }

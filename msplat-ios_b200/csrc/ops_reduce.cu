@@ -42,11 +42,17 @@ __global__ void __launch_bounds__(256) k_dz(int64_t m, int64_t n, const T* z, in
     auto one = [&](const Vec& a, const Vec& b, int64_t i) {
         Vec o;
 #pragma unroll
-        for (int q = 0; q < V; ++q) {
-            float v = to_f32(a.t[q]);
-            if (ACT != MSPLAT_ACT_NONE) v *= act_slope<ACT>(to_f32(b.t[q]));
-            o.t[q] = from_f32<T>(v);
-            sum[q] += v;
+        for (int q = 0; q < V; q += 2) {
+            constexpr int kNext = V > 1 ? 1 : 0;  // (one element is taken twice)
+            float2 v = make_float2(to_f32(a.t[q]), to_f32(a.t[q + kNext]));
+            if (ACT != MSPLAT_ACT_NONE)
+                v = __fmul2_rn(v, act_slope<ACT, T>(make_float2(to_f32(b.t[q]), to_f32(b.t[q + kNext]))));
+            o.t[q] = from_f32<T>(v.x);
+            sum[q] += v.x;
+            if (V > 1) {
+                o.t[q + kNext] = from_f32<T>(v.y);
+                sum[q + kNext] += v.y;
+            }
         }
         if (!dz) return;
         T* g = dz + i * lddz + j;

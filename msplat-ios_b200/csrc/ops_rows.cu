@@ -648,10 +648,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                         const int line = t / 8 + 32 * q;
                         float g[8];
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) {
-                            g[e] = chunk_at(a[q], e);
-                            if (ACT != MSPLAT_ACT_NONE) g[e] *= act_slope<ACT>(chunk_at(b[q], e));
-                            sums[c][e] += g[e];
+                        for (int e = 0; e < 8; e += 2) {
+                            float2 v = make_float2(chunk_at(a[q], e), chunk_at(a[q], e + 1));
+                            if (ACT != MSPLAT_ACT_NONE)
+                                v = __fmul2_rn(v, act_slope<ACT, T>(make_float2(chunk_at(b[q], e), chunk_at(b[q], e + 1))));
+                            g[e] = v.x;
+                            g[e + 1] = v.y;
+                            sums[c][e] += v.x;
+                            sums[c][e + 1] += v.y;
                         }
                         put8<T>(gs + c * kGGroup + line * 128 + ((t % 8) ^ (line & 7)) * 16, kGPlane, g);
                     }

@@ -330,24 +330,22 @@ __device__ __forceinline__ void box_copy(uint8_t* box, int first, TO* g, int64_t
     }
 }
 
+template <typename TO>
 __device__ __forceinline__ void activate32(float (&v)[32], int act) {
+    constexpr bool FULL = sizeof(TO) == 4;
+    auto pairs = [&](auto f) {
+#pragma unroll
+        for (int q = 0; q < 32; q += 2) {
+            const float2 y = f(make_float2(v[q], v[q + 1]));
+            v[q] = y.x;
+            v[q + 1] = y.y;
+        }
+    };
     switch (act) {
-        case MSPLAT_ACT_RELU:
-#pragma unroll
-            for (int q = 0; q < 32; ++q) v[q] = act_relu(v[q]);
-            break;
-        case MSPLAT_ACT_GELU:
-#pragma unroll
-            for (int q = 0; q < 32; ++q) v[q] = act_gelu(v[q]);
-            break;
-        case MSPLAT_ACT_SILU:
-#pragma unroll
-            for (int q = 0; q < 32; ++q) v[q] = act_silu(v[q]);
-            break;
-        case MSPLAT_ACT_SIGMOID:
-#pragma unroll
-            for (int q = 0; q < 32; ++q) v[q] = act_sigmoid(v[q]);
-            break;
+        case MSPLAT_ACT_RELU: pairs([](float2 z) { return make_float2(act_relu(z.x), act_relu(z.y)); }); break;
+        case MSPLAT_ACT_GELU: pairs([](float2 z) { return act_gelu<FULL>(z); }); break;
+        case MSPLAT_ACT_SILU: pairs([](float2 z) { return act_silu<FULL>(z); }); break;
+        case MSPLAT_ACT_SIGMOID: pairs([](float2 z) { return act_sigmoid<FULL>(z); }); break;
         default: break;
     }
 }
@@ -439,7 +437,7 @@ __device__ __forceinline__ bool write32(const Product& p, const Tiles& tl, const
             if (tl.tma_out && !free_now && !second) boxes_free(tl, lane);
             box_write<TO>(z, lane, first, v);
         }
-        activate32(v, p.act);
+        activate32<TO>(v, p.act);
         if (p.residual) {
             if (tl.tma_out) {
                 if (!second) {

@@ -1,5 +1,7 @@
 """Edges of the operators of msplat.ops (GPU): places, values and streams at which one kernel's answer could differ from
 another's, or from the formula's."""
+import math
+
 import pytest
 
 torch = pytest.importorskip("torch")
@@ -115,3 +117,75 @@ def test_loss_of_a_table_padded_with_the_lowest_value(m, v, value):
     assert not dw[7].any()
     if value != float("-inf"):  # 0 times -inf is NaN in the formula too
         R.check(dx, *want["dx"], "dx")
+
+
+# ---- activations, relative to their own size --------------------------------------------------------------------------
+
+# Steps of 2^-24 that the functions may be off by in 32 bits. gelu: the reciprocal and its argument (t: 2 steps, which
+# change erfc(x) e^(x^2) by 1.13 / 0.4 times as much), ten coefficients' roundings (1 at each end), the density (its
+# power 4, its exponent's two corrections 1) and two products: 14. sigmoid: the power 4, the exponent 1, sum, reciprocal 2,
+# product: 10.
+STEPS = 16 * 2.0 ** -24
+
+
+def phi(z):
+    """The Gaussian distribution function in 64 bits with all its bits in the negative tail (1 + erf cancels there)."""
+    return 0.5 * torch.special.erfc(-z / math.sqrt(2))
+
+
+def tail_values(t, low):
+    return torch.cat((torch.linspace(low, 0, 3001), torch.linspace(0, -low, 1001), torch.tensor([-1e-3, 1e-3, 0.0]))).to(
+        R.TYPES[t])
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("rows", (1, 40, 5000))
+@pytest.mark.parametrize("act,low", [("gelu", -12.5), ("silu", -80.0), ("sigmoid", -80.0)])
+def test_activations_keep_their_small_values(act, low, rows, t):
+    """act(z) for z passed through a layer of one input and weight 1: within half a step of the result's type and a few of
+    32 bits of act(z), however small it is."""
+    z = tail_values(t, low).cuda()
+    for out_t in {R.TYPES[t], torch.float32}:
+        if rows == 1:    # a row against many weights
+            y = ops().linear_forward(torch.ones(1, 1, dtype=z.dtype, device="cuda"), z[:, None].contiguous(), activation=act,
+                             out_dtype=out_t)[0]
+            at = z
+        elif rows == 40:
+            at = z[:rows * 100].reshape(rows, 100)
+            x = torch.zeros(rows, 100, dtype=z.dtype, device="cuda").copy_(at)
+            y = ops().linear_forward(x, torch.eye(100, dtype=z.dtype, device="cuda"), activation=act, out_dtype=out_t)
+        else:
+            at = z.repeat(2)[:rows, None].contiguous()
+            y = ops().linear_forward(at, torch.ones(1, 1, dtype=z.dtype, device="cuda"), activation=act, out_dtype=out_t)
+        want = at.double() * phi(at.double()) if act == "gelu" else R.act(at.double(), act)
+        off = (STEPS if out_t == torch.float32 else 2e-5) * want.abs() + 2.0 ** -126
+        R.check(y, want, off + R.rounded(want.abs() + off, out_t), act)
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("m", (40, 9000))
+@pytest.mark.parametrize("act,low", [("gelu", -12.5), ("silu", -80.0), ("sigmoid", -80.0)])
+def test_slopes_keep_their_small_values(act, low, m, t):
+    """dy act'(z) through dx of a layer with the weights 1: relative to its own size, away from where it changes its sign."""
+    n = 100
+    z = tail_values(t, low).repeat(4)[:m * n] if m == 40 else tail_values(t, low).repeat(m * n // 4000)[:m * n]
+    z = torch.cat((z, z.new_zeros(m * n - z.numel()))).reshape(m, n).cuda()
+    eye = torch.eye(n, dtype=z.dtype, device="cuda") if m == 40 else torch.eye(64, dtype=z.dtype, device="cuda")
+    z = z[:, :eye.shape[0]].contiguous()
+    x, dy = torch.zeros_like(z), torch.ones_like(z)
+    dx, _, _ = ops().linear_backward(x, eye, dy, preact=z, activation=act)
+    want = R.slope(z.double(), act)
+    if act == "sigmoid":  # q (1 - q), which cancels in the reference for large z
+        q = torch.sigmoid(-z.double().abs())
+        want = q * (1 - q)
+    if act == "gelu":
+        want = phi(z.double()) + z.double() * torch.exp(-z.double() ** 2 / 2) / math.sqrt(2 * math.pi)
+    # gelu: Phi + z phi, silu: q + z q (1 - q): rounded from the sizes of both terms
+    size = want.abs()
+    if act == "gelu":
+        size = phi(z.double()) + (z.double() * torch.exp(-z.double() ** 2 / 2) * 0.4).abs()
+    if act == "silu":
+        size = torch.sigmoid(z.double()) * (1 + (z.double() * torch.sigmoid(-z.double())).abs())
+    off = (STEPS if t == "f32" else 2e-5) * size + 2.0 ** -126
+    twice = off + 2 * R.rounded(want.abs() + off, R.TYPES[t])  # dz between the products, and dx
+    R.check(dx, want, twice, act)
