@@ -121,10 +121,19 @@ int msplat_loss_cross_entropy(int64_t m, int64_t v, int64_t d, const void* x, in
                               void* workspace, uint64_t workspace_bytes, void* stream);
 
 /* Waits for `stream`, then MSPLAT_OK, or MSPLAT_ERR_CUDA when a kernel of this
- * file gave up waiting for its own copies or products since the last call (its
- * waits are bounded; its results are then not valid). Not for use while a
- * stream is being captured. */
+ * file, on any stream of the same device, gave up waiting for its own copies or
+ * products since the last call for this stream (the first call: since the library
+ * was loaded). Its waits are bounded; its results are then not valid. Each
+ * stream's call tells of each failure once, so none is lost to another stream's
+ * call. One number per stream that has asked is kept. Not for use while a stream
+ * is being captured. */
 int msplat_ops_status(void* stream);
+
+/* Launches a kernel that waits one millisecond for something that never comes and
+ * gives up, as a kernel of `kernels` (0: 16-bit products, 1: other products, 2:
+ * many rows against a small matrix) would: for trying how a program deals with
+ * what msplat_ops_status then returns. No other result is touched. */
+int msplat_ops_rehearse_timeout(int32_t kernels, void* stream);
 
 #ifdef __cplusplus
 }

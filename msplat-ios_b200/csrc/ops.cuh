@@ -274,7 +274,8 @@ void launch_product(const Product& p, cudaStream_t s);
 bool can_product_tc16(const Product& p);
 int64_t stats_blocks_tc16(const Product& p);
 void launch_product_tc16(const Product& p, cudaStream_t s);
-bool gave_up_tc16(cudaStream_t s);
+unsigned gave_up_tc16(cudaStream_t s);
+void give_up_tc16(cudaStream_t s);
 void launch_product_tcv(const Product& p, cudaStream_t s);
 // layers of a few rows (ops_gemv.cu)
 bool can_product_gemv(const Product& p);
@@ -283,14 +284,16 @@ void launch_product_gemv(const Product& p, cudaStream_t s);
 bool can_product_few(const Product& p);
 void launch_product_few(const Product& p, cudaStream_t s);
 int64_t stats_blocks_tcv(const Product& p);
-bool gave_up_tcv(cudaStream_t s);
+unsigned gave_up_tcv(cudaStream_t s);
+void give_up_tcv(cudaStream_t s);
 
 // Many rows against a small matrix in one pass (ops_rows.cu): v x d w, at most
 // 128 x 64. slab: [rows_blocks(m)][v][slab_ld(d)] partial sums of dw, sums:
 // [rows_blocks(m)][v] of g; each may be null, and dx.
 bool fits_rows(int64_t m, int64_t v, int64_t d);
 int rows_blocks(int64_t m);
-bool gave_up_rows(cudaStream_t s);
+unsigned gave_up_rows(cudaStream_t s);
+void give_up_rows(cudaStream_t s);
 void launch_rows_labels(int64_t m, int64_t v, int64_t d, const void* x, int64_t ldx, const void* w, int64_t ldw,
                         const int32_t* targets, float logit_scale, float g_scale, const float* alpha, float* row_loss,
                         double* partial, void* dx, int64_t lddx, float* slab, int dtype, cudaStream_t s);

@@ -1,7 +1,11 @@
 // ops_api.cu — the entry points of include/msplat_ops.h: checks, the layout of
 // the caller's workspace, and the order of the launches.
 #include <algorithm>
+#include <array>
 #include <cmath>
+#include <map>
+#include <mutex>
+#include <utility>
 
 #include "ops.cuh"
 
@@ -223,6 +227,20 @@ void launch_gradient(Product q, const LossPlan& plan, float* slab, Split split, 
                         q.targets, labels, dtype, s);
 }
 
+// Makes a stream's device current (the null stream's is).
+struct OnDeviceOf {
+    int device = 0, before = 0;
+    explicit OnDeviceOf(cudaStream_t s) {
+        OPS_CK(cudaGetDevice(&before));
+        OPS_CK(cudaStreamGetDevice(s, &device));
+        if (device != before) OPS_CK(cudaSetDevice(device));
+    }
+    ~OnDeviceOf() {
+        if (device != before) cudaSetDevice(before);
+    }
+    OnDeviceOf(const OnDeviceOf&) = delete;
+};
+
 const char* at(const void* p, int64_t elements, int es) { return static_cast<const char*>(p) + elements * es; }
 char* at(void* p, int64_t elements, int es) { return static_cast<char*>(p) + elements * es; }
 
@@ -237,10 +255,29 @@ extern "C" {
 
 int msplat_ops_status(void* stream) {
     return guarded([&] {
-        const bool tc16 = gave_up_tc16(static_cast<cudaStream_t>(stream));
-        const bool rows = gave_up_rows(static_cast<cudaStream_t>(stream));
-        if (gave_up_tcv(static_cast<cudaStream_t>(stream)) || tc16 || rows)
-            throw Error(MSPLAT_ERR_CUDA, "a kernel gave up waiting: the results since the last call are not valid");
+        cudaStream_t s = static_cast<cudaStream_t>(stream);
+        OnDeviceOf on(s);
+        unsigned long long id = 0;
+        OPS_CK(cudaStreamGetId(s, &id));
+        const std::array<unsigned, 3> now = {gave_up_tc16(s), gave_up_tcv(s), gave_up_rows(s)};
+        // (a stream that has not asked yet starts from none)
+        static std::mutex lock;
+        static std::map<std::pair<int, unsigned long long>, std::array<unsigned, 3>> told;
+        std::lock_guard<std::mutex> hold(lock);
+        std::array<unsigned, 3>& last = told[{on.device, id}];
+        const bool more = last != now;
+        last = now;
+        if (more)
+            throw Error(MSPLAT_ERR_CUDA, "a kernel gave up waiting: results since this stream's last call are not valid");
+    });
+}
+
+int msplat_ops_rehearse_timeout(int32_t kernels, void* stream) {
+    return guarded([&] {
+        require(kernels >= 0 && kernels <= 2, "kernels must be 0, 1 or 2");
+        cudaStream_t s = static_cast<cudaStream_t>(stream);
+        OnDeviceOf on(s);
+        kernels == 0 ? give_up_tc16(s) : kernels == 1 ? give_up_tcv(s) : give_up_rows(s);
     });
 }
 

@@ -769,7 +769,8 @@ void launch(const RowsArgs& a, int dtype, cudaStream_t s) {
 
 }  // namespace
 
-bool gave_up_rows(cudaStream_t s) { return take_gave_up(s); }
+unsigned gave_up_rows(cudaStream_t s) { return count_gave_up(s); }
+void give_up_rows(cudaStream_t s) { launch_give_up(s); }
 
 bool fits_rows(int64_t m, int64_t v, int64_t d) { return v <= 128 && d <= 64 && m >= 8192; }
 int rows_blocks(int64_t m) { return (int)std::min<int64_t>(ceil_div(m, kBM), kSMs); }

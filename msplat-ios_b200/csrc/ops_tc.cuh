@@ -12,7 +12,7 @@ namespace ops {
 constexpr int kBM = 128;       // rows of a tile: the lanes of TMEM
 constexpr int kBR = 64;        // reduction length of one stage: 128 bytes of a 16-bit type, one swizzle span
 
-// Set when a wait in a kernel ran out (read and cleared by take_gave_up).
+// How many waits of this file's kernels ran out (each .cu file has its own).
 static __device__ unsigned g_ops_gave_up;
 
 // A wait gives up after this many nanoseconds; a block waits only for its own
@@ -51,9 +51,10 @@ __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
         : "memory");
     return ok;
 }
-// Waits for the phase, at most kWaitNs.
-__device__ __forceinline__ bool mbar_wait_bounded(uint32_t bar, uint32_t parity, volatile int* gave_up) {
-    const uint64_t end = now_ns() + kWaitNs;
+// Waits for the phase, at most `ns`.
+__device__ __forceinline__ bool mbar_wait_bounded(uint32_t bar, uint32_t parity, volatile int* gave_up,
+                                                  uint64_t ns = kWaitNs) {
+    const uint64_t end = now_ns() + ns;
     do {
         if (mbar_try(bar, parity)) return true;
         if (gave_up && *gave_up) return false;
@@ -62,11 +63,11 @@ __device__ __forceinline__ bool mbar_wait_bounded(uint32_t bar, uint32_t parity,
 }
 // Waits for the phase; false when this wait, or any other wait of the block,
 // gave up.
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* gave_up) {
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* gave_up, uint64_t ns = kWaitNs) {
     if (mbar_try(bar, parity)) return true;
-    if (mbar_wait_bounded(bar, parity, gave_up)) return true;
+    if (mbar_wait_bounded(bar, parity, gave_up, ns)) return true;
     *gave_up = 1;
-    atomicOr(&g_ops_gave_up, 1u);
+    atomicAdd(&g_ops_gave_up, 1u);
     return false;
 }
 
@@ -159,17 +160,27 @@ inline uint32_t instr_desc(bool bf16, bool a_mn, bool b_mn, int bn) {
            (uint32_t)(bn >> 3) << 17 | (uint32_t)(kBM >> 4) << 24;
 }
 
-// Whether a wait gave up in this translation unit's kernels since the last call.
-inline bool take_gave_up(cudaStream_t s) {
+// How many waits gave up in this file's kernels, once the stream (of the current
+// device) has finished. Static, as the counter is: one definition for all files
+// would read one file's.
+static unsigned count_gave_up(cudaStream_t s) {
     unsigned v = 0;
-    const unsigned zero = 0;
     OPS_CK(cudaMemcpyFromSymbolAsync(&v, g_ops_gave_up, sizeof(v), 0, cudaMemcpyDeviceToHost, s));
     OPS_CK(cudaStreamSynchronize(s));
-    if (v) {
-        OPS_CK(cudaMemcpyToSymbolAsync(g_ops_gave_up, &zero, sizeof(v), 0, cudaMemcpyHostToDevice, s));
-        OPS_CK(cudaStreamSynchronize(s));
-    }
-    return v != 0;
+    return v;
+}
+// A wait of a millisecond for a barrier at which nobody arrives.
+static __global__ void k_give_up() {
+    __shared__ uint64_t bar;
+    __shared__ int gave_up;
+    gave_up = 0;
+    mbar_init(smem_u32(&bar), 1);
+    mbar_wait(smem_u32(&bar), 0, &gave_up, 1000000);
+}
+static void launch_give_up(cudaStream_t s) {
+    note_launches(1);
+    k_give_up<<<1, 1, 0, s>>>();
+    OPS_CK(cudaGetLastError());
 }
 
 // How a product is cut into tiles.

@@ -299,7 +299,8 @@ bool tma_ready(const void* p, int64_t ld, int64_t rows, int elem) {
            (rows <= 1 || (ld * elem % 16 == 0 && ld * elem < (1ll << 40) / rows));
 }
 
-bool gave_up_tc16(cudaStream_t s) { return take_gave_up(s); }
+unsigned gave_up_tc16(cudaStream_t s) { return count_gave_up(s); }
+void give_up_tc16(cudaStream_t s) { launch_give_up(s); }
 
 bool can_product_tc16(const Product& p) {
     return p.dtype != MSPLAT_DTYPE_F32 && tma_ready(p.A, p.lda, p.a_mn ? p.R : p.M, 2) &&

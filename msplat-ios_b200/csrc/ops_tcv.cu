@@ -317,7 +317,8 @@ int columns_tcv(const Product& p) {
 
 }  // namespace
 
-bool gave_up_tcv(cudaStream_t s) { return take_gave_up(s); }
+unsigned gave_up_tcv(cudaStream_t s) { return count_gave_up(s); }
+void give_up_tcv(cudaStream_t s) { launch_give_up(s); }
 
 int64_t stats_blocks_tcv(const Product& p) { return stats_blocks_of(p, columns_tcv(p)); }
 

@@ -42,9 +42,10 @@ def _lib():
     L.msplat_loss_cross_entropy.argtypes = [i64, i64, i64, vp, i64, vp, i64, vp, f, f, vp, vp, vp, i64, vp, i64, i32,
                                             vp, u64, vp]
     L.msplat_ops_status.argtypes = [vp]
+    L.msplat_ops_rehearse_timeout.argtypes = [i32, vp]
     for name in ("msplat_linear_forward", "msplat_linear_backward_workspace", "msplat_linear_backward",
                  "msplat_dropout", "msplat_loss_cross_entropy_workspace", "msplat_loss_cross_entropy",
-                 "msplat_ops_status"):
+                 "msplat_ops_status", "msplat_ops_rehearse_timeout"):
         getattr(L, name).restype = C.c_int
     _L = L
     return L
@@ -282,7 +283,10 @@ def loss_cross_entropy(x, w, targets, logit_scale=1.0, weight=1.0, grad=True, st
 
 
 def status(stream=None):
-    """Waits for the stream and raises MsplatError when a kernel gave up
-    waiting since the last call (its waits are bounded)."""
+    """Waits for the stream and raises MsplatError when a kernel on any stream of
+    its device gave up waiting since the last call for this stream (its waits are
+    bounded)."""
     s = stream if stream is not None else torch.cuda.current_stream()
-    _check(_lib().msplat_ops_status(s.cuda_stream))
+    L = _lib()
+    with torch.cuda.device(s.device):
+        _check(L.msplat_ops_status(s.cuda_stream))

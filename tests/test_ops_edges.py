@@ -189,3 +189,31 @@ def test_slopes_keep_their_small_values(act, low, m, t):
     off = (STEPS if t == "f32" else 2e-5) * size + 2.0 ** -126
     twice = off + 2 * R.rounded(want.abs() + off, R.TYPES[t])  # dz between the products, and dx
     R.check(dx, want, twice, act)
+
+
+# ---- kernels that gave up waiting --------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("kernels", (0, 1, 2))
+def test_status_tells_every_stream_of_a_wait_that_ran_out(kernels):
+    """A wait for a barrier at which nobody arrives gives up after a millisecond, whichever kernels' it is; each stream's
+    next status raises, once, and another stream's call takes nothing away."""
+    o = ops()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+
+    def raises(s):
+        try:
+            o.status(s)
+            return False
+        except o.MsplatError as e:
+            assert "gave up" in str(e)
+            return True
+    for s in (*streams, None):
+        raises(s)  # what earlier tests left
+    assert not any(raises(s) for s in (*streams, None))
+    assert o._lib().msplat_ops_rehearse_timeout(kernels, streams[0].cuda_stream) == 0
+    assert raises(streams[0]) and raises(streams[1]) and raises(None)
+    assert not any(raises(s) for s in (*streams, None))
+    x, w = normal(220, 300, 64, "bf16"), normal(221, 64, 64, "bf16")
+    R.check(o.linear_forward(x, w), *R.linear(x, w, None, "none", None, torch.bfloat16)[:2], "y")
+    assert not raises(None)
