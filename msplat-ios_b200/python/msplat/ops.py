@@ -6,8 +6,12 @@ are contiguous (a slice of columns of a wider tensor will do), of one type per
 call: float32, float16 or bfloat16. The calls run on `stream` (by default the
 current stream of the tensors' device); results and workspaces come from
 torch's allocator on that stream, so calls on several streams, and calls
-captured into CUDA graphs, do not share any. There is no CPU or PyTorch
-fallback: a refused or failed call raises MsplatError.
+captured into CUDA graphs, do not share any. A `stream` that is given has to wait
+for whatever writes the call's inputs (Stream.wait_stream), and whoever reads the
+results elsewhere for it; the inputs' memory is kept until it has used them, even
+if they are freed. Gradients come from the calls for them, not from autograd: the
+results of tensors that require one are not part of its graph. There is no CPU or
+PyTorch fallback: a refused or failed call raises MsplatError.
 """
 from __future__ import annotations
 
@@ -131,6 +135,15 @@ def _leave(entered):
         c.__exit__(None, None, None)
 
 
+def _used(stream, *tensors):
+    """Keeps the memory of the caller's tensors, should they be freed, until the
+    stream that was given has used them."""
+    if stream is not None:
+        for t in tensors:
+            if t is not None:
+                t.record_stream(stream)
+
+
 def _handle(device):
     """The address of the current stream."""
     return _raw_stream(device.index)
@@ -187,6 +200,7 @@ def linear_forward(x, w, bias=None, activation="none", residual=None, preact=Non
             py, ldy = _matrix(out, "out", device, out_dtype, m, n)
         _check(L.msplat_linear_forward(m, n, k, px, ldx, pw, ldw, pb, act, pr, ldr, pz, ldz, py, ldy, dt,
                                        _DTYPES[out_dtype], _handle(device)))
+        _used(stream, x, w, bias, residual, preact, out)
     finally:
         _leave(entered)
     return out
@@ -219,6 +233,7 @@ def linear_backward(x, w, dy, preact=None, activation="none", need_dx=True, need
                                         dx.data_ptr() if need_dx else None, k, dw.data_ptr() if need_dw else None, k,
                                         dbias.data_ptr() if need_dbias else None, dt,
                                         ws.data_ptr() if size else None, size, _handle(device)))
+        _used(stream, x, w, dy, preact)
     finally:
         _leave(entered)
     return dx, dw, dbias
@@ -247,6 +262,7 @@ def dropout(x, p, seed, offset=0, residual=None, out=None, offset_dev=None, stre
         else:
             py, ldy = _matrix(out, "out", device, x.dtype, m, n)
         _check(L.msplat_dropout(m, n, px, ldx, pr, ldr, py, ldy, p, seed, offset, po, dt, _handle(device)))
+        _used(stream, x, residual, out, offset_dev)
     finally:
         _leave(entered)
     return out
@@ -277,6 +293,7 @@ def loss_cross_entropy(x, w, targets, logit_scale=1.0, weight=1.0, grad=True, st
                                            row_loss.data_ptr(), dx.data_ptr() if grad else None, d,
                                            dw.data_ptr() if grad else None, d, dt, ws.data_ptr() if size else None,
                                            size, _handle(device)))
+        _used(stream, x, w, targets)
     finally:
         _leave(entered)
     return loss, row_loss, dx, dw

@@ -217,3 +217,36 @@ def test_status_tells_every_stream_of_a_wait_that_ran_out(kernels):
     x, w = normal(220, 300, 64, "bf16"), normal(221, 64, 64, "bf16")
     R.check(o.linear_forward(x, w), *R.linear(x, w, None, "none", None, torch.bfloat16)[:2], "y")
     assert not raises(None)
+
+
+# ---- inputs that are freed while another stream still reads them ----------------------------------------------------------
+
+
+@pytest.mark.parametrize("op", ("linear_forward", "linear_backward", "dropout", "loss_cross_entropy"))
+def test_inputs_freed_before_the_given_stream_has_read_them(op):
+    """The caller's inputs are freed and their memory asked for again while the stream is still busy with something else."""
+    o, m, n, k = ops(), 3001, 37, 41
+
+    def inputs():
+        x, w, y = normal(230, m, k, "f32").clone(), normal(231, n, k, "f32").clone(), normal(232, m, n, "f32").clone()
+        return {"linear_forward": ((x, w), dict(bias=w[:, 0].contiguous(), residual=y, activation="gelu")),
+                "linear_backward": ((x, w, y), dict(preact=y.clone(), activation="gelu")),
+                "dropout": ((x, 0.3, 5), dict(residual=x.clone(), offset_dev=torch.tensor([7], device="cuda"))),
+                "loss_cross_entropy": ((x, w, labels(233, m, n)), {})}[op]
+    args, more = inputs()
+    want = getattr(o, op)(*args, **more)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(50_000_000)  # some 25 ms
+    got = getattr(o, op)(*args, **more, stream=side)
+    held = [t for t in (*args, *more.values()) if isinstance(t, torch.Tensor)]
+    sizes, at = [(t.shape, t.dtype) for t in held], {t.data_ptr() for t in held}
+    del args, more, held
+    again = [torch.empty(s, dtype=d, device="cuda") for s, d in sizes for _ in range(2)]
+    assert not side.query() and not at & {t.data_ptr() for t in again}
+    [t.fill_(-1) for t in again]
+    torch.cuda.synchronize()
+    want, got = ((v,) if isinstance(v, torch.Tensor) else v for v in (want, got))
+    for a, b in zip(want, got):
+        assert torch.equal(a, b)
