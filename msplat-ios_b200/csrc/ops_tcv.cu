@@ -7,10 +7,13 @@
 // of two factors is then h h' (accumulated on its own) and h m' + m h' + m m' +
 // h l' + l h' (accumulated together, 2^-8 smaller), six tcgen05.mma in place of
 // one; what is left out is below 2^-24 of the product. The tensor cores
-// truncate when they add (measured: 1e-9 of the sum per element of the
-// reduction), so a long reduction changes to a fresh accumulator after every
-// 512 elements while there are some, and the accumulators are added with
-// rounding at the end.
+// truncate when they add (measured: 2e-9 of a sum of one sign per element of the
+// reduction, 7e-7 after 512), so a 32-bit reduction changes to a fresh accumulator
+// after every 512 elements, and the accumulators are added with rounding by the
+// ends, after three of them already where the reduction is longer (LONG: 16384
+// elements of one sign are off by 1e-6 of their sum, with the last accumulator
+// taking all the rest they were off by 7e-5; 8192 x 2048 -> 1024 takes 350 us, 348
+// without). 16-bit reductions beyond the accumulators stay in the last one.
 //
 // A block owns 128 x bn tiles (bn 64 or 128) and walks its share of them. Warps
 // 12-19 load, split and store the stages (the layout is TMA's 128-byte swizzle,
@@ -50,7 +53,10 @@ struct Smem {
 };
 static_assert(offsetof(Smem, bias) % 16 == 0 && sizeof(Smem) <= 2048, "read as float4; share_memory counts 2048");
 
-template <typename T, int EPI, int BN>
+// LONG (32-bit factors, 64 columns): a reduction longer than a tile's accumulators
+// take goes through them in passes; the two groups of warps then take half of a
+// tile's columns each.
+template <typename T, int EPI, int BN, bool LONG>
 __global__ void __launch_bounds__(kThreads, 1)
     k_product_tcv(const __grid_constant__ Product p, const __grid_constant__ Tiles tl,
                   const __grid_constant__ OutMaps maps, const bool vec_a, const bool vec_b) {
@@ -59,6 +65,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     // accumulators of one tile: the groups' and, for split factors, the corrections'
     constexpr int kGroups = 512 / 2 / BN - (P > 1 ? 1 : 0);
     constexpr int kTileCols = 256;
+    constexpr int kPass = kGroups * kGroup;  // stages of a pass
+    static_assert(!LONG || (P > 1 && BN == 64), "passes are for what needs them");
+    // tiles of 64 columns: the two groups of warps take every other tile; wider
+    // ones and passes: each takes half of the columns
+    constexpr bool kByTile = BN == 64 && !LONG;
     const int stage_bytes = tl.stage_bytes;  // A, and B unless it is resident
     extern __shared__ __align__(1024) uint8_t dyn[];
     __shared__ Smem sm;
@@ -74,7 +85,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         for (int q = 0; q < 2; ++q) {
             mbar_init(smem_u32(&sm.acc_full[q]), 1);
-            mbar_init(smem_u32(&sm.acc_empty[q]), BN == 64 ? kEpiWarps / 2 : kEpiWarps);
+            mbar_init(smem_u32(&sm.acc_empty[q]), kByTile ? kEpiWarps / 2 : kEpiWarps);
         }
         mbar_init(smem_u32(&sm.drain), 1);
         for (int q = 0; q < 2 * kEpiWarps; ++q) mbar_init(smem_u32(&sm.residual[q / 2][q % 2]), 1);
@@ -133,9 +144,20 @@ __global__ void __launch_bounds__(kThreads, 1)
             tile_of(p, tl, w, tm, tn, split, r0, r1);
             if (!(ok = mbar_wait(smem_u32(&sm.acc_empty[acc]), acc_phase ^ 1, gave_up))) break;
             tc_fence_after();
-            const uint32_t d = tmem + acc * kTileCols, dc = d + kGroups * BN;
+            uint32_t d = tmem + acc * kTileCols, dc = d + kGroups * BN;
             int block = 0;
             for (int64_t r = r0; r < r1; r += kBR, ++block) {
+                if (LONG && block == kPass) {
+                    if (elect_one()) tc_commit(smem_u32(&sm.acc_full[acc]));
+                    __syncwarp();
+                    acc ^= 1;
+                    if (acc == 0) acc_phase ^= 1;
+                    if (!(ok = mbar_wait(smem_u32(&sm.acc_empty[acc]), acc_phase ^ 1, gave_up))) break;
+                    tc_fence_after();
+                    d = tmem + acc * kTileCols;
+                    dc = d + kGroups * BN;
+                    block = 0;
+                }
                 if (!(ok = mbar_wait(smem_u32(&sm.full[stage]), phase, gave_up))) break;
                 tc_fence_after();
                 if (elect_one()) {
@@ -185,9 +207,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kEpiRegs));
-        // tiles of 64 columns: the two groups of warps take every other tile;
-        // wider ones: each takes half of the columns
-        constexpr bool kByTile = BN == 64;
         constexpr int kHalf = kByTile ? BN : BN / 2;
         const int quarter = warp % 4, group = (warp - 4) / 4, half = kByTile ? 0 : group;
         WarpOut o;
@@ -211,9 +230,32 @@ __global__ void __launch_bounds__(kThreads, 1)
             tile_of(p, tl, w, tm, tn, split, r0, r1);
             const int64_t i0 = (int64_t)tm * kBM + quarter * 32, j0 = (int64_t)tn * BN + half * kHalf;
             const int64_t j_end = min(p.N, j0 + kHalf);
-            const int parts = (int)min((int64_t)kGroups, (r1 - r0 + kGroup * kBR - 1) / (kGroup * kBR));
             RowState row = row_begin<EPI>(p, i0, lane);
             if (EPI == kEpiLinear && j0 < j_end) fetch_residual(p, tl, maps, o, i0, j0, lane);
+            float total[LONG ? 32 : 1];
+            if (LONG) {  // all passes but the last
+#pragma unroll
+                for (int q = 0; q < (LONG ? 32 : 0); ++q) total[q] = 0.f;
+                for (; r1 - r0 > kPass * kBR; r0 += kPass * kBR) {
+                    if (!(ok = mbar_wait(smem_u32(&sm.acc_full[acc]), acc_phase, gave_up))) break;
+                    tc_fence_after();
+                    const uint32_t d = tmem + ((uint32_t)quarter << 21) + acc * kTileCols + half * kHalf;
+                    for (int g = kGroups; g >= 0; --g) {  // the corrections first
+                        uint32_t raw[32];
+                        tmem_load32(d + g * BN, raw);
+                        tmem_wait();
+#pragma unroll
+                        for (int q = 0; q < (LONG ? 32 : 0); ++q) total[q] += __uint_as_float(raw[q]);
+                    }
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(smem_u32(&sm.acc_empty[acc]));
+                    acc ^= 1;
+                    if (acc == 0) acc_phase ^= 1;
+                }
+                if (!ok) break;
+            }
+            const int parts = (int)min((int64_t)kGroups, (r1 - r0 + kGroup * kBR - 1) / (kGroup * kBR));
             if (!(ok = mbar_wait(smem_u32(&sm.acc_full[acc]), acc_phase, gave_up))) break;
             tc_fence_after();
             if (i0 < p.M) {
@@ -237,6 +279,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                         for (int q = 0; q < 32; ++q) v[q] += __uint_as_float(raw[q]);
                     }
+#pragma unroll
+                    for (int q = 0; q < (LONG ? 32 : 0); ++q) v[q] += total[q];
                     ok = columns32<T, EPI>(p, tl, maps, o, row, v, i0, j0, j, j + 32 < j_end ? j + 32 : p.N, split, lane,
                                            gave_up);
                 }
@@ -261,7 +305,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (warp == 1) tmem_free(tmem, 2 * kTileCols);
 }
 
-template <typename T, int EPI, int BN>
+template <typename T, int EPI, int BN, bool LONG = false>
 void run(const Product& p, Tiles tl, cudaStream_t s) {
     OutMaps maps{};
     set_outputs(p, tl, maps);
@@ -282,15 +326,23 @@ void run(const Product& p, Tiles tl, cudaStream_t s) {
         tl.stage_bytes = a_bytes + b_bytes;
         bytes = share_memory(p, tl, kEpiWarps, 0, 2, kMaxStages);
     }
-    allow_shared<k_product_tcv<T, EPI, BN>>(kBlockBytes + 1024);
+    allow_shared<k_product_tcv<T, EPI, BN, LONG>>(kBlockBytes + 1024);
     note_launches(1);
-    k_product_tcv<T, EPI, BN><<<grid, kThreads, bytes, s>>>(
+    k_product_tcv<T, EPI, BN, LONG><<<grid, kThreads, bytes, s>>>(
         p, tl, maps, vectors<T>(p.A, p.lda, p.a_mn ? p.R : p.M), vectors<T>(p.B, p.ldb, p.b_mn ? p.R : p.N));
     OPS_CK(cudaGetLastError());
 }
 
+// The length of the reduction that one tile makes.
+int64_t reduction(const Product& p) { return p.epi == kEpiSlab ? std::min(p.R, p.split_len) : p.R; }
+// 32-bit reductions longer than the accumulators of a tile of 64 columns take.
+bool in_passes(const Product& p) { return p.dtype == MSPLAT_DTYPE_F32 && reduction(p) > 3 * kGroup * kBR; }
+
 template <typename T, int EPI>
 void sized(const Product& p, const Tiles& tl, cudaStream_t s) {
+    if constexpr (sizeof(T) == 4) {
+        if (in_passes(p)) return run<T, EPI, 64, true>(p, tl, s);
+    }
     if (tl.bn == 64)
         run<T, EPI, 64>(p, tl, s);
     else
@@ -311,8 +363,7 @@ void typed(const Product& p, const Tiles& tl, cudaStream_t s) {
 // one accumulator's share needs (for 32-bit results).
 int columns_tcv(const Product& p) {
     const bool exact = p.dtype == MSPLAT_DTYPE_F32;
-    const int64_t len = p.epi == kEpiSlab ? std::min(p.R, p.split_len) : p.R;
-    return tile_columns(p, exact && len > kGroup * kBR ? 64 : 128);
+    return tile_columns(p, exact && reduction(p) > kGroup * kBR ? 64 : 128);
 }
 
 }  // namespace
@@ -320,7 +371,7 @@ int columns_tcv(const Product& p) {
 unsigned gave_up_tcv(cudaStream_t s) { return count_gave_up(s); }
 void give_up_tcv(cudaStream_t s) { launch_give_up(s); }
 
-int64_t stats_blocks_tcv(const Product& p) { return stats_blocks_of(p, columns_tcv(p)); }
+int64_t stats_blocks_tcv(const Product& p) { return in_passes(p) ? 2 * ceil_div(p.N, 64) : stats_blocks_of(p, columns_tcv(p)); }
 
 void launch_product_tcv(const Product& p, cudaStream_t s) {
     Tiles tl{};

@@ -122,3 +122,50 @@ def test_linear_gradients_keep_32_bits(m, n, k):
     for wrong in (torch.zeros_like(want), yd[:m // 2].T @ xd[:m // 2], dy.bfloat16().double().T @ x.bfloat16().double()):
         with pytest.raises(AssertionError):
             R.check(wrong, want, bound, "dw")
+
+
+def positive(seed, rows, cols):
+    return normal(seed, rows, cols, "f32").abs()
+
+
+def one_sign_bound(k, want):
+    """How far a sum of k positive 32-bit products may be: 512 of them are added 16 at a time in one accumulator, each
+    addition rounded towards zero (32 steps of 2^-23); the five smaller products of a split factor's parts, 2^-7 of the whole
+    together, 1536 at a time (480 steps of that); the accumulators in 32 bits, half a step each, and eight more."""
+    return want * (32 * 2.0 ** -23 + 480 * 2.0 ** -23 * 2.0 ** -7 + (k / 512 + 8) * 2.0 ** -24)
+
+
+@pytest.mark.parametrize("m,n,k", [(300, 200, 1536), (300, 200, 1537), (40, 9, 3100), (300, 200, 4096), (130, 70, 16_384),
+                                   (20_000, 66, 1800), (5000, 500, 2100)])
+@pytest.mark.parametrize("pad", (0, 3))
+def test_linear_long_reductions_of_one_sign(m, n, k, pad):
+    """32-bit sums of one sign, where truncating accumulators lose the same way at every step."""
+    x, w = positive(330, m, k + pad)[:, pad:], positive(331, n, k + pad)[:, pad:]
+    res, z = normal(332, m, n, "f32"), torch.empty(m, n, device="cuda")
+    y = ops().linear_forward(x, w, residual=res, preact=z)
+    want = x.double() @ w.double().T
+    R.check(z, want, one_sign_bound(k, want), "preact")
+    R.check(y, want + res.double(), one_sign_bound(k, want) + 2.0 ** -24 * (want + res.double()).abs(), "y")
+
+
+def test_linear_gradients_long_reductions_of_one_sign():
+    """dx over many outputs, and dw over rows in few pieces (a result of 32 MB leaves room for eight)."""
+    m, n, k = 32_768, 2048, 4096
+    x, dy, w = positive(333, m, k), positive(334, m, n), positive(335, n, k)
+    dx, dw, _ = ops().linear_backward(x, w, dy)
+    rows = torch.arange(0, m, 37, device="cuda")
+    want = dy[rows].double() @ w.double()
+    R.check(dx[rows], want, one_sign_bound(n, want), "dx")
+    cols = torch.arange(0, n, 7, device="cuda")
+    want = dy[:, cols].double().T @ x.double()
+    R.check(dw[cols], want, one_sign_bound(m, want), "dw")
+
+
+@pytest.mark.parametrize("m,v,d", [(300, 500, 1600), (20_000, 70, 2000), (40, 3000, 5000)])
+def test_loss_of_long_rows(m, v, d):
+    x, w = normal(336, m, d, "f32"), normal(337, v, d, "f32", std=d ** -0.5)
+    targets = labels(338, m, v)
+    got = ops().loss_cross_entropy(x, w, targets, weight=64.0)
+    want = R.loss(x, w, targets, 1.0, 64.0, torch.float32)
+    for a, name in zip(got, ("loss", "row_loss", "dx", "dw")):
+        R.check(a, *want[name], name)
