@@ -73,9 +73,11 @@ void check_workspace(const Arena& a, void* workspace, uint64_t bytes) {
 }
 
 // Pieces of a long reduction of an M x N result: enough tiles for every SM, in
-// pieces of at least 512. The tensor cores truncate when they add, so 32-bit
-// results take pieces of at most 1024 (whose sums are added with rounding) as
-// long as the pieces take no more than kSlabBytes.
+// pieces of at least 512. The tensor cores truncate when they add, so the pieces,
+// whose sums are added with rounding, are no longer than a type's rounding asks
+// for as long as they take no more than kSlabBytes: 1024 for 32 bits, 32768 for 16
+// (and four times the bytes, since such a piece has so much more to do), whose
+// one-signed sums are then off by 2e-4, less than half of half a step of f16.
 constexpr int64_t kSlabBytes = 256ll << 20;
 struct Split {
     int splits;
@@ -96,7 +98,8 @@ Split plan_split(int64_t M, int64_t N, int64_t R, int dtype) {
             s = q;
         }
     }
-    if (exact) s = std::max(s, std::min(ceil_div(R, 1024), std::max<int64_t>(1, kSlabBytes / (M * N * 4))));
+    const int64_t room = (exact ? kSlabBytes : 4 * kSlabBytes) / (M * N * 4);
+    s = std::max(s, std::min(ceil_div(R, exact ? 1024 : 32768), std::max<int64_t>(1, room)));
     const int64_t len = round_up(ceil_div(R, s), 64);
     return {(int)ceil_div(R, len), len};
 }

@@ -169,3 +169,21 @@ def test_loss_of_long_rows(m, v, d):
     want = R.loss(x, w, targets, 1.0, 64.0, torch.float32)
     for a, name in zip(got, ("loss", "row_loss", "dx", "dw")):
         R.check(a, *want[name], name)
+
+
+@pytest.mark.parametrize("t", ("f16", "bf16"))
+def test_linear_gradients_of_a_million_rows_and_one_sign(t):
+    """A 16-bit dw large enough for few pieces of its rows: half a step of the type, and what truncation takes from at most
+    32768 products, 16 at a time (2048 steps of 2^-23)."""
+    m, n, k = 1_000_000, 2048, 2048
+    x, dy = (torch.empty(m, k, dtype=R.TYPES[t], device="cuda") for _ in range(2))
+    g = torch.Generator(device="cuda").manual_seed(340)
+    x.uniform_(0.25, 1.75, generator=g)
+    dy.uniform_(0.25 / 2 ** 10, 1.75 / 2 ** 10, generator=g)  # sums of about 1000
+    _, dw, _ = ops().linear_backward(x, torch.zeros(n, k, dtype=x.dtype, device="cuda"), dy, need_dx=False, need_dbias=False)
+    some = torch.arange(0, n, 129, device="cuda")
+    want = sum(a[:, some].double().T @ b.double() for a, b in zip(dy.split(125_000), x.split(125_000)))
+    off = want * (2048 * 2.0 ** -23 + 64 * 2.0 ** -24)
+    R.check(dw[some], want, off + R.rounded(want + off, dw.dtype), "dw")
+    del x, dy
+    torch.cuda.empty_cache()
