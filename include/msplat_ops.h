@@ -18,7 +18,10 @@
  * wider record. dtype is the element type of every matrix and vector of a
  * call unless its comment says otherwise. Sums, softmax statistics and
  * activations are evaluated in 32 bits (matrix products of MSPLAT_DTYPE_F32
- * keep all 24 bits of both factors) and rounded once into the output's type.
+ * keep all 24 bits of both factors) and rounded once into the output's type. The
+ * tensor cores truncate where they add: sums of products of one sign are off by at
+ * most 2e-6 of themselves for MSPLAT_DTYPE_F32, and for the 16-bit types by 3e-5
+ * (MSPLAT_DTYPE_F32 outputs, logits) or 2e-4 (the others), however long they are.
  * Infinities and NaN act as in the formulas, except that an infinite factor of
  * MSPLAT_DTYPE_F32 may give NaN in place of an infinity beside a factor of 256 or
  * more, or below 2^-126, in size; MSPLAT_DTYPE_F32 factors below 1e-30 may lose

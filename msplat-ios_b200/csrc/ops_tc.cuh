@@ -142,7 +142,33 @@ __device__ __forceinline__ void tmem_load32(uint32_t addr, uint32_t (&r)[32]) {
           "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
         : "r"(addr));
 }
+__device__ __forceinline__ void tmem_store32(uint32_t addr, const uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};"
+        ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+        "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+        "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(addr)
+        : "memory");
+    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
 __device__ __forceinline__ void tmem_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+
+// Adds 32 columns of an accumulator, with rounding, to (or first puts them in) sums
+// that the warp keeps in TMEM.
+__device__ __forceinline__ void tmem_sum32(uint32_t acc, uint32_t sums, bool add) {
+    uint32_t v[32], w[32];
+    tmem_load32(acc, v);
+    if (add) tmem_load32(sums, w);
+    tmem_wait();
+    if (add) {
+#pragma unroll
+        for (int q = 0; q < 32; ++q) v[q] = __float_as_uint(__uint_as_float(v[q]) + __uint_as_float(w[q]));
+    }
+    tmem_store32(sums, v);
+}
 
 // Shared-memory operand descriptor, 128-byte swizzle. Rows of 128 bytes in
 // groups of eight (1024 bytes). Reduction contiguous: a row is one i, the
@@ -191,6 +217,7 @@ struct Tiles {
     int stages, stage_bytes;
     uint32_t idesc;
     int resident;        // stages of B that stay in shared memory (ops_tcv.cu)
+    int pass;            // stages of a pass through the accumulators, 0: all in one (ops_tc16.cu)
     // the outputs' boxes in shared memory
     int tma_out;         // they move by TMA (16-byte aligned outputs), else element by element
     int ring;            // boxes per output and warp, 1 or 2
@@ -550,6 +577,17 @@ __device__ __forceinline__ bool columns32(const Product& p, const Tiles& tl, con
 template <int EPI>
 __device__ __forceinline__ void row_end(const Product& p, const RowState& r, int64_t block) {
     if (EPI == kEpiStats && r.in) p.stats[block * p.stats_ld + r.i] = make_float2(r.top, r.sum);
+}
+
+// The length of the reduction that one tile makes.
+inline int64_t reduction(const Product& p) { return p.epi == kEpiSlab ? std::min(p.R, p.split_len) : p.R; }
+// How much of a reduction of 16-bit factors goes through the accumulators before
+// their sum is added with rounding. They truncate: of sums of one sign they take
+// (bf16 / f16) 1.1e-5 / 2.5e-5 after 4096 elements, 1.6e-4 / 2e-4 after 32768, 3e-3
+// after 524288. A 16-bit result's half step is 3.9e-3 / 4.9e-4; 32-bit results
+// and logits get the shorter pass.
+inline int64_t pass_length16(const Product& p) {
+    return p.epi == kEpiSlab || (p.epi == kEpiLinear && p.out_dtype == p.dtype) ? 32768 : 4096;
 }
 
 // Columns of a tile: the widest that still gives three SMs of four one, and for the

@@ -36,7 +36,13 @@ struct Smem {
 };
 static_assert(offsetof(Smem, bias) % 16 == 0 && sizeof(Smem) <= 2048, "read as float4; share_memory counts 2048");
 
-template <typename T, int EPI>
+// LONG: a reduction longer than pass_length16 goes through the accumulators in
+// passes, whose sums the ends keep in the TMEM behind them: tiles of 128 columns with
+// two accumulators, or of 256 with one (8192 x 8192 -> 4096 bf16 into f32 takes
+// 423 us so, 546 in tiles of 128, and 410 in one pass with three times the error). A
+// kernel of its own: tests for passes took 11% of 1M x 64 -> 64 and 4% of the wide
+// layer.
+template <typename T, int EPI, bool LONG>
 __global__ void __launch_bounds__(kThreads, 1)
     k_product_tc16(const __grid_constant__ Product p, const __grid_constant__ Tiles tl,
                    const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
@@ -46,7 +52,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     uint8_t* tiles = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(dyn) + 1023) & ~(uintptr_t)1023);
     uint8_t* boxes = tiles + (size_t)tl.stages * tl.stage_bytes;
-    const uint32_t tmem_cols = 2 * tl.bn;
+    const uint32_t tmem_cols = LONG ? 512 : 2 * tl.bn;
 
     if (threadIdx.x == 0) {
         for (int q = 0; q < tl.stages; ++q) {
@@ -69,6 +75,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     tc_fence_after();
     const uint32_t tmem = sm.tmem;
     volatile int* gave_up = &sm.gave_up;
+    // to the next accumulator
+    auto next = [&](int& acc, uint32_t& acc_phase) {
+        const bool one = LONG && tl.bn == 256;
+        if (!one) acc ^= 1;
+        if (acc == 0) acc_phase ^= 1;
+    };
 
     if (warp == 0) {
         if (elect_one()) {
@@ -126,8 +138,18 @@ __global__ void __launch_bounds__(kThreads, 1)
             tile_of(p, tl, w, tm, tn, split, r0, r1);
             if (!(ok = mbar_wait(smem_u32(&sm.acc_empty[acc]), acc_phase ^ 1, gave_up))) break;
             tc_fence_after();
-            const uint32_t d = tmem + acc * tl.bn;
-            for (int64_t r = r0; r < r1; r += kBR) {
+            uint32_t d = tmem + acc * tl.bn;
+            int block = 0;
+            for (int64_t r = r0; r < r1; r += kBR, ++block) {
+                if (LONG && block == tl.pass) {
+                    if (elect_one()) tc_commit(smem_u32(&sm.acc_full[acc]));
+                    __syncwarp();
+                    next(acc, acc_phase);
+                    if (!(ok = mbar_wait(smem_u32(&sm.acc_empty[acc]), acc_phase ^ 1, gave_up))) break;
+                    tc_fence_after();
+                    d = tmem + acc * tl.bn;
+                    block = 0;
+                }
                 if (!(ok = mbar_wait(smem_u32(&sm.full[stage]), phase, gave_up))) break;
                 tc_fence_after();
                 if (elect_one()) {
@@ -136,7 +158,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     const uint32_t step_a = p.a_mn ? 2048 >> 4 : 32 >> 4, step_b = p.b_mn ? 2048 >> 4 : 32 >> 4;
 #pragma unroll
                     for (int k = 0; k < kBR / 16; ++k)
-                        tc_mma(d, da + k * step_a, db + k * step_b, tl.idesc, r > r0 || k > 0);
+                        tc_mma(d, da + k * step_a, db + k * step_b, tl.idesc, (LONG ? block > 0 : r > r0) || k > 0);
                     tc_commit(smem_u32(&sm.empty[stage]));
                 }
                 __syncwarp();
@@ -148,8 +170,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (!ok) break;
             if (elect_one()) tc_commit(smem_u32(&sm.acc_full[acc]));
             __syncwarp();
-            acc ^= 1;
-            if (acc == 0) acc_phase ^= 1;
+            next(acc, acc_phase);
         }
         if (!ok) {
             // products in flight must end before the block frees TMEM
@@ -177,8 +198,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         bool ok = true;
         for (int w = blockIdx.x; w < tl.total && ok; w += gridDim.x) {
             if (by_tile && acc != group) {
-                acc ^= 1;
-                if (acc == 0) acc_phase ^= 1;
+                next(acc, acc_phase);
                 continue;
             }
             int tm, tn, split;
@@ -188,6 +208,20 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int64_t j_end = min(p.N, j0 + columns);
             RowState row = row_begin<EPI>(p, i0, lane);
             if (EPI == kEpiLinear && j0 < j_end) fetch_residual(p, tl, maps, o, i0, j0, lane);
+            // the sums of all passes but the last
+            const uint32_t sums = tmem + ((uint32_t)quarter << 21) + 256 + half * columns;
+            bool summed = false;
+            for (; LONG && r1 - r0 > tl.pass * kBR; r0 += tl.pass * kBR, summed = true) {
+                if (!(ok = mbar_wait(smem_u32(&sm.acc_full[acc]), acc_phase, gave_up))) break;
+                tc_fence_after();
+                const uint32_t d = tmem + ((uint32_t)quarter << 21) + acc * tl.bn + half * columns;
+                for (int c = 0; c < columns; c += 32) tmem_sum32(d + c, sums + c, summed);
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&sm.acc_empty[acc]));
+                next(acc, acc_phase);
+            }
+            if (LONG && !ok) break;
             if (!(ok = mbar_wait(smem_u32(&sm.acc_full[acc]), acc_phase, gave_up))) break;
             tc_fence_after();
             if (i0 < p.M) {
@@ -199,6 +233,12 @@ __global__ void __launch_bounds__(kThreads, 1)
                     float v[32];
 #pragma unroll
                     for (int q = 0; q < 32; ++q) v[q] = __uint_as_float(raw[q]);
+                    if (LONG && summed) {
+                        tmem_load32(sums + (uint32_t)(j - j0), raw);
+                        tmem_wait();
+#pragma unroll
+                        for (int q = 0; q < 32; ++q) v[q] += __uint_as_float(raw[q]);
+                    }
                     ok = columns32<T, EPI>(p, tl, maps, o, row, v, i0, j0, j, j + 32 < j_end ? j + 32 : p.N, split, lane,
                                            gave_up);
                 }
@@ -207,8 +247,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&sm.acc_empty[acc]));
-            acc ^= 1;
-            if (acc == 0) acc_phase ^= 1;
+            next(acc, acc_phase);
         }
         if (EPI != kEpiStats && lane == 0) {
             bulk_wait_all();
@@ -242,12 +281,16 @@ struct Maps {
     OutMaps out;
 };
 
+template <typename T, int EPI, bool LONG>
+void run_as(const Product& p, const Tiles& tl, const Maps& m, int bytes, cudaStream_t s) {
+    allow_shared<k_product_tc16<T, EPI, LONG>>(kBlockBytes + 1024);
+    note_launches(1);
+    k_product_tc16<T, EPI, LONG><<<std::min(tl.total, kSMs), kThreads, bytes, s>>>(p, tl, m.a, m.b, m.out);
+    OPS_CK(cudaGetLastError());
+}
 template <typename T, int EPI>
 void run(const Product& p, const Tiles& tl, const Maps& m, int bytes, cudaStream_t s) {
-    allow_shared<k_product_tc16<T, EPI>>(kBlockBytes + 1024);
-    note_launches(1);
-    k_product_tc16<T, EPI><<<std::min(tl.total, kSMs), kThreads, bytes, s>>>(p, tl, m.a, m.b, m.out);
-    OPS_CK(cudaGetLastError());
+    tl.pass ? run_as<T, EPI, true>(p, tl, m, bytes, s) : run_as<T, EPI, false>(p, tl, m, bytes, s);
 }
 
 template <typename T>
@@ -307,11 +350,14 @@ bool can_product_tc16(const Product& p) {
            tma_ready(p.B, p.ldb, p.b_mn ? p.R : p.N, 2);
 }
 
-int64_t stats_blocks_tc16(const Product& p) { return stats_blocks_of(p, tile_columns(p, 256)); }
+static bool in_passes(const Product& p) { return reduction(p) > pass_length16(p); }
+static int columns_tc16(const Product& p) { return std::max(in_passes(p) ? 128 : 64, tile_columns(p, 256)); }
+int64_t stats_blocks_tc16(const Product& p) { return stats_blocks_of(p, columns_tc16(p)); }
 
 void launch_product_tc16(const Product& p, cudaStream_t s) {
     Tiles tl{};
-    tl.bn = tile_columns(p, 256);
+    tl.bn = columns_tc16(p);
+    tl.pass = in_passes(p) ? (int)(pass_length16(p) / kBR) : 0;
     set_tiles(p, tl);
     tl.stage_bytes = (kBM + tl.bn) * 128;
     tl.idesc = instr_desc(p.dtype == MSPLAT_DTYPE_BF16, p.a_mn, p.b_mn, tl.bn);

@@ -13,7 +13,8 @@
 // ends, after three of them already where the reduction is longer (LONG: 16384
 // elements of one sign are off by 1e-6 of their sum, with the last accumulator
 // taking all the rest they were off by 7e-5; 8192 x 2048 -> 1024 takes 350 us, 348
-// without). 16-bit reductions beyond the accumulators stay in the last one.
+// without). 16-bit reductions take passes where pass_length16 says so, and stay in the
+// last accumulator before.
 //
 // A block owns 128 x bn tiles (bn 64 or 128) and walks its share of them. Warps
 // 12-19 load, split and store the stages (the layout is TMA's 128-byte swizzle,
@@ -53,9 +54,11 @@ struct Smem {
 };
 static_assert(offsetof(Smem, bias) % 16 == 0 && sizeof(Smem) <= 2048, "read as float4; share_memory counts 2048");
 
-// LONG (32-bit factors, 64 columns): a reduction longer than a tile's accumulators
-// take goes through them in passes; the two groups of warps then take half of a
-// tile's columns each.
+// LONG: a reduction longer than a tile's accumulators take (16 bits: than
+// pass_length16) goes through them in passes. 32 bits (64 columns): the two groups
+// of warps take half of a tile's columns each and hold the passes' sums in
+// registers; 16 bits (128 columns): in the columns of TMEM that one accumulator per
+// tile leaves.
 template <typename T, int EPI, int BN, bool LONG>
 __global__ void __launch_bounds__(kThreads, 1)
     k_product_tcv(const __grid_constant__ Product p, const __grid_constant__ Tiles tl,
@@ -63,10 +66,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     constexpr int P = planes<T>();
     constexpr int kA = P * kBM * 128, kB = P * BN * 128;
     // accumulators of one tile: the groups' and, for split factors, the corrections'
-    constexpr int kGroups = 512 / 2 / BN - (P > 1 ? 1 : 0);
+    constexpr bool kInTmem = LONG && P == 1;
+    constexpr int kGroups = kInTmem ? 1 : 512 / 2 / BN - (P > 1 ? 1 : 0);
     constexpr int kTileCols = 256;
-    constexpr int kPass = kGroups * kGroup;  // stages of a pass
-    static_assert(!LONG || (P > 1 && BN == 64), "passes are for what needs them");
+    constexpr int kPass = kInTmem ? 4096 / kBR : kGroups * kGroup;  // stages of a pass
+    static_assert(!LONG || BN == (P > 1 ? 64 : 128), "32 columns per thread are held, boxes of 16 bits have 64");
     // tiles of 64 columns: the two groups of warps take every other tile; wider
     // ones and passes: each takes half of the columns
     constexpr bool kByTile = BN == 64 && !LONG;
@@ -232,20 +236,26 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int64_t j_end = min(p.N, j0 + kHalf);
             RowState row = row_begin<EPI>(p, i0, lane);
             if (EPI == kEpiLinear && j0 < j_end) fetch_residual(p, tl, maps, o, i0, j0, lane);
-            float total[LONG ? 32 : 1];
+            float total[LONG && !kInTmem ? 32 : 1];
+            const uint32_t sums = tmem + ((uint32_t)quarter << 21) + BN + half * kHalf;  // (kInTmem)
+            bool summed = false;
             if (LONG) {  // all passes but the last
 #pragma unroll
-                for (int q = 0; q < (LONG ? 32 : 0); ++q) total[q] = 0.f;
-                for (; r1 - r0 > kPass * kBR; r0 += kPass * kBR) {
+                for (int q = 0; q < (LONG && !kInTmem ? 32 : 0); ++q) total[q] = 0.f;
+                for (; r1 - r0 > kPass * kBR; r0 += kPass * kBR, summed = true) {
                     if (!(ok = mbar_wait(smem_u32(&sm.acc_full[acc]), acc_phase, gave_up))) break;
                     tc_fence_after();
                     const uint32_t d = tmem + ((uint32_t)quarter << 21) + acc * kTileCols + half * kHalf;
-                    for (int g = kGroups; g >= 0; --g) {  // the corrections first
-                        uint32_t raw[32];
-                        tmem_load32(d + g * BN, raw);
-                        tmem_wait();
+                    if constexpr (kInTmem) {
+                        for (int c = 0; c < kHalf; c += 32) tmem_sum32(d + c, sums + c, summed);
+                    } else {
+                        for (int g = kGroups; g >= 0; --g) {  // (the corrections first)
+                            uint32_t raw[32];
+                            tmem_load32(d + g * BN, raw);
+                            tmem_wait();
 #pragma unroll
-                        for (int q = 0; q < (LONG ? 32 : 0); ++q) total[q] += __uint_as_float(raw[q]);
+                            for (int q = 0; q < (LONG && !kInTmem ? 32 : 0); ++q) total[q] += __uint_as_float(raw[q]);
+                        }
                     }
                     tc_fence_before();
                     __syncwarp();
@@ -280,7 +290,13 @@ __global__ void __launch_bounds__(kThreads, 1)
                         for (int q = 0; q < 32; ++q) v[q] += __uint_as_float(raw[q]);
                     }
 #pragma unroll
-                    for (int q = 0; q < (LONG ? 32 : 0); ++q) v[q] += total[q];
+                    for (int q = 0; q < (LONG && !kInTmem ? 32 : 0); ++q) v[q] += total[q];
+                    if (kInTmem && summed) {
+                        tmem_load32(sums + c, raw);
+                        tmem_wait();
+#pragma unroll
+                        for (int q = 0; q < 32; ++q) v[q] += __uint_as_float(raw[q]);
+                    }
                     ok = columns32<T, EPI>(p, tl, maps, o, row, v, i0, j0, j, j + 32 < j_end ? j + 32 : p.N, split, lane,
                                            gave_up);
                 }
@@ -333,16 +349,15 @@ void run(const Product& p, Tiles tl, cudaStream_t s) {
     OPS_CK(cudaGetLastError());
 }
 
-// The length of the reduction that one tile makes.
-int64_t reduction(const Product& p) { return p.epi == kEpiSlab ? std::min(p.R, p.split_len) : p.R; }
-// 32-bit reductions longer than the accumulators of a tile of 64 columns take.
-bool in_passes(const Product& p) { return p.dtype == MSPLAT_DTYPE_F32 && reduction(p) > 3 * kGroup * kBR; }
+// 32-bit reductions longer than the accumulators of a tile of 64 columns take,
+// and 16-bit ones longer than a pass may be.
+bool in_passes(const Product& p) {
+    return reduction(p) > (p.dtype == MSPLAT_DTYPE_F32 ? 3 * kGroup * kBR : pass_length16(p));
+}
 
 template <typename T, int EPI>
 void sized(const Product& p, const Tiles& tl, cudaStream_t s) {
-    if constexpr (sizeof(T) == 4) {
-        if (in_passes(p)) return run<T, EPI, 64, true>(p, tl, s);
-    }
+    if (in_passes(p)) return run<T, EPI, sizeof(T) == 4 ? 64 : 128, true>(p, tl, s);
     if (tl.bn == 64)
         run<T, EPI, 64>(p, tl, s);
     else
@@ -363,6 +378,7 @@ void typed(const Product& p, const Tiles& tl, cudaStream_t s) {
 // one accumulator's share needs (for 32-bit results).
 int columns_tcv(const Product& p) {
     const bool exact = p.dtype == MSPLAT_DTYPE_F32;
+    if (in_passes(p)) return exact ? 64 : 128;
     return tile_columns(p, exact && reduction(p) > kGroup * kBR ? 64 : 128);
 }
 
@@ -371,7 +387,7 @@ int columns_tcv(const Product& p) {
 unsigned gave_up_tcv(cudaStream_t s) { return count_gave_up(s); }
 void give_up_tcv(cudaStream_t s) { launch_give_up(s); }
 
-int64_t stats_blocks_tcv(const Product& p) { return in_passes(p) ? 2 * ceil_div(p.N, 64) : stats_blocks_of(p, columns_tcv(p)); }
+int64_t stats_blocks_tcv(const Product& p) { return in_passes(p) ? 2 * ceil_div(p.N, columns_tcv(p)) : stats_blocks_of(p, columns_tcv(p)); }
 
 void launch_product_tcv(const Product& p, cudaStream_t s) {
     Tiles tl{};

@@ -187,3 +187,40 @@ def test_linear_gradients_of_a_million_rows_and_one_sign(t):
     R.check(dw[some], want, off + R.rounded(want + off, dw.dtype), "dw")
     del x, dy
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("t", ("f16", "bf16"))
+@pytest.mark.parametrize("out", ("same", "f32"))
+@pytest.mark.parametrize("m,n,k", [(130, 70, 4097), (300, 300, 20_000), (40, 130, 32_769), (200, 150, 40_000),
+                                   (9, 20, 140_001), (20_000, 260, 5000)])
+@pytest.mark.parametrize("pad", (0, 8, 3))
+def test_linear_16_bit_long_reductions_of_one_sign(m, n, k, pad, out, t):
+    """Half a step of the result's type, and what truncation takes from the products of one pass, 16 at a time: 4096 for 32-bit
+    results (256 steps of 2^-23, and as many again, since f16 products are cut too), 32768 for 16-bit ones; passes in 32 bits."""
+    g = torch.Generator(device="cuda").manual_seed(350)
+    x = torch.empty(m, k + pad, dtype=R.TYPES[t], device="cuda").uniform_(0.25, 1.75, generator=g)[:, pad:]
+    w = (torch.empty(n, k + pad, device="cuda").uniform_(0.25, 1.75, generator=g) / k).to(R.TYPES[t])[:, pad:]
+    out_t = torch.float32 if out == "f32" else R.TYPES[t]
+    w = w * 64 if t == "f16" else w  # not below f16's normal numbers
+    w = torch.nn.functional.pad(w, (pad, 0))[:, pad:]
+    z = torch.empty(m, n, dtype=out_t, device="cuda")
+    res = torch.full((m, n), -1.0, dtype=out_t, device="cuda")
+    y = ops().linear_forward(x, w, residual=res, preact=z, out_dtype=out_t)
+    want = torch.cat([a.double() @ w.double().T for a in x.split(2000)])
+    length = 4096 if out == "f32" else 32_768
+    off = want * (2 * length / 16 * 2.0 ** -23 + (k / length + 2) * 2.0 ** -24)
+    R.check(z, want, off + R.rounded(want + off, out_t), "preact")
+    off = off + 2.0 ** -24 * (want - 1).abs()
+    R.check(y, want - 1, off + R.rounded((want - 1).abs() + off, out_t), "y")
+
+
+@pytest.mark.parametrize("t", ("f16", "bf16"))
+@pytest.mark.parametrize("m,v,d", [(300, 300, 4200), (100, 1000, 9000)])
+@pytest.mark.parametrize("pad", (0, 3))
+def test_loss_16_bit_of_long_rows(m, v, d, pad, t):
+    x, w = normal(351, m, d, t, pad=pad, lead=pad), normal(352, v, d, t, std=d ** -0.5, pad=pad, lead=pad)
+    targets = labels(353, m, v)
+    got = ops().loss_cross_entropy(x, w, targets, weight=64.0)
+    want = R.loss(x, w, targets, 1.0, 64.0, R.TYPES[t])
+    for a, name in zip(got, ("loss", "row_loss", "dx", "dw")):
+        R.check(a, *want[name], name)
