@@ -14,6 +14,7 @@ namespace ops {
 namespace {
 
 constexpr int kWarps = 4;
+constexpr int kSpan = 512;  // steps of a warp that one sum takes (LONG)
 
 template <typename T>
 __device__ __forceinline__ void unpack8(const T* g, float (&v)[16 / sizeof(T)]) {
@@ -32,7 +33,10 @@ __device__ __forceinline__ void unpack8(const T* g, float (&v)[16 / sizeof(T)]) 
     }
 }
 
-template <typename T, typename TO, int MT, bool VEC>
+// LONG: the sums start afresh after kSpan steps of the warp, and the rounded-off bits
+// of 32-bit sums of millions of products stay small. (A kernel of its own: the outer
+// loop takes 8 x 4096 -> 1024 f32 from 13 to 17 us.)
+template <typename T, typename TO, int MT, bool VEC, bool LONG>
 __global__ void __launch_bounds__(kWarps * 32) k_gemv(const __grid_constant__ Product p) {
     constexpr int E = VEC ? 16 / sizeof(T) : 1;
     const int lane = threadIdx.x % 32;
@@ -41,12 +45,21 @@ __global__ void __launch_bounds__(kWarps * 32) k_gemv(const __grid_constant__ Pr
     const int M = (int)p.M;
     const T* x = static_cast<const T*>(p.A);
     const T* w = static_cast<const T*>(p.B) + n * p.ldb;
-    float acc[MT];
+    float acc[MT], total[MT];
 #pragma unroll
-    for (int m = 0; m < MT; ++m) acc[m] = 0.f;
+    for (int m = 0; m < MT; ++m) acc[m] = total[m] = 0.f;
     const int64_t whole = VEC ? p.R / E * E : p.R;
+    int step = 0;
 #pragma unroll 2
     for (int64_t k = lane * E; k < whole; k += 32 * E) {
+        if (LONG && ++step == kSpan) {
+            step = 0;
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+                total[m] += acc[m];
+                acc[m] = 0.f;
+            }
+        }
         float b[E];
         if constexpr (VEC)
             unpack8<T>(w + k, b);
@@ -72,7 +85,7 @@ __global__ void __launch_bounds__(kWarps * 32) k_gemv(const __grid_constant__ Pr
     float mine = 0.f;
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
-        float s = acc[m];
+        float s = LONG ? total[m] + acc[m] : acc[m];
 #pragma unroll
         for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(~0u, s, o);
         mine = lane == m ? s : mine;
@@ -92,10 +105,11 @@ void run(const Product& p, cudaStream_t s) {
                      (p.M <= 1 || p.lda % E == 0) && (p.N <= 1 || p.ldb % E == 0);
     const unsigned grid = (unsigned)ceil_div(p.N, kWarps);
     note_launches(1);
-    if (vec)
-        k_gemv<T, TO, MT, true><<<grid, kWarps * 32, 0, s>>>(p);
+    auto go = [&](auto kernel) { kernel<<<grid, kWarps * 32, 0, s>>>(p); };
+    if (p.R > kSpan * 32 * (vec ? E : 1))
+        vec ? go(k_gemv<T, TO, MT, true, true>) : go(k_gemv<T, TO, MT, false, true>);
     else
-        k_gemv<T, TO, MT, false><<<grid, kWarps * 32, 0, s>>>(p);
+        vec ? go(k_gemv<T, TO, MT, true, false>) : go(k_gemv<T, TO, MT, false, false>);
     OPS_CK(cudaGetLastError());
 }
 

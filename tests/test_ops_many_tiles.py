@@ -224,3 +224,15 @@ def test_loss_16_bit_of_long_rows(m, v, d, pad, t):
     want = R.loss(x, w, targets, 1.0, 64.0, R.TYPES[t])
     for a, name in zip(got, ("loss", "row_loss", "dx", "dw")):
         R.check(a, *want[name], name)
+
+
+@pytest.mark.parametrize("lead", (0, 1))
+def test_linear_few_rows_of_many_inputs(lead):
+    """Two rows of 64 million equal inputs: a lane adds at most 4096 products (half a step each) before that sum is added to
+    the others."""
+    k = 1 << 26
+    x = torch.full((2, k + 4), 0.1, device="cuda")[:, lead:lead + k]
+    w = torch.full((3, k + 4), 0.7, device="cuda")[:, lead:lead + k]
+    y = ops().linear_forward(x, w)
+    want = torch.full((2, 3), k, dtype=torch.float64, device="cuda") * float(x[0, 0]) * float(w[0, 0])
+    R.check(y, want, want * (4096 + k / (512 * 32) + 8) * 2.0 ** -24, "y")
