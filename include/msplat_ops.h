@@ -1,8 +1,9 @@
 /*
  * msplat_ops.h — C ABI of the operators for learned per-Gaussian attributes.
  *
- * A scene may carry a learned feature vector per Gaussian. These operators
- * turn such features into what the training step reads or is trained on:
+ * A caller may keep a learned feature vector per Gaussian of a fixed set (the
+ * trainer's checkpoints and densification do not carry it). These operators turn
+ * such features into what the training step reads or is trained on:
  *   msplat_linear_*              fully connected layers, e.g. the [N,3] colours
  *                                that msplat_shard_forward_backward_rgb takes
  *                                and, from the colour columns of its gradient
@@ -10,7 +11,8 @@
  *   msplat_dropout               dropout, forward and backward
  *   msplat_loss_cross_entropy    a label loss with its gradients, beside
  *                                msplat_loss_ssim_noalloc
- * The weights they produce gradients for are updated with msplat_fused_adam.
+ * Weights of MSPLAT_DTYPE_F32 are updated from their gradients with
+ * msplat_fused_adam, which takes that type only.
  * None of them has a counterpart in the reference.
  *
  * Matrices are row-major device memory of the current device with a row
@@ -21,7 +23,7 @@
  * keep all 24 bits of both factors) and rounded once into the output's type. The
  * tensor cores truncate where they add: sums of products of one sign are off by at
  * most 2e-6 of themselves for MSPLAT_DTYPE_F32, and for the 16-bit types by 3e-5
- * (MSPLAT_DTYPE_F32 outputs, logits) or 2e-4 (the others), however long they are.
+ * (MSPLAT_DTYPE_F32 outputs, logits) or 2e-4 (the others), with up to 2^20 products.
  * Infinities and NaN act as in the formulas, except that an infinite factor of
  * MSPLAT_DTYPE_F32 may give NaN in place of an infinity beside a factor of 256 or
  * more, or below 2^-126, in size; MSPLAT_DTYPE_F32 factors below 1e-30 may lose
@@ -62,7 +64,8 @@ enum {
 
 /* z = x w^T + bias, y = act(z) + residual for x [m,k], w [n,k], bias [n] (may
  * be NULL), residual [m,n] (may be NULL) and y [m,n]; z is also written to
- * preact [m,n] when that is not NULL (msplat_linear_backward reads it).
+ * preact [m,n] when that is not NULL (msplat_linear_backward reads it, if y_dtype
+ * is dtype).
  * residual, preact and y have the type y_dtype: dtype, or MSPLAT_DTYPE_F32.
  * residual may be the same memory as y (then ldr == ldy). m may be 0; n and k
  * are at least 1, and m, n, k at most 2^30. Needs no workspace. */
@@ -73,8 +76,8 @@ int msplat_linear_forward(int64_t m, int64_t n, int64_t k, const void* x, int64_
 /* Gradients of msplat_linear_forward from dy = dL/dy [m,n]:
  * dz = dy act'(z), dx = dz w [m,k], dw = dz^T x [n,k], dbias = column sums of
  * dz [n]; dL/dresidual is dy itself. Each of dx, dw, dbias may be NULL.
- * preact is z as the forward wrote it; it is not read (may be NULL) for
- * MSPLAT_ACT_NONE. x may be NULL without dw, w without dx. dx, dw and dbias are
+ * preact is z as a forward with y_dtype = dtype wrote it; it is not read (may be
+ * NULL) for MSPLAT_ACT_NONE. x may be NULL without dw, w without dx. dx, dw and dbias are
  * overwritten, with zeros in dw and dbias when m is 0. Every matrix has the
  * type dtype; for the 16-bit types dz is rounded to dtype between the two
  * products. */

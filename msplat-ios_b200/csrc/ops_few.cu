@@ -192,7 +192,8 @@ void typed(const Product& p, cudaStream_t s) {
 // there: f32 16 -> 3 32 / 100, 64 -> 3 61 / 106, 256 -> 3 111 / 168, 64 -> 8
 // 75 / 102, 64 -> 16 141 / 106; f16 61 -> 3 unaligned 54 / 165; aligned bf16 16
 // -> 3 32 / 71, 16 -> 8 42 / 66, 64 -> 3 44 / 52, 64 -> 8 58 / 46, 256 -> 3 75
-// / 63. Few rows leave too few warps.
+// / 63. Few rows leave too few warps for long ones: f32 256 -> 3 takes 16 / 14 with
+// 1024 to 8192 rows and 23 / 29 with 65536, 64 -> 3 8 / 10 to 9 / 11, 16 -> 3 6 / 10.
 bool can_product_few(const Product& p) {
     if (p.epi != kEpiLinear || p.a_mn || p.b_mn || p.targets || p.alpha_dev || p.alpha != 1.f) return false;
     if (p.N > 8 || p.M < 4096 || p.R * outputs(p.N) * 4 > kMostWeights) return false;

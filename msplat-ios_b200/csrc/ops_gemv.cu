@@ -6,7 +6,8 @@
 // the rows of x beside it out of the L1 cache, and joins its 32 lanes' sums at
 // the end. No descriptors, no barriers. On the GPU, us here / in tiles of the
 // tensor cores: 1 x 512 -> 512 bf16 1.8 / 6.0, 8 rows 2.9 / 6.2, 8 x 1024 -> 4096 7.2
-// / 8.4, 8 x 4096 -> 1024 f32 13 / 81.
+// / 8.4, 8 x 4096 -> 1024 f32 13 / 81. With twice the rows (a build for 16) bf16
+// 9 x 512 -> 512 5.1 / 8.4 but 9 x 1024 -> 4096 14.3 / 10.4, f32 16.6 / 27.
 #include "ops.cuh"
 
 namespace msplat {

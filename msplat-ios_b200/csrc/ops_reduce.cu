@@ -9,6 +9,12 @@ namespace msplat {
 namespace ops {
 namespace {
 
+// dz of 16-bit types is rounded to the type, since it is a factor of two products
+// on the tensor cores: in two parts they would be twice as long (110 and 98 us for
+// the wide case below). Its rounding, independent from element to element, adds to
+// the output's: 0.0024 of the norm of dx and dw in bf16 where rounding the output
+// alone is 0.0017. The column sums add dz before it is rounded.
+//
 // A block takes a piece of the rows and up to 32 vectors of V columns (16 bytes
 // when the matrices are aligned, else one element); `lanes` threads (a power of
 // two) share a row. Bound by reading z and dy and writing dz: each thread has

@@ -23,9 +23,10 @@
 // for a tile's columns fit beside the stages (a layer's weights for many rows), a
 // block keeps to one column of tiles and loads them once (resident).
 //
-// 1M x 32 -> 64 f32 takes 117 us without and 168 with GELU and preact kept
-// (3.8 TB/s): issuing the split and the ends takes half of the slots, and two
-// stages are all that three parts leave room for.
+// 1M x 32 -> 64 f32 takes 117 us without and 179 with GELU and preact kept
+// (3.6 TB/s): issuing the split and the ends takes half of the slots, and two
+// stages are all that three parts leave room for; one where preact is kept, n is
+// above 64 and k in 65 .. 512 (96 KB a stage beside the outputs' boxes).
 #include <cstddef>
 
 #include "ops_load.cuh"

@@ -175,7 +175,8 @@ def linear_forward(x, w, bias=None, activation="none", residual=None, preact=Non
 
     activation: one of ACTIVATIONS. out_dtype: x's type (default) or float32,
     the type of residual, preact and the result. preact [m, n], when given,
-    receives the activation's argument, which linear_backward needs. out [m,
+    receives the activation's argument, which linear_backward needs (in x's type:
+    with out_dtype float32 and 16-bit x, convert preact and dy for it). out [m,
     n], when given, receives the result (it may be residual itself)."""
     L = _lib()
     dt = _dtype(x)
