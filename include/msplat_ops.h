@@ -22,7 +22,7 @@
  * activations are evaluated in 32 bits (matrix products of MSPLAT_DTYPE_F32
  * keep all 24 bits of both factors) and rounded once into the output's type. The
  * tensor cores truncate where they add: sums of products of one sign are off by at
- * most 2e-6 of themselves for MSPLAT_DTYPE_F32, and for the 16-bit types by 3e-5
+ * most 4e-6 of themselves for MSPLAT_DTYPE_F32, and for the 16-bit types by 3e-5
  * (MSPLAT_DTYPE_F32 outputs, logits) or 2e-4 (the others), with up to 2^20 products.
  * Infinities and NaN act as in the formulas, except that an infinite factor of
  * MSPLAT_DTYPE_F32 may give NaN in place of an infinity beside a factor of 256 or

@@ -91,12 +91,18 @@ __device__ __forceinline__ float2 exp2_rest(float2 b, float2 r) {
     const float2 e = make_float2(exp2_fast(b.x), exp2_fast(b.y));
     return __ffma2_rn(__fmul2_rn(e, r), both(-kLn2), e);
 }
-// min(|z|, 14), NaN for NaN
-__device__ __forceinline__ float size14(float z) {
+// The smaller and the larger of two, NaN for NaN.
+__device__ __forceinline__ float least(float a, float b) {
     float x;
-    asm("min.NaN.f32 %0, %1, %2;" : "=f"(x) : "f"(fabsf(z)), "f"(14.f));
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(x) : "f"(a), "f"(b));
     return x;
 }
+__device__ __forceinline__ float most(float a, float b) {
+    float x;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(x) : "f"(a), "f"(b));
+    return x;
+}
+__device__ __forceinline__ float size14(float z) { return least(fabsf(z), 14.f); }
 // x = size14(z): the distribution function of -x as tail * density
 __device__ __forceinline__ float2 normal_tail(float2 x, float2* density) {
     const float2 u = __ffma2_rn(x, both(0.4f * 0.70710678118654752f), both(1.f));
@@ -137,15 +143,15 @@ template <bool FULL>
 __device__ __forceinline__ float2 logistic(float2 z, float2* rest) {
     float2 e;
     if (FULL) {
-        const float2 x = make_float2(fminf(fmaxf(z.x, -88.f), 88.f), fminf(fmaxf(z.y, -88.f), 88.f));
+        const float2 x = make_float2(least(most(z.x, -88.f), 88.f), least(most(z.y, -88.f), 88.f));
         const float2 b = __fmul2_rn(x, both(-kLog2e));
         e = exp2_rest(b, __ffma2_rn(x, both(kLog2eRest), __ffma2_rn(x, both(kLog2e), b)));
     } else {
-        e = make_float2(fminf(exp2_fast(-kLog2e * z.x), 3e38f), fminf(exp2_fast(-kLog2e * z.y), 3e38f));
+        e = make_float2(least(exp2_fast(-kLog2e * z.x), 3e38f), least(exp2_fast(-kLog2e * z.y), 3e38f));
     }
     const float2 q = make_float2(recip_fast(1.f + e.x), recip_fast(1.f + e.y));
     *rest = __fmul2_rn(q, e);
-    return make_float2(z.x != z.x ? z.x : q.x, z.y != z.y ? z.y : q.y);
+    return q;
 }
 __device__ __forceinline__ float act_relu(float z) { return z < 0.f ? 0.f : z; }
 template <bool FULL>
@@ -169,12 +175,12 @@ __device__ __forceinline__ float2 act_sigmoid(float2 z) {
 }
 // act(z) for a result of type TO
 template <typename TO>
-__device__ __forceinline__ float activate(float z, int act) {
+__device__ __forceinline__ float2 activate(float2 z, int act) {
     constexpr bool FULL = sizeof(TO) == 4;
-    return act == MSPLAT_ACT_RELU      ? act_relu(z)
-           : act == MSPLAT_ACT_GELU    ? act_gelu<FULL>(both(z)).x
-           : act == MSPLAT_ACT_SILU    ? act_silu<FULL>(both(z)).x
-           : act == MSPLAT_ACT_SIGMOID ? act_sigmoid<FULL>(both(z)).x
+    return act == MSPLAT_ACT_RELU      ? make_float2(act_relu(z.x), act_relu(z.y))
+           : act == MSPLAT_ACT_GELU    ? act_gelu<FULL>(z)
+           : act == MSPLAT_ACT_SILU    ? act_silu<FULL>(z)
+           : act == MSPLAT_ACT_SIGMOID ? act_sigmoid<FULL>(z)
                                        : z;
 }
 // act'(z) for gradients of type T

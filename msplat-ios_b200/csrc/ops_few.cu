@@ -135,13 +135,16 @@ __global__ void __launch_bounds__(kThreads, 6) k_few(const __grid_constant__ Pro
         }
         if (i >= p.M) continue;
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
+        for (int n = 0; n < NT; n += 2) {
             if (n >= N) break;
-            const float z = acc[n] + bias[n];
-            if (p.preact) static_cast<TO*>(p.preact)[i * p.ldz + n] = from_f32<TO>(z);
-            float y = activate<TO>(z, p.act);
-            if (p.residual) y += to_f32(static_cast<const TO*>(p.residual)[i * p.ldr + n]);
-            static_cast<TO*>(p.out)[i * p.ldo + n] = from_f32<TO>(y);
+            const float2 z = make_float2(acc[n] + bias[n], acc[n + 1] + bias[n + 1]), y = activate<TO>(z, p.act);
+            auto put = [&](int q, float zq, float yq) {
+                if (p.preact) static_cast<TO*>(p.preact)[i * p.ldz + q] = from_f32<TO>(zq);
+                if (p.residual) yq += to_f32(static_cast<const TO*>(p.residual)[i * p.ldr + q]);
+                static_cast<TO*>(p.out)[i * p.ldo + q] = from_f32<TO>(yq);
+            };
+            put(n, z.x, y.x);
+            if (n + 1 < N) put(n + 1, z.y, y.y);
         }
     }
     asm volatile("cp.async.wait_all;" ::: "memory");

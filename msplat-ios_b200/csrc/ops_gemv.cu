@@ -94,7 +94,7 @@ __global__ void __launch_bounds__(kWarps * 32) k_gemv(const __grid_constant__ Pr
     if (lane >= M) return;
     const float z = mine + (p.bias ? to_f32(static_cast<const T*>(p.bias)[n]) : 0.f);
     if (p.preact) static_cast<TO*>(p.preact)[lane * p.ldz + n] = from_f32<TO>(z);
-    float y = activate<TO>(z, p.act);
+    float y = activate<TO>(both(z), p.act).x;
     if (p.residual) y += to_f32(static_cast<const TO*>(p.residual)[lane * p.ldr + n]);
     static_cast<TO*>(p.out)[lane * p.ldo + n] = from_f32<TO>(y);
 }

@@ -238,7 +238,7 @@ def test_inputs_freed_before_the_given_stream_has_read_them(op):
     torch.cuda.synchronize()
     side = torch.cuda.Stream()
     with torch.cuda.stream(side):
-        torch.cuda._sleep(50_000_000)  # some 25 ms
+        torch.cuda._sleep(1_000_000_000)  # some half a second
     got = getattr(o, op)(*args, **more, stream=side)
     held = [t for t in (*args, *more.values()) if isinstance(t, torch.Tensor)]
     sizes, at = [(t.shape, t.dtype) for t in held], {t.data_ptr() for t in held}
@@ -250,3 +250,28 @@ def test_inputs_freed_before_the_given_stream_has_read_them(op):
     want, got = ((v,) if isinstance(v, torch.Tensor) else v for v in (want, got))
     for a, b in zip(want, got):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("m", (1, 40, 5000))
+@pytest.mark.parametrize("act", ("relu", "gelu", "silu", "sigmoid"))
+def test_activations_of_what_is_not_finite(act, m, t):
+    """NaN stays NaN, at infinity the activations are their limits (silu at -inf may be NaN, as its formula is)."""
+    values = torch.tensor([float("nan"), float("inf"), float("-inf"), 1.0, -100.0, 100.0], dtype=R.TYPES[t], device="cuda")
+    one = torch.ones(1, 1, dtype=values.dtype, device="cuda")
+    if m == 1:
+        y = ops().linear_forward(one, values[:, None].contiguous(), activation=act)[0]
+    else:  # a column of inputs, the same values again and again
+        x = values.repeat(m // 6 + 1)[:m, None].contiguous()
+        y = ops().linear_forward(x, one, activation=act)[:6, 0]
+    y = y.double().tolist()
+    assert math.isnan(y[0])
+    assert y[1] == (1.0 if act == "sigmoid" else math.inf)
+    assert y[2] == 0 or (act == "silu" and math.isnan(y[2]))
+    assert abs(y[4]) <= 1e-40 and y[5] == (1.0 if act == "sigmoid" else 100.0) and y[3] > 0.7
+    z = values.repeat(m)[:, None].contiguous()
+    dx, _, _ = ops().linear_backward(torch.zeros_like(z), one, torch.ones_like(z), preact=z, activation=act)
+    d = dx[:6, 0].double().tolist()
+    assert math.isnan(d[0]) or act == "relu"
+    assert d[5] == (0.0 if act == "sigmoid" else 1.0) or abs(d[5]) < 1e-40
+    assert abs(d[4]) < 1e-40
