@@ -267,7 +267,7 @@ struct Product {
     float2* stats;            // [column blocks][stats_ld]
     int64_t stats_ld;
     float* label_logit;       // [M]
-    const float* lse;         // [M], in units of log2
+    const float2* norm;       // [M]: largest logit in units of log2, 1 / sum of the exponentials relative to it
 };
 
 // Column blocks that a kEpiStats product leaves statistics of; at most
@@ -318,8 +318,9 @@ void launch_dz(int64_t m, int64_t n, const void* z, int64_t ldz, int act, const 
 // out[i, j] = alpha * sum_p slab[p][i][j]; slab rows of ld floats
 void launch_slab_sum(int64_t rows, int64_t cols, const float* slab, int64_t ld, int pieces, void* out, int64_t ldo, float alpha,
                      const float* alpha_dev, const int32_t* targets, int64_t labels, int dtype, cudaStream_t s);
-// Joins the column blocks' statistics of m rows into lse (log2 units) and
-// row_loss; partial[block] = (sum of the labelled rows' losses, their number).
+// Joins the column blocks' statistics of m rows into norm (as in Product; not one
+// logarithm of the sum, whose rounding would be a common factor of a row's
+// probabilities: 4e-5 at logits of 1000) and row_loss; partial[block] = (sum of the labelled rows' losses, their number).
 struct JoinArgs {
     int64_t m, blocks;
     const float2* stats;
@@ -327,7 +328,7 @@ struct JoinArgs {
     const float* label_logit;
     const int32_t* targets;
     int64_t labels;
-    float* lse;
+    float2* norm;
     float* row_loss;
     double* partial;      // [join_blocks(m)][2]
 };

@@ -153,7 +153,8 @@ struct LossPlan {
     bool by_rows;                      // gradient pieces are rows of the table's full width, else columns
     int64_t chunk, ldg;
     Split sx, sw;                      // reductions of dx (over labels) and dw (over rows)
-    float *lse, *label_logit, *alpha;
+    float *label_logit, *alpha;
+    float2* norm;
     double* partial;
     float2* stats;
     // x's labelled rows and, when rows of d 16-bit elements are no multiple of 16
@@ -174,7 +175,7 @@ struct LossPlan {
         stats_rows = round_up(std::max<int64_t>(kStatsBytes / (8 * blocks), 1), 256);
         if (stats_rows > m) stats_rows = m;
         alpha = a.take<float>(1);
-        lse = a.take<float>(m);
+        norm = a.take<float2>(m);
         label_logit = a.take<float>(m);
         partial = a.take<double>(2 * ceil_div(m, stats_rows) * join_blocks(stats_rows));
         stats = a.take<float2>(blocks * stats_rows);
@@ -508,7 +509,7 @@ int msplat_loss_cross_entropy(int64_t m, int64_t v, int64_t d, const void* x, in
             j.stats = plan.stats; j.stats_ld = plan.stats_rows;
             j.label_logit = plan.label_logit + r0;
             j.targets = targets + r0; j.labels = v;
-            j.lse = plan.lse + r0;
+            j.norm = plan.norm + r0;
             j.row_loss = row_loss ? row_loss + r0 : nullptr;
             j.partial = plan.partial + 2 * joined;
             launch_join(j, s);
@@ -530,7 +531,7 @@ int msplat_loss_cross_entropy(int64_t m, int64_t v, int64_t d, const void* x, in
             p.targets = targets + r0;
             p.epi = kEpiGrad;
             p.col0 = l0;
-            p.lse = plan.lse + r0;
+            p.norm = plan.norm + r0;
             p.out = plan.g; p.ldo = plan.ldg; p.out_dtype = dtype;
             launch_product(p, s);
             if (dx) {

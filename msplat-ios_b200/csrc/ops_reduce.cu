@@ -185,9 +185,8 @@ __global__ void __launch_bounds__(1024) k_join(JoinArgs a, int shares) {
             const int32_t t = i < a.m ? a.targets[i] : -1;
             const bool has = t >= 0 && t < a.labels;
             if (i < a.m) {
-                const float lse = top + log2f(total);
-                const float row = has ? (lse - a.label_logit[i]) * kLn2 : 0.f;
-                a.lse[i] = lse;
+                const float row = has ? ((top - a.label_logit[i]) + log2f(total)) * kLn2 : 0.f;
+                a.norm[i] = make_float2(top, 1.f / total);
                 if (a.row_loss) a.row_loss[i] = row;
                 if (has) {
                     sum += row;

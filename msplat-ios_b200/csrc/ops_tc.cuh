@@ -393,7 +393,7 @@ struct RowState {
     int64_t i;
     bool in, zero;
     int32_t target;
-    float lse, top, sum, alpha;
+    float top, sum, alpha;  // (kEpiGrad: sum is the factor of the exponentials)
 };
 
 template <int EPI>
@@ -402,14 +402,17 @@ __device__ __forceinline__ RowState row_begin(const Product& p, int64_t i0, int 
     r.i = i0 + lane;
     r.in = r.i < p.M;
     r.target = -1;
-    r.lse = 0.f;
     r.top = -INFINITY;
     r.sum = 0.f;
     r.zero = false;
     r.alpha = p.alpha;
     if (EPI == kEpiStats || EPI == kEpiGrad) {
         if (r.in) r.target = __ldg(p.targets + r.i);
-        if (EPI == kEpiGrad && r.in) r.lse = __ldg(p.lse + r.i);
+        if (EPI == kEpiGrad && r.in) {
+            const float2 norm = __ldg(p.norm + r.i);
+            r.top = norm.x;
+            r.sum = norm.y * p.g_scale;
+        }
     }
     if (EPI == kEpiLinear) {
         if (p.alpha_dev) r.alpha *= __ldg(p.alpha_dev);
@@ -554,8 +557,7 @@ __device__ __forceinline__ bool columns32(const Product& p, const Tiles& tl, con
         const float to2 = p.logit_scale * kLog2e;
 #pragma unroll
         for (int q = 0; q < 32; ++q) {
-            v[q] = exp2_fast(__fmul_rn(v[q], to2) - r.lse);
-            if (sizeof(T) == 2) v[q] *= p.g_scale;
+            v[q] = exp2_fast(__fmul_rn(v[q], to2) - r.top) * r.sum;
         }
         const int64_t at = r.target - p.col0 - j0;
         if (__any_sync(~0u, at >= 0 && at < 32)) {

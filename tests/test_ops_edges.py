@@ -275,3 +275,19 @@ def test_activations_of_what_is_not_finite(act, m, t):
     assert math.isnan(d[0]) or act == "relu"
     assert d[5] == (0.0 if act == "sigmoid" else 1.0) or abs(d[5]) < 1e-40
     assert abs(d[4]) < 1e-40
+
+
+@pytest.mark.parametrize("m,v,d", [(300, 300, 40), (20_000, 200, 24), (40, 3000, 100), (9000, 100, 32)])
+@pytest.mark.parametrize("level", (1, 16, 64))
+def test_loss_gradients_of_a_row_sum_to_nothing(m, v, d, level):
+    """All embeddings have the same first column, so that logits of up to 4096 differ as those of the other columns do: softmax
+    minus one-hot sums to 0, and so does the first column of dx. Its terms are off by the exponential's 2 steps of 2^-23 and
+    their sum's few roundings; the product adds at most 188 times 16 of them, rounded towards zero (a step of a sum below 1,
+    the rest small): 2^-17 of the column's 64 in all."""
+    x, w = normal(240, m, d, "f32"), normal(241, v, d, "f32", std=d ** -0.5)
+    x[:, 0], w[:, 0] = float(level), 64.0
+    targets = labels(242, m, v, off=0.2)
+    count = int(((targets >= 0) & (targets < v)).sum())
+    _, _, dx, _ = ops().loss_cross_entropy(x, w, targets, weight=float(count))
+    assert float(dx[:, 0].abs().max()) <= 64 * 2.0 ** -17
+    assert float(dx.abs().max()) > 0.1
