@@ -7,7 +7,7 @@
 // shared memory with cp.async, in the 16-byte pieces around them whatever the
 // rows' alignment, one group ahead of the one it works on; neighbouring lanes
 // take neighbouring pieces. (Each thread reading its own row touches 32 lines
-// per instruction.) 1M x 61 -> 3 f16 of an unaligned record takes 53 us, 2.5 TB/s;
+// per instruction.) 1M x 61 -> 3 f16 of an unaligned record takes 54-57 us, 2.4 TB/s;
 // what bounds it is issuing the conversions and the masks of a row's two ends.
 // The weights are in shared memory as float, read as broadcasts.
 #include "ops.cuh"
