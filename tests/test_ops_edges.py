@@ -244,7 +244,8 @@ def test_inputs_freed_before_the_given_stream_has_read_them(op):
     sizes, at = [(t.shape, t.dtype) for t in held], {t.data_ptr() for t in held}
     del args, more, held
     again = [torch.empty(s, dtype=d, device="cuda") for s, d in sizes for _ in range(2)]
-    assert not side.query() and not at & {t.data_ptr() for t in again}
+    # (a host that took longer than the stream may have the memory back)
+    assert side.query() or not at & {t.data_ptr() for t in again}
     [t.fill_(-1) for t in again]
     torch.cuda.synchronize()
     want, got = ((v,) if isinstance(v, torch.Tensor) else v for v in (want, got))
