@@ -31,9 +31,9 @@
  * wider record is neither used nor written, but 16-byte pieces of it between the
  * first and the last element of a matrix may be read.
  *
- * Calls are asynchronous on `stream`, allocate no device memory, keep nothing between
- * calls (but what msplat_ops_status says) and may be captured into a CUDA graph. Sizes are at most 2^30. Working memory comes from the
- * caller: *_workspace gives its size in bytes, the pointer must be 256-byte
+ * Calls are asynchronous on `stream`, allocate no device memory, keep nothing
+ * between calls (but what msplat_ops_status says) and may be captured into a CUDA
+ * graph. Sizes are at most 2^30. Working memory comes from the caller: *_workspace gives its size in bytes, the pointer must be 256-byte
  * aligned, and two calls that may run at the same time (on two streams, or in
  * two graphs) need two of them. Results do not depend on the order in which
  * blocks run. Outputs must not overlap inputs or one another unless a comment

@@ -320,7 +320,8 @@ void launch_slab_sum(int64_t rows, int64_t cols, const float* slab, int64_t ld, 
                      const float* alpha_dev, const int32_t* targets, int64_t labels, int dtype, cudaStream_t s);
 // Joins the column blocks' statistics of m rows into norm (as in Product; not one
 // logarithm of the sum, whose rounding would be a common factor of a row's
-// probabilities: 4e-5 at logits of 1000) and row_loss; partial[block] = (sum of the labelled rows' losses, their number).
+// probabilities: 4e-5 at logits of 1000) and row_loss; partial[block] = (sum of the
+// labelled rows' losses, their number).
 struct JoinArgs {
     int64_t m, blocks;
     const float2* stats;

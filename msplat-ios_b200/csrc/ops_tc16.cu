@@ -11,9 +11,9 @@
 // operand is ever copied into another layout.
 //
 // 65536 x 1024 x 1024 bf16 takes 113 us without an activation (1216 TFLOP/s; the
-// library's product 102), 144 with GELU and a residual (176 at a sustained run's clocks),
-// whose ends then take as long as the products; 8192 x 32768 x 512 softmax statistics 183 (1500 TFLOP/s,
-// tensor pipe 85%). With a reduction of 64 the ends bound it: 65536 x 1024 in 54.
+// library's product 102), 144 with GELU and a residual (176 at a sustained run's
+// clocks), whose ends then take as long as the products; 8192 x 32768 x 512 softmax
+// statistics 183 (1500 TFLOP/s, tensor pipe 84%). With a reduction of 64 the ends bound it: 65536 x 1024 in 54.
 #include <cstddef>
 
 #include "ops_tc.cuh"
